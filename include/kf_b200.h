@@ -266,6 +266,45 @@ KF_API int kf_set_pdl(int mode);
  * No counterpart in the reference (its mbarrier waits spin without a bound: infer-opt/round12_lowp_stack/impl/attn16o.cu:77-79). */
 KF_API int kf_check_device_error(void);
 
+/* ---- Operators for training on packed images and clips ------------------------------------------------------------- */
+
+/* LayerNorm that keeps each row's statistics: x [rows, d] (row stride ldx elements; f32 | bf16 | f16) -> y [rows, d] contiguous
+ * (f32 | bf16 | f16), mean and rstd fp32 [rows].  w fp32 [d], b fp32 [d] or NULL.  d from 1 to 8192.
+ * Statistics and products in fp32; no counterpart kernel in the reference, whose training runs nn.LayerNorm
+ * (src/lightly_train/_models/dinov3/dinov3_src/models/vision_transformer.py:44). */
+KF_API int kf_layer_norm_fwd(int in_dtype, const void* x, int64_t ldx, const float* w, const float* b, float eps, int rows, int d, int out_dtype,
+                             void* y, float* mean, float* rstd, void* stream);
+
+/* Its gradient: dy [rows, d] (row stride lddy, 0 for one row repeated; the type of y), x, w, mean and rstd as in the forward ->
+ * dx [rows, d] contiguous in x's type, dw and db fp32 [d] (db may be NULL).  dres (NULL or [rows, d] in x's type, row stride ldres) is
+ * added to dx: the gradient that reaches the rows past the norm, as in a pre-norm residual block.
+ * ws: kf_layer_norm_ws_bytes(rows, d) bytes of device memory for the partial column sums (current device).  No atomics: the same bits
+ * on every run of one device type. */
+KF_API int64_t kf_layer_norm_ws_bytes(int64_t rows, int d);
+KF_API int kf_layer_norm_bwd(int in_dtype, const void* x, int64_t ldx, int dy_dtype, const void* dy, int64_t lddy, const float* w, const float* mean,
+                             const float* rstd, const void* dres, int64_t ldres, int rows, int d, void* dx, float* dw, float* db, void* ws,
+                             int64_t ws_bytes, void* stream);
+
+/* types of rotary positions */
+#define KF_POS_I32 0
+#define KF_POS_I64 1
+#define KF_POS_F32 2
+
+/* Rotary positions with several axes: x [G, T, H, D] -> y, the first 2P channels of every head turned by
+ * angle(t, p) = pos[t, axis[p]] * freq[p] * pi, the others copied.  Pair p: channels (p, p + P), or (2p, 2p + 1) with interleaved != 0.
+ * inverse != 0 turns by the negative angle, which is the gradient.  y may be x.  P <= 128, D <= 256.
+ * Counterpart of the turn itself: apply_rope (src/lightly_train/_models/dinov3/dinov3_src/layers/attention.py:23-34). */
+typedef struct kf_rope_params {
+  const void* x;         /* f32 | bf16 | f16, channels contiguous                                  */
+  void* y;               /* the same type and shape                                                 */
+  const void* pos;       /* KF_POS_* [T, axes], strides ps_t and ps_a                               */
+  const double* freq;    /* [P] half turns per unit of position: frequency in radians / pi          */
+  const int* axis;       /* [P] the column of pos that turns the pair                               */
+  int64_t xs_g, xs_t, xs_h, ys_g, ys_t, ys_h, ps_t, ps_a; /* strides in elements                    */
+  int dtype, pos_kind, G, T, H, D, P, interleaved, inverse;
+} kf_rope_params;
+KF_API int kf_rope_axes(const kf_rope_params* p, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -33,6 +33,13 @@ class GemmParams(C.Structure):
                 ("out_row_group", C.c_int), ("out_row_stride", C.c_int), ("out_row_offset", C.c_int), ("y_dbg", C.c_void_p), ("batch", C.c_int), ("a_rows_per_batch", C.c_int), ("w_rows_per_batch", C.c_int)]
 
 
+class RopeParams(C.Structure):
+    """mirror of kf_rope_params (include/kf_b200.h)."""
+    _fields_ = [("x", C.c_void_p), ("y", C.c_void_p), ("pos", C.c_void_p), ("freq", C.c_void_p), ("axis", C.c_void_p), ("xs_g", C.c_int64), ("xs_t", C.c_int64),
+                ("xs_h", C.c_int64), ("ys_g", C.c_int64), ("ys_t", C.c_int64), ("ys_h", C.c_int64), ("ps_t", C.c_int64), ("ps_a", C.c_int64), ("dtype", C.c_int),
+                ("pos_kind", C.c_int), ("G", C.c_int), ("T", C.c_int), ("H", C.c_int), ("D", C.c_int), ("P", C.c_int), ("interleaved", C.c_int), ("inverse", C.c_int)]
+
+
 _lib = None
 
 
@@ -57,6 +64,8 @@ def lib() -> C.CDLL:
         L.kf_sf_bytes.restype = C.c_int64
         L.kf_sf_bytes.argtypes = [C.c_int64, C.c_int64, C.c_int]
         vp, i32, i64, f32 = C.c_void_p, C.c_int, C.c_int64, C.c_float
+        L.kf_layer_norm_ws_bytes.restype = i64
+        L.kf_layer_norm_ws_bytes.argtypes = [i64, i32]
         sigs = {
             "kf_quant_rows": [i32, i32, vp, i64, i32, i32, vp, vp, i32, vp, vp, vp],
             "kf_ln_quant": [i32, vp, vp, vp, f32, i32, i32, vp, i32, vp, vp, vp, vp],
@@ -79,6 +88,9 @@ def lib() -> C.CDLL:
             "kf_patch_embed_static": [vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp],
             "kf_dw_ln": [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, f32, i32, vp],
             "kf_semantic": [vp, vp, i32, i32, i32, i32, vp, vp, vp],
+            "kf_layer_norm_fwd": [i32, vp, i64, vp, vp, f32, i32, i32, i32, vp, vp, vp, vp],
+            "kf_layer_norm_bwd": [i32, vp, i64, i32, vp, i64, vp, vp, vp, vp, i64, i32, i32, vp, vp, vp, vp, i64, vp],
+            "kf_rope_axes": [C.POINTER(RopeParams), vp],
             "kf_resize_norm": [vp, vp, i32, i32, i32, i32, C.POINTER(C.c_float), C.POINTER(C.c_float), vp],
         }
         for name, args in sigs.items():

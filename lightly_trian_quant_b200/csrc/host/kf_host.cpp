@@ -12,6 +12,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -644,6 +645,150 @@ PyObject* semantic(PyObject* const* v) {
   return t;
 }
 
+// ------------------------------------------------------------------------------------------------ operators for training
+// These run on the device their first tensor lives on, on torch's current stream of that device; the others have to live there too.
+void same_device(const at::Tensor& a, const at::Tensor& b, const char* op, const char* what) {
+  if (a.device() != b.device()) fail("%s: %s lives on another device than the first operand", op, what);
+}
+
+// x as rows of its last dimension: the stride between them.  A 2-D tensor may have any (0 repeats one row), others are contiguous.
+int64_t row_stride(const at::Tensor& x, const char* op, const char* what) {
+  const int64_t d = x.size(-1);
+  if (x.dim() == 2) {
+    if (d > 1 && x.stride(1) != 1) fail("%s: %s must have a contiguous last dimension", op, what);
+    return x.stride(0);
+  }
+  if (!x.is_contiguous()) fail("%s: %s must be contiguous (or two-dimensional with a contiguous last dimension)", op, what);
+  return d;
+}
+
+const at::Tensor& affine(PyObject* o, const at::Tensor& x, int64_t d, const char* op, const char* what) {
+  const at::Tensor& t = cuda_tensor(o, what);
+  if (t.scalar_type() != at::kFloat || !t.is_contiguous() || t.numel() != d) fail("%s: %s must be contiguous fp32 with %lld elements", op, what, (long long)d);
+  same_device(x, t, op, what);
+  return t;
+}
+
+// rows and width of x as the kernels take them
+void norm_shape(const at::Tensor& x, const char* op, int64_t* rows, int64_t* d) {
+  if (x.dim() < 1 || x.size(-1) < 1 || x.size(-1) > 8192) fail("%s: x must be [..., d] with d from 1 to 8192", op);
+  if (dtype_code(x.scalar_type()) < 0) fail("%s: unsupported dtype %s", op, c10::toString(x.scalar_type()));
+  *d = x.size(-1);
+  *rows = x.numel() / *d;
+  if (*rows > INT32_MAX) fail("%s: %lld rows are more than a call takes", op, (long long)*rows);
+}
+
+PyObject* tuple3(at::Tensor a, at::Tensor b, PyObject* c) {
+  PyObject* t = PyTuple_New(3);
+  PyTuple_SET_ITEM(t, 0, THPVariable_Wrap(std::move(a)));
+  PyTuple_SET_ITEM(t, 1, THPVariable_Wrap(std::move(b)));
+  PyTuple_SET_ITEM(t, 2, c);
+  return t;
+}
+
+// x, w, b | None, eps, out dtype code (-1: that of x)
+PyObject* layer_norm_fwd(PyObject* const* v) {
+  const char* const op = "layer_norm_fwd";
+  const at::Tensor& x = cuda_tensor(v[0], "x");
+  int64_t rows, d;
+  norm_shape(x, op, &rows, &d);
+  const int64_t ldx = row_stride(x, op, "x");
+  const float* w = affine(v[1], x, d, op, "w").data_ptr<float>();
+  const float* b = v[2] == Py_None ? nullptr : affine(v[2], x, d, op, "b").data_ptr<float>();
+  const float eps = (float)to_float(v[3]);
+  const int in = dtype_code(x.scalar_type()), asked = (int)to_int(v[4]), out = asked < 0 ? in : asked;
+  const c10::cuda::CUDAGuard guard(x.device());
+  at::Tensor y = empty(x.sizes(), dtype_of(out), x.device()), mean = empty({rows}, at::kFloat, x.device()), rstd = empty({rows}, at::kFloat, x.device());
+  launch(op, kf_layer_norm_fwd, in, (const void*)x.data_ptr(), ldx, w, b, eps, (int)rows, (int)d, out, y.data_ptr(), mean.data_ptr<float>(), rstd.data_ptr<float>(), stream());
+  return tuple3(std::move(y), std::move(mean), THPVariable_Wrap(std::move(rstd)));
+}
+
+// dy, x, w, mean, rstd, dres | None, want db
+PyObject* layer_norm_bwd(PyObject* const* v) {
+  const char* const op = "layer_norm_bwd";
+  const at::Tensor &dy = cuda_tensor(v[0], "dy"), &x = cuda_tensor(v[1], "x");
+  int64_t rows, d;
+  norm_shape(x, op, &rows, &d);
+  need(dy.sizes() == x.sizes() && dtype_code(dy.scalar_type()) >= 0, "layer_norm_bwd: dy must be f32, bf16 or f16 of the shape of x");
+  same_device(x, dy, op, "dy");
+  const int64_t ldx = row_stride(x, op, "x"), lddy = row_stride(dy, op, "dy");
+  const float* w = affine(v[2], x, d, op, "w").data_ptr<float>();
+  const float *mean = affine(v[3], x, rows, op, "mean").data_ptr<float>(), *rstd = affine(v[4], x, rows, op, "rstd").data_ptr<float>();
+  const void* dres = nullptr;
+  int64_t ldres = 0;
+  if (v[5] != Py_None) {
+    const at::Tensor& r = cuda_tensor(v[5], "dres");
+    need(r.sizes() == x.sizes() && r.scalar_type() == x.scalar_type(), "layer_norm_bwd: dres must have the shape and type of x");
+    same_device(x, r, op, "dres");
+    ldres = row_stride(r, op, "dres");
+    dres = r.data_ptr();
+  }
+  const bool want_db = truth(v[6]);
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int64_t bytes = kf_layer_norm_ws_bytes(rows, (int)d);
+  if (bytes < 0) check((int)bytes, "kf_layer_norm_ws_bytes");
+  at::Tensor dx = empty(x.sizes(), x.scalar_type(), x.device()), dw = empty({d}, at::kFloat, x.device()), db, ws = empty({bytes / 4}, at::kFloat, x.device());
+  if (want_db) db = empty({d}, at::kFloat, x.device());
+  launch(op, kf_layer_norm_bwd, dtype_code(x.scalar_type()), (const void*)x.data_ptr(), ldx, dtype_code(dy.scalar_type()), (const void*)dy.data_ptr(), lddy, w, mean, rstd, dres, ldres,
+         (int)rows, (int)d, dx.data_ptr(), dw.data_ptr<float>(), want_db ? db.data_ptr<float>() : nullptr, ws.data_ptr(), bytes, stream());
+  return tuple3(std::move(dx), std::move(dw), want_db ? THPVariable_Wrap(std::move(db)) : new_ref(Py_None));
+}
+
+// [T, H, D] or [G, T, H, D], channels contiguous
+struct Heads {
+  int64_t g, t, h, d, sg, st, sh;
+};
+Heads heads_of(const at::Tensor& x, const char* op, const char* what) {
+  if ((x.dim() != 3 && x.dim() != 4) || (x.size(-1) > 1 && x.stride(-1) != 1)) fail("%s: %s must be [T, H, D] or [G, T, H, D] with contiguous channels", op, what);
+  const int o = (int)x.dim() - 3;
+  return {o ? x.size(0) : 1, x.size(o), x.size(o + 1), x.size(o + 2), o ? x.stride(0) : 0, x.stride(o), x.stride(o + 1)};
+}
+
+// x, pos, freq (fp64 [P]), axis (int32 [P]), axes, head channels, interleaved, inverse, out | None
+PyObject* rope_axes(PyObject* const* v) {
+  const char* const op = "rope_axes";
+  const at::Tensor &x = cuda_tensor(v[0], "x"), &pos = cuda_tensor(v[1], "pos"), &freq = cuda_tensor(v[2], "freq"), &axis = cuda_tensor(v[3], "axis");
+  const Heads s = heads_of(x, op, "x");
+  const int64_t axes = to_int(v[4]), D = to_int(v[5]);
+  if (dtype_code(x.scalar_type()) < 0) fail("%s: unsupported dtype %s", op, c10::toString(x.scalar_type()));
+  if (s.d != D) fail("%s: the table is for %lld channels per head, x has %lld", op, (long long)D, (long long)s.d);
+  if (pos.dim() != 2 || pos.size(0) != s.t || pos.size(1) != axes)
+    fail("%s: pos must be [T=%lld, axes=%lld]", op, (long long)s.t, (long long)axes);
+  const at::ScalarType pt = pos.scalar_type();
+  need(pt == at::kInt || pt == at::kLong || pt == at::kFloat, "rope_axes: pos must be int32, int64 or fp32");
+  if (s.g > INT32_MAX || s.t > INT32_MAX || s.h > INT32_MAX) fail("%s: shape does not fit 32-bit sizes", op);
+  for (int i = 0; i < 3; ++i)
+    if (x.device() != (i == 0 ? pos : i == 1 ? freq : axis).device()) fail("%s: pos and the table must live on the device of x", op);
+  const c10::cuda::CUDAGuard guard(x.device());
+  at::Tensor out;
+  if (v[8] == Py_None) {
+    out = empty(x.sizes(), x.scalar_type(), x.device());
+  } else {
+    out = cuda_tensor(v[8], "out");
+    need(out.sizes() == x.sizes() && out.scalar_type() == x.scalar_type(), "rope_axes: out must have the shape and type of x");
+    same_device(x, out, op, "out");
+  }
+  const Heads o = heads_of(out, op, "out");
+  if (v[8] != Py_None) {
+    need((o.sg != 0 || o.g < 2) && (o.st != 0 || o.t < 2) && (o.sh != 0 || o.h < 2), "rope_axes: out must not be an expanded tensor");
+    writable(out);
+  }
+  kf_rope_params p = {};
+  p.x = x.data_ptr();
+  p.y = out.data_ptr();
+  p.pos = pos.data_ptr();
+  p.freq = freq.data_ptr<double>();
+  p.axis = axis.data_ptr<int>();
+  p.xs_g = s.sg; p.xs_t = s.st; p.xs_h = s.sh; p.ys_g = o.sg; p.ys_t = o.st; p.ys_h = o.sh; p.ps_t = pos.stride(0); p.ps_a = pos.stride(1);
+  p.dtype = dtype_code(x.scalar_type());
+  p.pos_kind = pt == at::kInt ? KF_POS_I32 : pt == at::kLong ? KF_POS_I64 : KF_POS_F32;
+  p.G = (int)s.g; p.T = (int)s.t; p.H = (int)s.h; p.D = (int)s.d; p.P = (int)freq.numel();
+  p.interleaved = truth(v[6]);
+  p.inverse = truth(v[7]);
+  launch(op, kf_rope_axes, (const kf_rope_params*)&p, stream());
+  return v[8] == Py_None ? THPVariable_Wrap(std::move(out)) : new_ref(v[8]);
+}
+
 // a weight: does the next GEMM with it read it ahead of its predecessor's end?
 PyObject* reads_weight_early(PyObject* const* v) {
   const Ref q = attr(v[0], s_q), sf = attr(v[0], s_sf);
@@ -679,6 +824,7 @@ PyMethodDef g_methods[] = {KF_ENTRY(quant_rows, 4),     KF_ENTRY(ln_quant, 7),  
                            KF_ENTRY(qkv_rope, 10),      KF_ENTRY(gemm_gelu_q, 6), KF_ENTRY(bmm_nt, 3),   KF_ENTRY(gemm_tokens, 8),    KF_ENTRY(broadcast_rows, 3),
                            KF_ENTRY(ln_tail, 8),        KF_ENTRY(attn_fwd, 3),   KF_ENTRY(attn_fwd_quant, 4), KF_ENTRY(im2col_patch16, 1), KF_ENTRY(dw_ln, 10),
                            KF_ENTRY(semantic, 3),       KF_ENTRY(amax_scale, 5), KF_ENTRY(ln_amax_scale, 7),
+                           KF_ENTRY(layer_norm_fwd, 5), KF_ENTRY(layer_norm_bwd, 7), KF_ENTRY(rope_axes, 9),
                            KF_ENTRY(reads_weight_early, 1), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_kf_host", "native operator layer over libkf_b200.so", -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

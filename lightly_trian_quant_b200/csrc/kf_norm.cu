@@ -1,0 +1,381 @@
+// LayerNorm for training: forward that keeps each row's statistics, and the gradients of rows, weight and bias.
+//
+//   y  = xh * w + b,  xh = (x - mean) * rstd
+//   g  = dy * w;  dx = rstd * (g - mean(g) - xh * mean(g * xh)) (+ dres);  dw = sum over rows of dy * xh;  db = sum over rows of dy
+//
+// A row belongs to a group of W warps (1, 2, 4 or 8 of a CTA's 8), its values stay in registers between the statistics and their use: one
+// pass over memory in either direction.  Chunks of 8 values where width, strides and addresses allow 16-byte accesses, single values
+// otherwise.  Statistics, sums and products in fp32 whatever the tensors' types.
+// The weight's gradient is summed in registers over the rows of a group, over the groups of a CTA through shared memory in their order, and
+// over the CTAs by a second launch: no atomics, the same bits from run to run.
+#include "kf_common.cuh"
+
+namespace kf {
+
+constexpr int LN_THREADS = 256, LN_WARPS = 8, LN_MAX_WIDTH = 8192;
+
+template <typename T>
+__device__ __forceinline__ float ln_to_float(T v) { return static_cast<float>(v); }
+template <typename T>
+__device__ __forceinline__ uint32_t ln_pack2(float a, float b) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+template <typename T>
+__device__ __forceinline__ float2 ln_unpack2(uint32_t w) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+  else return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
+template <int CH, typename T>
+__device__ __forceinline__ void ln_load(const T* p, float (&v)[CH]) {
+  if constexpr (CH == 1) {
+    v[0] = ln_to_float(__ldg(p));
+  } else if constexpr (sizeof(T) == 4) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  } else {
+    const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = ln_unpack2<T>(w[i]);
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+  }
+}
+template <int CH, typename T>
+__device__ __forceinline__ void ln_store(T* p, const float (&v)[CH]) {
+  if constexpr (CH == 1) {
+    *p = static_cast<T>(v[0]);
+  } else if constexpr (sizeof(T) == 4) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+  } else {
+    *reinterpret_cast<uint4*>(p) = make_uint4(ln_pack2<T>(v[0], v[1]), ln_pack2<T>(v[2], v[3]), ln_pack2<T>(v[4], v[5]), ln_pack2<T>(v[6], v[7]));
+  }
+}
+
+// The sum of a value over the W warps of a group; `red` has a slot per warp of the CTA.  Two calls in a row use different slots.
+__device__ __forceinline__ float2 ln_group_sum(float2 s, int W, int group, int warp, int lane, float2* red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    s.x += __shfl_xor_sync(0xffffffffu, s.x, o);
+    s.y += __shfl_xor_sync(0xffffffffu, s.y, o);
+  }
+  if (W > 1) {
+    if (lane == 0) red[warp] = s;
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(W * 32) : "memory");
+    s = red[group * W];
+    for (int i = 1; i < W; ++i) {
+      const float2 o = red[group * W + i];
+      s.x += o.x;
+      s.y += o.y;
+    }
+  }
+  return s;
+}
+
+struct LnArgs {
+  const void *x, *dy, *dres;
+  const float *w, *b;
+  float *mean, *rstd;
+  void *y, *dx;
+  float* part;                       // backward: [gridDim.x][2][d]
+  int64_t ldx, lddy, ldres;
+  int rows, d, W;
+  float eps, inv_d;
+};
+
+template <typename TI, typename TO, int CH, int NC>
+__global__ void __launch_bounds__(LN_THREADS) layer_norm_fwd_kernel(const __grid_constant__ LnArgs a) {
+  __shared__ float2 red[2][LN_WARPS];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int group = warp / a.W, groups = LN_WARPS / a.W, t = (warp - group * a.W) * 32 + lane, step = a.W * 32;
+  pdl_wait();
+  for (int64_t row = (int64_t)blockIdx.x * groups + group; row < a.rows; row += (int64_t)gridDim.x * groups) {
+    const TI* x = static_cast<const TI*>(a.x) + row * a.ldx;
+    float v[NC][CH];
+    float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = (t + i * step) * CH;
+      if (c < a.d) {
+        ln_load<CH>(x + c, v[i]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < CH; ++j) v[i][j] = 0.f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+#pragma unroll
+      for (int j = 0; j < CH; ++j) s.x += v[i][j];
+    const float mean = ln_group_sum(s, a.W, group, warp, lane, red[0]).x * a.inv_d;
+    s.x = 0.f;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const bool in = (t + i * step) * CH < a.d;
+#pragma unroll
+      for (int j = 0; j < CH; ++j) {
+        v[i][j] = in ? v[i][j] - mean : 0.f;
+        s.x = fmaf(v[i][j], v[i][j], s.x);
+      }
+    }
+    const float rstd = rsqrtf(ln_group_sum(s, a.W, group, warp, lane, red[1]).x * a.inv_d + a.eps);
+    TO* y = static_cast<TO*>(a.y) + row * a.d;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = (t + i * step) * CH;
+      if (c < a.d) {
+        float w[CH], b[CH];
+        ln_load<CH>(a.w + c, w);
+        if (a.b) {
+          ln_load<CH>(a.b + c, b);
+        } else {
+#pragma unroll
+          for (int j = 0; j < CH; ++j) b[j] = 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < CH; ++j) v[i][j] = fmaf(v[i][j] * rstd, w[j], b[j]);
+        ln_store<CH>(y + c, v[i]);
+      }
+    }
+    if (t == 0) {
+      a.mean[row] = mean;
+      a.rstd[row] = rstd;
+    }
+  }
+}
+
+template <typename TI, typename TO, int CH, int NC>
+__global__ void __launch_bounds__(LN_THREADS) layer_norm_bwd_kernel(const __grid_constant__ LnArgs a) {
+  extern __shared__ float colsum[];  // [2][d], where a CTA has more than one group
+  __shared__ float2 red[2][LN_WARPS];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int group = warp / a.W, groups = LN_WARPS / a.W, t = (warp - group * a.W) * 32 + lane, step = a.W * 32;
+  pdl_wait();
+  float w[NC][CH], aw[NC][CH], ab[NC][CH];
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    const int c = (t + i * step) * CH;
+    if (c < a.d) {
+      ln_load<CH>(a.w + c, w[i]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < CH; ++j) w[i][j] = 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < CH; ++j) aw[i][j] = ab[i][j] = 0.f;
+  }
+  int turn = 0;
+  for (int64_t row = (int64_t)blockIdx.x * groups + group; row < a.rows; row += (int64_t)gridDim.x * groups, turn ^= 1) {
+    const TI* x = static_cast<const TI*>(a.x) + row * a.ldx;
+    const TO* dy = static_cast<const TO*>(a.dy) + row * a.lddy;
+    const float mean = __ldg(a.mean + row), rstd = __ldg(a.rstd + row);
+    float xh[NC][CH], g[NC][CH];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = (t + i * step) * CH;
+      if (c < a.d) {
+        ln_load<CH>(x + c, xh[i]);
+        ln_load<CH>(dy + c, g[i]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < CH; ++j) {
+          xh[i][j] = mean;
+          g[i][j] = 0.f;
+        }
+      }
+    }
+    float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+#pragma unroll
+      for (int j = 0; j < CH; ++j) {
+        xh[i][j] = (xh[i][j] - mean) * rstd;
+        aw[i][j] = fmaf(g[i][j], xh[i][j], aw[i][j]);
+        ab[i][j] += g[i][j];
+        g[i][j] *= w[i][j];
+        s.x += g[i][j];
+        s.y = fmaf(g[i][j], xh[i][j], s.y);
+      }
+    s = ln_group_sum(s, a.W, group, warp, lane, red[turn]);
+    const float m1 = s.x * a.inv_d, m2 = s.y * a.inv_d;
+    TI* dx = static_cast<TI*>(a.dx) + row * a.d;
+    const TI* dres = a.dres ? static_cast<const TI*>(a.dres) + row * a.ldres : nullptr;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = (t + i * step) * CH;
+      if (c < a.d) {
+        float r[CH];
+#pragma unroll
+        for (int j = 0; j < CH; ++j) r[j] = 0.f;
+        if (dres) ln_load<CH>(dres + c, r);
+#pragma unroll
+        for (int j = 0; j < CH; ++j) r[j] = fmaf(rstd, g[i][j] - m1 - xh[i][j] * m2, r[j]);
+        ln_store<CH>(dx + c, r);
+      }
+    }
+  }
+  // the groups of this CTA, in their order; then the CTA's line of the partial sums
+  float* part = a.part + (size_t)blockIdx.x * 2 * a.d;
+  for (int k = 0; k < groups; ++k) {
+    if (group == k) {
+      float* to = k == groups - 1 ? part : colsum;
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        const int c = (t + i * step) * CH;
+        if (c < a.d) {
+#pragma unroll
+          for (int j = 0; j < CH; ++j) {
+            to[c + j] = k ? colsum[c + j] + aw[i][j] : aw[i][j];
+            to[a.d + c + j] = k ? colsum[a.d + c + j] + ab[i][j] : ab[i][j];
+          }
+        }
+      }
+    }
+    if (groups > 1) __syncthreads();
+  }
+}
+
+// dw, db = the sum of `n` lines [2][d]: 32 columns per CTA, 8 threads per column
+__global__ void __launch_bounds__(256) layer_norm_cols_kernel(const float* __restrict__ part, int n, int d, float* __restrict__ dw, float* __restrict__ db) {
+  __shared__ float sm[8][33];
+  pdl_wait();
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int64_t c = (int64_t)blockIdx.x * 32 + tx;
+  float s = 0.f;
+  if (c < 2 * (int64_t)d) {
+#pragma unroll 4
+    for (int i = ty; i < n; i += 8) s += part[(size_t)i * 2 * d + c];
+  }
+  sm[ty][tx] = s;
+  __syncthreads();
+  if (ty == 0 && c < 2 * (int64_t)d) {
+#pragma unroll
+    for (int k = 1; k < 8; ++k) s += sm[k][tx];
+    if (c < d) dw[c] = s;
+    else if (db) db[c - d] = s;
+  }
+}
+
+// warps per row: at most 32 values per thread
+static int ln_warps(int d) { return d <= 1024 ? 1 : d <= 2048 ? 2 : d <= 4096 ? 4 : 8; }
+
+static int ln_grid(int64_t rows, int d, int per_sm, int* grid) {
+  int sms = 0;
+  const int rc = device_sm_count(&sms);
+  if (rc != KF_OK) return rc;
+  const int groups = LN_WARPS / ln_warps(d);
+  const int64_t blocks = (rows + groups - 1) / groups, most = (int64_t)sms * per_sm;
+  *grid = (int)(blocks < most ? blocks : most);
+  return KF_OK;
+}
+constexpr int LN_FWD_PER_SM = 8, LN_BWD_PER_SM = 2;
+
+// f(TI, TO, CH, NC) for the types, the access width and the values per thread of a call
+template <typename TI, typename TO, typename F>
+static int ln_by_width(bool wide, int d, F&& f) {
+  const int lanes = ln_warps(d) * 32;
+  if (wide) {
+    const int n = (d / 8 + lanes - 1) / lanes;
+    if (n <= 1) return f(TI{}, TO{}, std::integral_constant<int, 8>{}, std::integral_constant<int, 1>{});
+    if (n <= 2) return f(TI{}, TO{}, std::integral_constant<int, 8>{}, std::integral_constant<int, 2>{});
+    if (n <= 3) return f(TI{}, TO{}, std::integral_constant<int, 8>{}, std::integral_constant<int, 3>{});
+    return f(TI{}, TO{}, std::integral_constant<int, 8>{}, std::integral_constant<int, 4>{});
+  }
+  const int n = (d + lanes - 1) / lanes;
+  if (n <= 4) return f(TI{}, TO{}, std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{});
+  if (n <= 12) return f(TI{}, TO{}, std::integral_constant<int, 1>{}, std::integral_constant<int, 12>{});
+  return f(TI{}, TO{}, std::integral_constant<int, 1>{}, std::integral_constant<int, 32>{});
+}
+template <typename TI, typename F>
+static int ln_by_out(int out_dtype, bool wide, int d, F&& f) {
+  if (out_dtype == KF_F32) return ln_by_width<TI, float>(wide, d, f);
+  if (out_dtype == KF_BF16) return ln_by_width<TI, __nv_bfloat16>(wide, d, f);
+  return ln_by_width<TI, __half>(wide, d, f);
+}
+template <typename F>
+static int ln_by_type(int in_dtype, int out_dtype, bool wide, int d, F&& f) {
+  if (in_dtype == KF_F32) return ln_by_out<float>(out_dtype, wide, d, f);
+  if (in_dtype == KF_BF16) return ln_by_out<__nv_bfloat16>(out_dtype, wide, d, f);
+  return ln_by_out<__half>(out_dtype, wide, d, f);
+}
+
+static bool ln_aligned(const void* p, int64_t pitch_bytes) { return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)pitch_bytes) & 15) == 0; }
+static int64_t ln_size(int dtype) { return dtype == KF_F32 ? 4 : 2; }
+static bool ln_float_type(int dtype) { return dtype == KF_F32 || dtype == KF_BF16 || dtype == KF_F16; }
+
+}  // namespace kf
+
+using namespace kf;
+
+extern "C" int64_t kf_layer_norm_ws_bytes(int64_t rows, int d) {
+  if (rows < 0 || d <= 0 || d > LN_MAX_WIDTH) {
+    set_error("kf_layer_norm_ws_bytes: bad argument rows=%lld d=%d", (long long)rows, d);
+    return KF_ERR_BAD_ARGUMENT;
+  }
+  int grid = 0;
+  const int rc = ln_grid(rows, d, LN_BWD_PER_SM, &grid);
+  if (rc != KF_OK) return rc > 0 ? KF_ERR_UNSUPPORTED : rc;
+  return (int64_t)grid * 2 * d * 4;
+}
+
+extern "C" int kf_layer_norm_fwd(int in_dtype, const void* x, int64_t ldx, const float* w, const float* b, float eps, int rows, int d, int out_dtype, void* y,
+                                 float* mean, float* rstd, void* stream) {
+  KF_REQUIRE(ln_float_type(in_dtype) && ln_float_type(out_dtype), "kf_layer_norm_fwd: types must be f32, bf16 or f16");
+  KF_REQUIRE(rows >= 0 && d > 0 && d <= LN_MAX_WIDTH && ldx >= 0, "kf_layer_norm_fwd: bad shape rows=%d d=%d (at most %d wide)", rows, d, LN_MAX_WIDTH);
+  if (rows == 0) return KF_OK;
+  KF_REQUIRE(x && w && y && mean && rstd, "kf_layer_norm_fwd: null pointer");
+  LnArgs a{};
+  a.x = x; a.ldx = ldx; a.w = w; a.b = b; a.mean = mean; a.rstd = rstd; a.y = y; a.rows = rows; a.d = d; a.W = ln_warps(d); a.eps = eps; a.inv_d = 1.0f / (float)d;
+  const bool wide = d % 8 == 0 && ln_aligned(x, ldx * ln_size(in_dtype)) && ln_aligned(y, 0) && ln_aligned(w, 0) && ln_aligned(b, 0);
+  int grid = 0;
+  const int rc = ln_grid(rows, d, LN_FWD_PER_SM, &grid);
+  if (rc != KF_OK) return rc;
+  return ln_by_type(in_dtype, out_dtype, wide, d, [&](auto ti, auto to, auto ch, auto nc) {
+    return cuda_status(launch_maybe_pdl(rows, layer_norm_fwd_kernel<decltype(ti), decltype(to), decltype(ch)::value, decltype(nc)::value>, dim3(grid), dim3(LN_THREADS), 0,
+                                        static_cast<cudaStream_t>(stream), a),
+                       "kf_layer_norm_fwd launch");
+  });
+}
+
+extern "C" int kf_layer_norm_bwd(int in_dtype, const void* x, int64_t ldx, int dy_dtype, const void* dy, int64_t lddy, const float* w, const float* mean,
+                                 const float* rstd, const void* dres, int64_t ldres, int rows, int d, void* dx, float* dw, float* db, void* ws, int64_t ws_bytes,
+                                 void* stream) {
+  KF_REQUIRE(ln_float_type(in_dtype) && ln_float_type(dy_dtype), "kf_layer_norm_bwd: types must be f32, bf16 or f16");
+  KF_REQUIRE(rows >= 0 && d > 0 && d <= LN_MAX_WIDTH && ldx >= 0 && lddy >= 0 && ldres >= 0, "kf_layer_norm_bwd: bad shape rows=%d d=%d (at most %d wide)", rows, d,
+             LN_MAX_WIDTH);
+  KF_REQUIRE(w && dw, "kf_layer_norm_bwd: null pointer");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (rows == 0) {
+    cudaError_t e = cudaMemsetAsync(dw, 0, (size_t)d * 4, st);
+    if (e == cudaSuccess && db) e = cudaMemsetAsync(db, 0, (size_t)d * 4, st);
+    return cuda_status(e, "kf_layer_norm_bwd memset");
+  }
+  KF_REQUIRE(x && dy && mean && rstd && dx && ws, "kf_layer_norm_bwd: null pointer");
+  int grid = 0;
+  int rc = ln_grid(rows, d, LN_BWD_PER_SM, &grid);
+  if (rc != KF_OK) return rc;
+  KF_REQUIRE(ws_bytes >= (int64_t)grid * 2 * d * 4, "kf_layer_norm_bwd: workspace of %lld bytes, needs %lld", (long long)ws_bytes, (long long)grid * 2 * d * 4);
+  LnArgs a{};
+  a.x = x; a.ldx = ldx; a.dy = dy; a.lddy = lddy; a.dres = dres; a.ldres = ldres; a.w = w; a.mean = const_cast<float*>(mean); a.rstd = const_cast<float*>(rstd);
+  a.dx = dx; a.part = static_cast<float*>(ws); a.rows = rows; a.d = d; a.W = ln_warps(d); a.inv_d = 1.0f / (float)d;
+  const bool wide = d % 8 == 0 && ln_aligned(x, ldx * ln_size(in_dtype)) && ln_aligned(dy, lddy * ln_size(dy_dtype)) && ln_aligned(dres, ldres * ln_size(in_dtype)) &&
+                    ln_aligned(dx, 0) && ln_aligned(w, 0);
+  const size_t smem = a.W < LN_WARPS ? (size_t)2 * d * 4 : 0;
+  rc = ln_by_type(in_dtype, dy_dtype, wide, d, [&](auto ti, auto to, auto ch, auto nc) {
+    return cuda_status(launch_maybe_pdl(rows, layer_norm_bwd_kernel<decltype(ti), decltype(to), decltype(ch)::value, decltype(nc)::value>, dim3(grid), dim3(LN_THREADS), smem, st, a),
+                       "kf_layer_norm_bwd launch");
+  });
+  if (rc != KF_OK) return rc;
+  return cuda_status(launch_maybe_pdl(rows, layer_norm_cols_kernel, dim3((2 * d + 31) / 32), dim3(256), 0, st, static_cast<const float*>(ws), grid, d, dw, db),
+                     "kf_layer_norm_bwd column sums launch");
+}

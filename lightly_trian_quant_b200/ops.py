@@ -347,6 +347,66 @@ def attn_fwd_quant(qkv: torch.Tensor, out: ActBuf, pre: float = 1.0, recip_div: 
     return _h.attn_fwd_quant(*args) if TIMING is None else _timed("attn_fwd", _h.attn_fwd_quant, args)
 
 
+# ------------------------------------------------------------------------------------------------ training on packed images and clips
+# These run on the device of their operands, on torch's current stream there.  Each takes its gradient as an operator of its own; grad.py makes
+# differentiable functions of them.
+def layer_norm_fwd(x: torch.Tensor, w: torch.Tensor, b: Optional[torch.Tensor], eps: float, dtype: Optional[torch.dtype] = None):
+    """LayerNorm over the last dimension of x [..., d] (f32 | bf16 | f16, d from 1 to 8192; contiguous, or two-dimensional with any row
+    stride) -> (y in dtype (x's own by default), mean fp32 [rows], rstd fp32 [rows]).  w, b: fp32 [d], b may be None."""
+    global LAUNCHES
+    LAUNCHES += 1
+    args = (x, w, b, eps, -1 if dtype is None else _DT[dtype])
+    return _h.layer_norm_fwd(*args) if TIMING is None else _timed("layer_norm_fwd", _h.layer_norm_fwd, args)
+
+
+def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, *, dres: Optional[torch.Tensor] = None,
+                   bias: bool = True):
+    """Gradients of layer_norm_fwd -> (dx in x's type, dw fp32 [d], db fp32 [d] or None with bias=False).  dres (shape and type of x) is added to
+    dx: the gradient that goes past the norm in a residual block.  No atomics: the same bits from run to run."""
+    global LAUNCHES
+    LAUNCHES += 2
+    args = (dy, x, w, mean, rstd, dres, bias)
+    return _h.layer_norm_bwd(*args) if TIMING is None else _timed("layer_norm_bwd", _h.layer_norm_bwd, args)
+
+
+class RopeTable:
+    """Which channels of a head are turned by which position, and how fast: freqs[a] lists the frequencies (radians per unit of position) of the
+    pairs that axis a turns, axis by axis.  With P pairs in all, pair p is channels (p, p + P) of the head, or (2p, 2p + 1) with interleaved=True;
+    channels 2P .. head_dim - 1 pass through.  The backbone's tables (half layout, 2 * pi / periods for rows and for columns) are
+    RopeTable([f, f], 64) with f = 2 * pi / rope_embed.periods."""
+
+    __slots__ = ("head_dim", "axes", "interleaved", "freq", "axis")
+
+    def __init__(self, freqs, head_dim: int, *, interleaved: bool = False, device="cuda"):
+        import math
+
+        flat = [float(f) for fs in freqs for f in fs]
+        if not 1 <= head_dim <= 256 or 2 * len(flat) > head_dim:
+            raise KfError(f"RopeTable: {len(flat)} pairs do not fit {head_dim} channels (256 at most)")
+        if not all(math.isfinite(f) for f in flat):
+            raise KfError("RopeTable: frequencies must be finite")
+        self.head_dim, self.axes, self.interleaved = int(head_dim), len(freqs), bool(interleaved)
+        self.freq = torch.tensor([f / math.pi for f in flat], dtype=torch.float64, device=device)
+        self.axis = torch.tensor([a for a, fs in enumerate(freqs) for _ in fs], dtype=torch.int32, device=device)
+
+    @classmethod
+    def geometric(cls, channels, head_dim: int, *, base: float = 10000.0, **kw) -> "RopeTable":
+        """channels[a] channels for axis a with frequencies base^(-2i / channels[a])."""
+        if any(n < 0 or n % 2 for n in channels):
+            raise KfError(f"RopeTable: channels per axis must be even, got {list(channels)}")
+        return cls([[base ** (-2.0 * i / n) for i in range(n // 2)] for n in channels], head_dim, **kw)
+
+
+def rope_axes(x: torch.Tensor, pos: torch.Tensor, table: RopeTable, *, inverse: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """x [T, H, D] or [G, T, H, D] (f32 | bf16 | f16, channels contiguous, any other strides) with every head turned by its token's positions
+    pos [T, axes] (int32 | int64 | fp32).  inverse=True turns back, which is also the gradient.  out may be x.  Tokens that are not to be turned
+    (cls, registers, queries) have position 0.  Angles are exact to fp32 however far the position."""
+    global LAUNCHES
+    LAUNCHES += 1
+    args = (x, pos, table.freq, table.axis, table.axes, table.head_dim, table.interleaved, inverse, out)
+    return _h.rope_axes(*args) if TIMING is None else _timed("rope_axes", _h.rope_axes, args)
+
+
 # ------------------------------------------------------------------------------------------------ patch embed / head / pre / post
 def gemm_tokens(a: torch.Tensor, W: QWeight, bias, out: torch.Tensor, rows_per_image: int, tokens_per_image: int, row_offset: int,
                 round_bf16: bool = False) -> torch.Tensor:
