@@ -305,6 +305,47 @@ typedef struct kf_rope_params {
 } kf_rope_params;
 KF_API int kf_rope_axes(const kf_rope_params* p, void* stream);
 
+/* Attention over packed sequences with a tanh cap, a bias by distance, document and prefix masks; head dimension 64, bf16 | f16.
+ *
+ * Sequences lie behind one another in the rows of q (Tq rows) and of k and v (Tk rows).  Sequence d has Lq queries and Lk keys; query i stands
+ * at position p = i + Lk - Lq of its keys.  s = scale * q . k; with cap > 0: s = cap * tanh(s / cap); with slopes: s -= slopes[head] * |p - j|.
+ * A query sees the keys of its own sequence only: all of them, or (causal) key j with j <= p or j < prefix of the sequence.
+ * o = softmax(s) v, lse = log sum exp(s); a query that sees nothing has o = 0, lse = -inf and no part in any gradient.
+ * Query head h reads key head h / (Hq / Hk).  Rows of o, lse and the gradients that belong to no sequence are not written; rows of q, k, v
+ * behind a sequence are not used whatever they hold.  Inside a sequence k and v have to be finite.
+ *
+ * The host describes the batch by two tables of records of eight int32 in device memory, one per 128 rows of a sequence, in any order (the
+ * longest work first is the fastest):
+ *   q_tiles  {first query row, rows (1 .. 128), first key row of the sequence, Lk, p of the first row, prefix (Lk where not causal), slot, 0};
+ *            slots number the tiles 0 .. n_q_tiles - 1, those of one sequence one after the other
+ *   k_tiles  {first key row, rows, first query row of the sequence, Lq, index of the first key, Lk - Lq, prefix, slot of the sequence's first
+ *            query tile}
+ * Records must lie inside the tensors: the kernels take them as they are.
+ *
+ * Replaces nothing of the reference's fast paths, which have no mask and no gradient; the model's attention in training is
+ * src/lightly_train/_task_models/dinov3_eomt_semantic_segmentation/task_model.py:674-698. */
+typedef struct kf_heads {
+  void* ptr;               /* [rows, heads, 64], 16-byte aligned                                       */
+  int64_t row_stride;      /* in elements, multiples of 8, at least 64                                 */
+  int64_t head_stride;
+} kf_heads;
+typedef struct kf_attn_pack_params {
+  int dtype, Hq, Hk, n_q_tiles, n_k_tiles;
+  float scale, cap;        /* scale > 0; cap 0 = none                                                  */
+  int64_t Tq, Tk;
+  const int32_t *q_tiles, *k_tiles;
+  const float* slopes;     /* fp32 [Hq] or NULL                                                        */
+  float* lse;              /* fp32 [Hq, Tq]: written by the forward, read by the gradient              */
+  kf_heads q, k, v, o;     /* o: written by the forward, read by the gradient                          */
+  kf_heads dout, dq, dk, dv; /* gradient only                                                          */
+  void* ws;                /* gradient only: kf_attn_pack_ws_bytes bytes                               */
+  int64_t ws_bytes;
+} kf_attn_pack_params;
+KF_API int kf_attn_pack_fwd(const kf_attn_pack_params* p, void* stream);
+/* dq, dk, dv from dout and what the forward read and wrote (the same tables, scale, cap and slopes; slopes have no gradient).  No atomics. */
+KF_API int64_t kf_attn_pack_ws_bytes(int Hq, int n_q_tiles);
+KF_API int kf_attn_pack_bwd(const kf_attn_pack_params* p, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

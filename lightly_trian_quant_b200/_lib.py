@@ -40,6 +40,19 @@ class RopeParams(C.Structure):
                 ("pos_kind", C.c_int), ("G", C.c_int), ("T", C.c_int), ("H", C.c_int), ("D", C.c_int), ("P", C.c_int), ("interleaved", C.c_int), ("inverse", C.c_int)]
 
 
+class Heads(C.Structure):
+    """mirror of kf_heads."""
+    _fields_ = [("ptr", C.c_void_p), ("row_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class AttnPackParams(C.Structure):
+    """mirror of kf_attn_pack_params."""
+    _fields_ = [("dtype", C.c_int), ("Hq", C.c_int), ("Hk", C.c_int), ("n_q_tiles", C.c_int), ("n_k_tiles", C.c_int), ("scale", C.c_float), ("cap", C.c_float),
+                ("Tq", C.c_int64), ("Tk", C.c_int64), ("q_tiles", C.c_void_p), ("k_tiles", C.c_void_p), ("slopes", C.c_void_p), ("lse", C.c_void_p),
+                ("q", Heads), ("k", Heads), ("v", Heads), ("o", Heads), ("dout", Heads), ("dq", Heads), ("dk", Heads), ("dv", Heads), ("ws", C.c_void_p),
+                ("ws_bytes", C.c_int64)]
+
+
 _lib = None
 
 
@@ -64,6 +77,8 @@ def lib() -> C.CDLL:
         L.kf_sf_bytes.restype = C.c_int64
         L.kf_sf_bytes.argtypes = [C.c_int64, C.c_int64, C.c_int]
         vp, i32, i64, f32 = C.c_void_p, C.c_int, C.c_int64, C.c_float
+        L.kf_attn_pack_ws_bytes.restype = i64
+        L.kf_attn_pack_ws_bytes.argtypes = [i32, i32]
         L.kf_layer_norm_ws_bytes.restype = i64
         L.kf_layer_norm_ws_bytes.argtypes = [i64, i32]
         sigs = {
@@ -90,6 +105,8 @@ def lib() -> C.CDLL:
             "kf_semantic": [vp, vp, i32, i32, i32, i32, vp, vp, vp],
             "kf_layer_norm_fwd": [i32, vp, i64, vp, vp, f32, i32, i32, i32, vp, vp, vp, vp],
             "kf_layer_norm_bwd": [i32, vp, i64, i32, vp, i64, vp, vp, vp, vp, i64, i32, i32, vp, vp, vp, vp, i64, vp],
+            "kf_attn_pack_fwd": [C.POINTER(AttnPackParams), vp],
+            "kf_attn_pack_bwd": [C.POINTER(AttnPackParams), vp],
             "kf_rope_axes": [C.POINTER(RopeParams), vp],
             "kf_resize_norm": [vp, vp, i32, i32, i32, i32, C.POINTER(C.c_float), C.POINTER(C.c_float), vp],
         }

@@ -789,6 +789,144 @@ PyObject* rope_axes(PyObject* const* v) {
   return v[8] == Py_None ? THPVariable_Wrap(std::move(out)) : new_ref(v[8]);
 }
 
+// An operand [rows, heads, 64] of the packed attention.
+kf_heads pack_heads(const at::Tensor& t) { return {t.data_ptr(), t.stride(0), t.stride(1)}; }
+const at::Tensor& pack_tensor(PyObject* o, const at::Tensor* first, const char* op, const char* what) {
+  const at::Tensor& t = cuda_tensor(o, what);
+  if (t.dim() != 3 || t.size(2) != 64 || t.stride(2) != 1) fail("%s: %s must be [rows, heads, 64] with contiguous channels", op, what);
+  if (first) {
+    if (t.scalar_type() != first->scalar_type()) fail("%s: %s must have the type of q", op, what);
+    same_device(*first, t, op, what);
+  } else if (t.scalar_type() != at::kBFloat16 && t.scalar_type() != at::kHalf) {
+    fail("%s: %s must be bf16 or f16", op, what);
+  }
+  return t;
+}
+void same_shape(const at::Tensor& a, const at::Tensor& b, const char* op, const char* what) {
+  if (a.sizes() != b.sizes()) fail("%s: %s has another shape than the operand it belongs to", op, what);
+}
+void same_place(const at::Tensor& t, const char* op, const char* what) {          // written row by row from many threads
+  for (int i = 0; i < 2; ++i)
+    if (t.size(i) > 1 && t.stride(i) == 0) fail("%s: %s must not be an expanded tensor", op, what);
+}
+
+// What both directions share.  v: q, k, v, q_tiles, k_tiles, query rows, key rows, scale, cap, slopes | None
+struct Pack {
+  const at::Tensor &q, &k, &v;
+  kf_attn_pack_params p;
+  int64_t q_rows, k_rows;
+};
+const at::Tensor& pack_table(PyObject* o, const at::Tensor& q, const char* op) {
+  const at::Tensor& t = cuda_tensor(o, "plan");
+  if (t.scalar_type() != at::kInt || t.dim() != 2 || t.size(1) != 8 || !t.is_contiguous() || t.size(0) > INT32_MAX) fail("%s: the plan's tables must be contiguous int32 [n, 8]", op);
+  same_device(q, t, op, "the plan");
+  return t;
+}
+Pack pack_operands(PyObject* const* v, const char* op) {
+  const at::Tensor& q = pack_tensor(v[0], nullptr, op, "q");
+  Pack c{q, pack_tensor(v[1], &q, op, "k"), pack_tensor(v[2], &q, op, "v"), {}, to_int(v[5]), to_int(v[6])};
+  same_shape(c.k, c.v, op, "v");
+  if (c.q_rows > q.size(0) || c.k_rows > c.k.size(0))
+    fail("%s: the plan is for %lld query and %lld key rows, there are %lld and %lld", op, (long long)c.q_rows, (long long)c.k_rows, (long long)q.size(0), (long long)c.k.size(0));
+  if (q.size(1) < 1 || c.k.size(1) < 1 || q.size(1) > 65536 || q.size(1) % c.k.size(1))
+    fail("%s: %lld query heads do not share %lld key heads evenly", op, (long long)q.size(1), (long long)c.k.size(1));
+  const at::Tensor &qt = pack_table(v[3], q, op), &kt = pack_table(v[4], q, op);
+  kf_attn_pack_params& p = c.p;
+  p.dtype = dtype_code(q.scalar_type());
+  p.Hq = (int)q.size(1);
+  p.Hk = (int)c.k.size(1);
+  p.n_q_tiles = (int)qt.size(0);
+  p.n_k_tiles = (int)kt.size(0);
+  p.scale = (float)to_float(v[7]);
+  p.cap = (float)to_float(v[8]);
+  p.Tq = q.size(0);
+  p.Tk = c.k.size(0);
+  p.q_tiles = qt.data_ptr<int>();
+  p.k_tiles = kt.data_ptr<int>();
+  if (v[9] != Py_None) p.slopes = affine(v[9], q, q.size(1), op, "slopes").data_ptr<float>();
+  p.q = pack_heads(q);
+  p.k = pack_heads(c.k);
+  p.v = pack_heads(c.v);
+  return c;
+}
+// A new tensor of this shape: the first `used` rows are written by the call, the others are zero.
+at::Tensor pack_new(const at::Tensor& like, int64_t used) {
+  at::Tensor t = empty(like.sizes(), like.scalar_type(), like.device());
+  if (used < t.size(0)) {
+    const Unlocked unlocked;
+    t.narrow(0, used, t.size(0) - used).zero_();
+  }
+  return t;
+}
+
+// ..., out | None
+PyObject* attn_packed(PyObject* const* v) {
+  const char* const op = "attn_packed";
+  Pack c = pack_operands(v, op);
+  const c10::cuda::CUDAGuard guard(c.q.device());
+  at::Tensor out;
+  if (v[10] == Py_None) {
+    out = pack_new(c.q, c.q_rows);
+  } else {
+    out = pack_tensor(v[10], &c.q, op, "out");
+    same_shape(c.q, out, op, "out");
+    same_place(out, op, "out");
+    writable(out);
+  }
+  at::Tensor lse = empty({c.q.size(1), c.q.size(0)}, at::kFloat, c.q.device());
+  if (c.q_rows < c.q.size(0)) {
+    const Unlocked unlocked;
+    lse.narrow(1, c.q_rows, c.q.size(0) - c.q_rows).zero_();
+  }
+  c.p.o = pack_heads(out);
+  c.p.lse = lse.data_ptr<float>();
+  launch(op, kf_attn_pack_fwd, (const kf_attn_pack_params*)&c.p, stream());
+  if (v[10] == Py_None) return pair(std::move(out), std::move(lse));
+  PyObject* t = PyTuple_New(2);
+  PyTuple_SET_ITEM(t, 0, new_ref(v[10]));
+  PyTuple_SET_ITEM(t, 1, THPVariable_Wrap(std::move(lse)));
+  return t;
+}
+
+// ..., dout, out, lse, dq | None, dk | None, dv | None
+PyObject* attn_packed_bwd(PyObject* const* v) {
+  const char* const op = "attn_packed_bwd";
+  Pack c = pack_operands(v, op);
+  const at::Tensor &dout = pack_tensor(v[10], &c.q, op, "dout"), &out = pack_tensor(v[11], &c.q, op, "out"), &lse = cuda_tensor(v[12], "lse");
+  same_shape(c.q, dout, op, "dout");
+  same_shape(c.q, out, op, "out");
+  if (lse.scalar_type() != at::kFloat || !lse.is_contiguous() || lse.dim() != 2 || lse.size(0) != c.q.size(1) || lse.size(1) != c.q.size(0))
+    fail("%s: lse must be contiguous fp32 [query heads, query rows]", op);
+  same_device(c.q, lse, op, "lse");
+  const c10::cuda::CUDAGuard guard(c.q.device());
+  const at::Tensor* const of[3] = {&c.q, &c.k, &c.v};
+  const char* const names[3] = {"dq", "dk", "dv"};
+  at::Tensor g[3];
+  for (int i = 0; i < 3; ++i) {
+    if (v[13 + i] == Py_None) continue;
+    g[i] = pack_tensor(v[13 + i], &c.q, op, names[i]);
+    same_shape(*of[i], g[i], op, names[i]);
+    same_place(g[i], op, names[i]);
+  }
+  for (int i = 0; i < 3; ++i) {
+    if (g[i].defined()) writable(g[i]);
+    else g[i] = pack_new(*of[i], i ? c.k_rows : c.q_rows);
+  }
+  c.p.dout = pack_heads(dout);
+  c.p.o = pack_heads(out);
+  c.p.lse = lse.data_ptr<float>();
+  c.p.dq = pack_heads(g[0]);
+  c.p.dk = pack_heads(g[1]);
+  c.p.dv = pack_heads(g[2]);
+  c.p.ws_bytes = kf_attn_pack_ws_bytes(c.p.Hq, c.p.n_q_tiles);
+  at::Tensor ws = empty({c.p.ws_bytes / 4}, at::kFloat, c.q.device());
+  c.p.ws = ws.data_ptr();
+  launch(op, kf_attn_pack_bwd, (const kf_attn_pack_params*)&c.p, stream());
+  PyObject* t = PyTuple_New(3);
+  for (int i = 0; i < 3; ++i) PyTuple_SET_ITEM(t, i, v[13 + i] == Py_None ? THPVariable_Wrap(std::move(g[i])) : new_ref(v[13 + i]));
+  return t;
+}
+
 // a weight: does the next GEMM with it read it ahead of its predecessor's end?
 PyObject* reads_weight_early(PyObject* const* v) {
   const Ref q = attr(v[0], s_q), sf = attr(v[0], s_sf);
@@ -825,6 +963,7 @@ PyMethodDef g_methods[] = {KF_ENTRY(quant_rows, 4),     KF_ENTRY(ln_quant, 7),  
                            KF_ENTRY(ln_tail, 8),        KF_ENTRY(attn_fwd, 3),   KF_ENTRY(attn_fwd_quant, 4), KF_ENTRY(im2col_patch16, 1), KF_ENTRY(dw_ln, 10),
                            KF_ENTRY(semantic, 3),       KF_ENTRY(amax_scale, 5), KF_ENTRY(ln_amax_scale, 7),
                            KF_ENTRY(layer_norm_fwd, 5), KF_ENTRY(layer_norm_bwd, 7), KF_ENTRY(rope_axes, 9),
+                           KF_ENTRY(attn_packed, 11),   KF_ENTRY(attn_packed_bwd, 16),
                            KF_ENTRY(reads_weight_early, 1), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_kf_host", "native operator layer over libkf_b200.so", -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -46,7 +46,7 @@
 // (attn16o.cu:184-194); with fp32 accumulation it is mathematically neutral and is accepted but not applied.
 #include <type_traits>
 
-#include "kf_sm100.cuh"
+#include "kf_attn.cuh"
 
 namespace kf {
 
@@ -76,46 +76,6 @@ struct AttnArgs {
   uint8_t *Qo, *SFo;
   const float* tso;
 };
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// 2^t for a pair without the special-function unit: t = n + f with n = round(t) taken from the low mantissa bits of
-// t + 1.5 * 2^23 and f in [-0.5, 0.5]; 2^f by a cubic (minimax for the relative error on that interval: 7.6e-5, far
-// below the rounding of the 16-bit P it feeds); n goes into the exponent field by an integer add.  t is clamped at -126
-// (the result is then 2^-126 instead of 0: it vanishes in the 16-bit P and in the row sum alike) and at 127, behind which the add
-// would wrap to anything, a small or a negative number too: a row with such an element has a sum that no limit lets pass.  A t that
-// is no number passes the clamps and the add makes a huge element of it, with the same effect (a clamp that drops it would drop the key).  All of it runs on the
-// FMA and integer pipes, as packed pairs where the operation exists.
-// Clamps and no check of the largest t: that costs an instruction less, but a register through the key loop (captured, us: B 14, H 12, N 1605, MXFP8 out
-// 137.5 against 135.3; B 1, H 16, N 1605 22.2 against 21.9).
-__device__ __forceinline__ float clamp_ex2(float t) {
-  asm("max.NaN.f32 %0, %0, 0fC2FC0000;\n\tmin.NaN.f32 %0, %0, 0f42FE0000;" : "+f"(t));   // [-126, 127]
-  return t;
-}
-__device__ __forceinline__ float2 ex2_poly2(float2 t) {
-  t.x = clamp_ex2(t.x);
-  t.y = clamp_ex2(t.y);
-  const float2 r = add2(t, splat2(12582912.f));
-  const float2 n = add2(r, splat2(-12582912.f));
-  const float2 f = fma2(n, splat2(-1.f), t);
-  float2 p = fma2(f, splat2(0x1.c43e56p-5f), splat2(0x1.f0df98p-3f));
-  p = fma2(p, f, splat2(0x1.62f24ap-1f));
-  p = fma2(p, f, splat2(0x1.fff686p-1f));
-  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(r.x) << 23)), __int_as_float(__float_as_int(p.y) + (__float_as_int(r.y) << 23)));
-}
-
-__device__ __forceinline__ uint32_t pack16(float a, float b, int f16) {
-  if (f16) {
-    __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<uint32_t*>(&h);
-  }
-  __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<uint32_t*>(&h);
-}
 
 // F16: 16-bit type of q / k / v / P / O (0 = bf16); OUT: -1 = plain 16-bit output, else the KF_FMT_* of the fused
 // output quantisation.  Compile-time so that the softmax loop carries one copy of its code.

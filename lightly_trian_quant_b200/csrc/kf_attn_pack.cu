@@ -1,0 +1,575 @@
+// Attention forward over packed sequences (images or clips of different lengths behind one another), head dimension 64, on the sm_100a
+// tensor cores.
+//
+//   s = scale * q . k;  with a cap: s = cap * tanh(s / cap);  with slopes: s -= slope(head) * |position of q - index of k|
+//   a query sees keys [0, limit) of its own sequence (QTile::limit: all, or up to itself and the prefix); o = softmax(s) v over them,
+//   lse = log sum exp(s); a query that sees nothing has o = 0 and lse = -inf
+//
+// The machine is that of the forward over equal images (kf_attn.cu: roles, S buffers in tensor memory, P over the first half of its S,
+// key tiles of 96, the running maximum that is only looked for where a tile's row sum came out too large).  What differs:
+//   - an item is a record of the host's table and a head; items have different numbers of key tiles, the longest first, and none is
+//     possible: every role steps from item to item with its own cursor
+//   - a tile may reach behind the end of its sequence: the scores there are masked one by one, the rows of V are set to zero in shared
+//     memory by the warp that issues the products (P is 0 there, but 0 * NaN is not)
+//   - with a cap or slopes the scores are brought to the exponent's scale in registers before the maximum; tanh(y) = 1 - 2 / (1 + e^2y):
+//     absolute error ~1e-7, which the cap scales (tanh.approx would leave 2^-11)
+//   - the polynomial exponential is a degree finer, for the log-sum-exp
+#include <type_traits>
+
+#include "kf_attn.cuh"
+
+namespace kf {
+
+constexpr int PK_BM = 128, PK_BN = 96, PK_D = 64;
+constexpr int PK_THREADS = 256;                        // warps 0..3 softmax, 4 TMA, 5 MMA issuer, 6 and 7 idle
+constexpr int PK_REGS_SOFTMAX = 208, PK_REGS_LEAN = 48; // 128 * 208 + 128 * 48 <= 256 * 128, the allocation at launch
+constexpr int PK_KV = 3;
+constexpr int PK_QTILE = PK_BM * PK_D * 2, PK_KTILE = PK_BN * PK_D * 2;
+constexpr int PK_OFF_K = 2 * PK_QTILE, PK_OFF_V = PK_OFF_K + PK_KV * PK_KTILE, PK_OFF_BAR = PK_OFF_V + PK_KV * PK_KTILE;
+constexpr size_t PK_SMEM = (size_t)PK_OFF_BAR + 256;
+constexpr float PK_SUM_LIMIT = 32768.f;
+constexpr int PK_POLY_K = 3;                           // element pairs PK_POLY_K .. 3 of every four take the polynomial exponential
+constexpr int PK_SBUF = 2;
+constexpr int PK_TMEM_COLS = 256, PK_COL_O = PK_SBUF * PK_BN;
+static_assert(PK_COL_O + PK_D <= PK_TMEM_COLS, "TMEM budget");
+
+struct PackFwdArgs {
+  void* O;
+  int64_t o_st, o_sh;       // strides of O in elements
+  float* lse;               // [Hq, lse_ld]
+  int64_t lse_ld;
+  const int4* tiles;        // QTile records
+  int n_tiles, Hq, share;   // share = query heads per key head
+  float scale_log2;         // scale * log2(e)
+  float cap_in, cap_out;    // 2 * scale * log2(e) / cap, cap * log2(e)
+  const float* slopes;      // [Hq]
+  int wide;                 // rows of O are 32-byte aligned
+  unsigned int* err;
+};
+
+template <int F16, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(PK_THREADS, 2)
+attn_pack_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                     const __grid_constant__ PackFwdArgs a) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + PK_OFF_BAR);
+  uint64_t *q_full = bars, *q_empty = bars + 2, *k_full = bars + 4, *k_empty = k_full + PK_KV, *v_full = k_empty + PK_KV, *v_empty = v_full + PK_KV,
+           *s_full = v_empty + PK_KV, *p_full = s_full + PK_SBUF, *o_full = p_full + PK_SBUF;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(o_full + PK_SBUF);
+  volatile uint32_t* abort_flag = tmem_holder + 1;
+
+  pdl_launch_dependents();
+  const int warp = warp_index(), lane = threadIdx.x & 31;
+  const int items = a.n_tiles * a.Hq;
+  const int n_my = (int)blockIdx.x < items ? (items - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x : 0;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
+    }
+    for (int i = 0; i < PK_KV; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
+    }
+    for (int i = 0; i < PK_SBUF; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 128);
+      mbar_init(&o_full[i], 1);
+    }
+    *abort_flag = 0u;
+    fence_mbar_init();
+  }
+  if (warp == 5) {
+    tmem_alloc(tmem_holder, PK_TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_wait();
+  const uint32_t tmem_base = *tmem_holder;
+  const WaitCtx ctx{abort_flag, a.err};
+  const bool bad_align = (smem_u32(smem) & 1023u) != 0;
+  if (bad_align && threadIdx.x == 0 && atomicCAS(&a.err[0], 0u, 99u) == 0u) {
+    a.err[1] = 110;
+    a.err[2] = blockIdx.x;
+  }
+  auto tile_of = [&](int it) { return load_tile<QTile>(a.tiles, ((int)blockIdx.x + it * (int)gridDim.x) / a.Hq); };
+  auto head_of = [&](int it) { return ((int)blockIdx.x + it * (int)gridDim.x) % a.Hq; };
+  auto key_tiles = [](const QTile& t) { return (t.limit(t.rows - 1) + PK_BN - 1) / PK_BN; };
+
+  if (warp >= 4) {
+  setmaxnreg_dec<PK_REGS_LEAN>();
+  if (bad_align) {
+    // nothing was issued; fall through to the teardown
+  } else if (warp == 4) {
+    // ------------------------------------------------------------------ TMA producer
+    if (elect_one()) {
+      prefetch_tmap(&tmQ);
+      prefetch_tmap(&tmK);
+      prefetch_tmap(&tmV);
+    }
+    uint32_t st = 0, ph = 1;
+    bool ok = !__any_sync(0xffffffffu, *static_cast<volatile unsigned int*>(a.err) != 0u);   // has an earlier launch failed?
+    if (!ok) *abort_flag = 1u;
+    uint32_t qi = 0;                                                              // items with keys so far
+    for (int it = 0; it < n_my && ok; ++it) {
+      const QTile t = tile_of(it);
+      const int n_kt = key_tiles(t), h = head_of(it), hk = h / a.share;
+      if (n_kt == 0) continue;
+      const uint32_t qb = qi & 1;
+      if (!mbar_wait_warp(&q_empty[qb], ((qi >> 1) & 1) ^ 1, ctx, 40)) break;
+      if (elect_one()) {
+        mbar_expect_tx(&q_full[qb], PK_QTILE);
+        tma_load_3d(smem + qb * PK_QTILE, &tmQ, 0, h, t.row, &q_full[qb]);
+      }
+      __syncwarp();
+      ++qi;
+      for (int j = 0; j < n_kt; ++j) {
+        if (!mbar_wait_warp(&k_empty[st], ph, ctx, 41)) { ok = false; break; }
+        if (elect_one()) {
+          mbar_expect_tx(&k_full[st], PK_KTILE);
+          tma_load_3d(smem + PK_OFF_K + st * PK_KTILE, &tmK, 0, hk, t.k_row + j * PK_BN, &k_full[st]);
+        }
+        __syncwarp();
+        if (!mbar_wait_warp(&v_empty[st], ph, ctx, 42)) { ok = false; break; }
+        if (elect_one()) {
+          mbar_expect_tx(&v_full[st], PK_KTILE);
+          tma_load_3d(smem + PK_OFF_V + st * PK_KTILE, &tmV, 0, hk, t.k_row + j * PK_BN, &v_full[st]);
+        }
+        __syncwarp();
+        if (++st == PK_KV) {
+          st = 0;
+          ph ^= 1;
+        }
+      }
+    }
+  } else if (warp == 5) {
+    // ------------------------------------------------------------------ MMA issuer: S(0), S(1), then PV(G) and S(G + 2) for every step
+    const uint32_t idesc_s = idesc_f16(F16 ? 0u : 1u, PK_BN);
+    const uint32_t idesc_o = idesc_f16(F16 ? 0u : 1u, PK_D) | (1u << 16);     // B (= V) is MN-major
+    const uint32_t t_o = tmem_base + PK_COL_O;
+    const bool leader = elect_one();
+    struct Cursor {                                                          // a key tile of an item; items without keys are stepped over
+      int it, j, n, k_len;
+    };
+    auto settle = [&](Cursor& c) {                                           // c.it: the first item at or behind it that has keys
+      for (; c.it < n_my; ++c.it) {
+        const QTile t = tile_of(c.it);
+        c.j = 0;
+        c.n = key_tiles(t);
+        c.k_len = t.k_len;
+        if (c.n > 0) return;
+      }
+    };
+    auto advance = [&](Cursor& c) {
+      if (++c.j == c.n) {
+        ++c.it;
+        settle(c);
+      }
+    };
+    Cursor s{0, 0, 0, 0};                                                    // the next S product
+    settle(s);
+    Cursor v = s;                                                            // the next PV product
+    uint32_t s_qi = 0, k_st = 0, k_ph = 0;
+    auto issue_s = [&](uint32_t buf) {
+      const uint64_t qdesc = smem_desc_sw128(smem_u32(smem + (s_qi & 1) * PK_QTILE));
+      const uint64_t kdesc = smem_desc_sw128(smem_u32(smem + PK_OFF_K + k_st * PK_KTILE));
+      const uint32_t t_s = tmem_base + buf * PK_BN;
+      const bool last = s.j + 1 == s.n;
+      if (leader) {
+#pragma unroll
+        for (int kk = 0; kk < PK_D / 16; ++kk) mma_f16(t_s, qdesc + 2 * kk, kdesc + 2 * kk, idesc_s, kk != 0);
+        tc_commit(&s_full[buf]);
+        tc_commit(&k_empty[k_st]);
+        if (last) tc_commit(&q_empty[s_qi & 1]);
+      }
+      __syncwarp();
+      if (last) ++s_qi;
+      advance(s);
+      if (++k_st == PK_KV) {
+        k_st = 0;
+        k_ph ^= 1;
+      }
+    };
+    bool ok = true;
+    for (uint32_t G = 0; G < PK_SBUF && s.it < n_my && ok; ++G) {
+      ok = (s.j != 0 || mbar_wait_warp(&q_full[s_qi & 1], (s_qi >> 1) & 1, ctx, 43)) && mbar_wait_warp(&k_full[k_st], k_ph, ctx, 44);
+      tc_fence_after();
+      if (ok) issue_s(G);
+    }
+    uint32_t buf = 0, pph = 0, st = 0, vph = 0;
+    while (v.it < n_my && ok) {
+      const bool more = s.it < n_my;
+      if (more && s.j == 0 && !mbar_wait_warp(&q_full[s_qi & 1], (s_qi >> 1) & 1, ctx, 43)) break;
+      const int valid = v.k_len - v.j * PK_BN;                               // rows of this V tile that belong to the sequence
+      if (valid < PK_BN) {
+        if (!mbar_wait_warp(&v_full[st], vph, ctx, 45)) break;
+        zero_rows(smem + PK_OFF_V + st * PK_KTILE, valid, PK_BN, lane);
+      }
+      if (more) {
+        if (!mbar_wait_warp3(&p_full[buf], pph, &v_full[st], vph, &k_full[k_st], k_ph, ctx, 46)) break;
+      } else {
+        if (!mbar_wait_warp3(&p_full[buf], pph, &v_full[st], vph, &v_full[st], vph, ctx, 46)) break;
+      }
+      tc_fence_after();
+      const uint32_t t_p = tmem_base + buf * PK_BN;
+      const uint64_t vdesc = smem_desc_sw128(smem_u32(smem + PK_OFF_V + st * PK_KTILE));
+      if (leader) {
+#pragma unroll
+        for (int kk = 0; kk < PK_BN / 16; ++kk)
+          mma_f16_ta(t_o, t_p + 8 * kk, vdesc + (uint64_t)(kk * (2048 >> 4)), idesc_o, (v.j | kk) != 0);
+        tc_commit(&o_full[buf]);
+        tc_commit(&v_empty[st]);
+      }
+      __syncwarp();
+      if (more) issue_s(buf);
+      advance(v);
+      if (++buf == PK_SBUF) {
+        buf = 0;
+        pph ^= 1;
+      }
+      if (++st == PK_KV) {
+        st = 0;
+        vph ^= 1;
+      }
+    }
+  }
+  } else {
+    setmaxnreg_inc<PK_REGS_SOFTMAX>();
+    if (!bad_align) {
+    // ------------------------------------------------------------------ softmax: thread = query row
+    const int row = warp * 32 + lane;
+    const uint32_t t_lane = tmem_base + ((uint32_t)(warp * 32) << 16);
+    constexpr bool RAW = !CAP && !BIAS;                          // the registers hold raw products: the scale is applied with the maximum
+    const float sc = RAW ? a.scale_log2 : 1.f;
+    const float2 sc2 = splat2(sc);
+    bool ok = true;
+    uint32_t buf = 0, sph = 0;
+    auto exp_half = [&](const uint32_t (&r)[32], uint32_t* w, float2 mn2, float2& s0, float2& s1) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float2 p[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 x = make_float2(__uint_as_float(r[8 * i + 2 * k]), __uint_as_float(r[8 * i + 2 * k + 1]));
+          const float2 t = RAW ? fma2(x, sc2, mn2) : add2(x, mn2);
+          p[k] = k >= PK_POLY_K ? ex2_poly2_fine(t) : make_float2(ex2(t.x), ex2(t.y));
+        }
+        s0 = add2(s0, add2(p[0], p[1]));
+        s1 = add2(s1, add2(p[2], p[3]));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[4 * i + k] = pack16(p[k].x, p[k].y, F16);
+      }
+    };
+    auto row_max = [](const uint32_t (&r)[32], float mx) {
+      float m4[4] = {mx, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int i = 0; i < 16; ++i) m4[i & 3] = max3(m4[i & 3], __uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+      return amax_nan(amax_nan(m4[0], m4[1]), amax_nan(m4[2], m4[3]));
+    };
+    auto store32 = [&](uint8_t* dst, const uint32_t* w) {
+      if (a.wide) {
+        stg8w(dst, w);
+      } else {
+        reinterpret_cast<uint4*>(dst)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        reinterpret_cast<uint4*>(dst)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+      }
+    };
+    for (int it = 0; it < n_my && ok; ++it) {
+    const QTile tile = tile_of(it);
+    const int h = head_of(it);
+    const int n_kt = key_tiles(tile);
+    const int lim = row < tile.rows ? tile.limit(row) : 0;       // keys this row sees
+    const int warp_lim = tile.limit(warp * 32);                  // the fewest of the warp's rows that exist (rows that do not are not stored)
+    const float slope = BIAS ? __ldg(a.slopes + h) * 1.4426950408889634f : 0.f;
+    const float at = (float)(tile.pos + row);
+    // raw products -> logits in units of the exponent, then the keys that the row does not see
+    auto logits = [&](uint32_t (&r)[32], int key0) {
+      if constexpr (!RAW) {
+        const float gap = at - (float)key0;
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          float2 x = make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1]));
+          if constexpr (CAP) {
+            const float2 rc = make_float2(rcp_approx(1.f + ex2(x.x * a.cap_in)), rcp_approx(1.f + ex2(x.y * a.cap_in)));
+            x = fma2(rc, splat2(-2.f * a.cap_out), splat2(a.cap_out));
+          } else {
+            x = mul2(x, splat2(a.scale_log2));
+          }
+          if constexpr (BIAS) {
+            x.x = fmaf(-slope, fabsf(gap - (float)i), x.x);
+            x.y = fmaf(-slope, fabsf(gap - (float)(i + 1)), x.y);
+          }
+          r[i] = __float_as_uint(x.x);
+          r[i + 1] = __float_as_uint(x.y);
+        }
+      }
+      if (key0 + 32 > warp_lim) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (key0 + i >= lim) r[i] = 0xff800000u;
+      }
+    };
+    float m_run = 0.f, l_run = 0.f;
+    uint32_t ra[32], rb[32], rc[32];                             // the S row of this step: keys 0..31, 32..63 and 64..95 of the tile
+    if (n_kt > 0) {
+      ok = mbar_wait_warp(&s_full[buf], sph, ctx, 47);
+      if (!ok) break;
+      tc_fence_after();
+      tmem_ld32(t_lane + buf * PK_BN, ra);
+      tmem_ld32(t_lane + buf * PK_BN + 32, rb);
+      tmem_ld32(t_lane + buf * PK_BN + 64, rc);
+    }
+    for (int j = 0; j < n_kt; ++j) {
+      const uint32_t t_s = t_lane + buf * PK_BN, cur = buf, cph = sph;
+      if (++buf == PK_SBUF) {
+        buf = 0;
+        sph ^= 1;
+      }
+      const bool prefetch = j + 1 < n_kt;
+      const int kbase = j * PK_BN;
+      tmem_ld_wait();
+      tmem_ld_fence(ra);
+      tmem_ld_fence(rb);
+      tmem_ld_fence(rc);
+      logits(ra, kbase);
+      logits(rb, kbase + 32);
+      logits(rc, kbase + 64);
+      if (j == 0) {
+        m_run = row_max(rb, row_max(ra, -INFINITY));
+        if (m_run == -INFINITY) m_run = 0.f;                     // a row that sees nothing
+      }
+      const float2 mn2 = splat2(-m_run * sc);
+      float2 s0 = make_float2(0.f, 0.f), s1 = s0;
+      uint32_t w[48];
+      exp_half(ra, w, mn2, s0, s1);
+      const bool ready = mbar_test_wait(&s_full[buf], sph);
+      exp_half(rb, w + 16, mn2, s0, s1);
+      if (prefetch) {
+        if (!__all_sync(0xffffffffu, ready) && !mbar_wait_warp(&s_full[buf], sph, ctx, 47)) { ok = false; break; }
+        tc_fence_after();
+        tmem_ld32(t_lane + buf * PK_BN, ra);
+        tmem_ld32(t_lane + buf * PK_BN + 32, rb);
+      }
+      exp_half(rc, w + 32, mn2, s0, s1);
+      if (prefetch) tmem_ld32(t_lane + buf * PK_BN + 64, rc);
+      float sum = (s0.x + s0.y) + (s1.x + s1.y), alpha = 1.f;
+      const bool need = row < tile.rows && !(sum <= PK_SUM_LIMIT);   // rows that are not stored go on with whatever they have
+      if (__any_sync(0xffffffffu, need)) {
+        uint32_t r[32];
+        float mx = m_run;
+#pragma unroll 1
+        for (int c = 0; c < PK_BN / 32; ++c) {
+          tmem_ld32(t_s + 32 * c, r);
+          tmem_ld_wait();
+          tmem_ld_fence(r);
+          logits(r, kbase + 32 * c);
+          mx = row_max(r, mx);
+        }
+        if (need) {
+          alpha = ex2((m_run - mx) * sc);
+          m_run = mx;
+        }
+        s0 = s1 = make_float2(0.f, 0.f);
+#pragma unroll 1
+        for (int c = 0; c < PK_BN / 32; ++c) {
+          tmem_ld32(t_s + 32 * c, r);
+          tmem_ld_wait();
+          tmem_ld_fence(r);
+          logits(r, kbase + 32 * c);
+          if (c == 0) exp_half(r, w, splat2(-m_run * sc), s0, s1);
+          else if (c == 1) exp_half(r, w + 16, splat2(-m_run * sc), s0, s1);
+          else exp_half(r, w + 32, splat2(-m_run * sc), s0, s1);
+        }
+        sum = (s0.x + s0.y) + (s1.x + s1.y);
+        if (j > 0) {                                             // rescale O: PV(G - 1) must have landed first
+          const uint32_t pb = cur == 0 ? PK_SBUF - 1 : cur - 1;
+          if (!mbar_wait_warp(&o_full[pb], cur == 0 ? cph ^ 1 : cph, ctx, 48)) { ok = false; break; }
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < 2; ++c) {
+            tmem_ld32(t_lane + PK_COL_O + 32 * c, r);
+            tmem_ld_wait();
+            tmem_ld_fence(r);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
+            tmem_st32(t_lane + PK_COL_O + 32 * c, r);
+          }
+        }
+      }
+      l_run = l_run * alpha + sum;
+      tmem_st32(t_s, *reinterpret_cast<const uint32_t(*)[32]>(w));
+      tmem_st16(t_s + 32, w + 32);
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&p_full[cur]);
+    }
+    // the item's last PV product
+    if (ok && n_kt > 0) ok = mbar_wait_warp(&o_full[buf == 0 ? PK_SBUF - 1 : buf - 1], buf == 0 ? sph ^ 1 : sph, ctx, 49);
+    if (ok) {
+      uint32_t r0[32], r1[32];
+      if (n_kt > 0) {
+        tc_fence_after();
+        tmem_ld32(t_lane + PK_COL_O, r0);
+        tmem_ld32(t_lane + PK_COL_O + 32, r1);
+        tmem_ld_wait();
+        tmem_ld_fence(r0);
+        tmem_ld_fence(r1);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) r0[i] = r1[i] = 0u;
+      }
+      if (row < tile.rows) {
+        const bool none = lim == 0;                              // (its sum is not quite 0: the polynomial gives 2^-126 for masked keys)
+        const float inv = 1.0f / l_run;
+        uint32_t w[32];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          w[i] = pack16(__uint_as_float(r0[2 * i]) * inv, __uint_as_float(r0[2 * i + 1]) * inv, F16);
+          w[16 + i] = pack16(__uint_as_float(r1[2 * i]) * inv, __uint_as_float(r1[2 * i + 1]) * inv, F16);
+        }
+        if (none) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) w[i] = 0u;
+        }
+        uint8_t* dst = static_cast<uint8_t*>(a.O) + 2 * ((int64_t)(tile.row + row) * a.o_st + (int64_t)h * a.o_sh);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) store32(dst + 32 * i, w + 8 * i);
+        a.lse[(int64_t)h * a.lse_ld + tile.row + row] = none ? -INFINITY : (m_run * sc + log2f(l_run)) * 0.6931471805599453f;
+      }
+    }
+    }   // items
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag && !bad_align) {
+    for (int i = 0; i < 64; ++i) __nanosleep(2000);
+  }
+  if (warp == 5) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, PK_TMEM_COLS);
+  }
+}
+
+// Encoding costs about a microsecond of host time: kept per thread, direct-mapped by the arguments.
+int make_tmap_heads(CUtensorMap* map, const void* base, int64_t rows, int heads, int64_t row_stride, int64_t head_stride, int box_rows) {
+  struct Slot {
+    const void* base;
+    int64_t rows, row_stride, head_stride;
+    int heads, box_rows;
+    CUtensorMap map;
+  };
+  constexpr int SLOTS = 64;
+  static thread_local Slot cache[SLOTS] = {};
+  const uintptr_t k = (reinterpret_cast<uintptr_t>(base) >> 4) * 0x9E3779B97F4A7C15ull + (uintptr_t)rows * 31 + (uintptr_t)row_stride * 7 + (uintptr_t)box_rows;
+  Slot& slot = cache[(k >> 32 ^ k) % SLOTS];
+  if (slot.base == base && slot.rows == rows && slot.row_stride == row_stride && slot.head_stride == head_stride && slot.heads == heads && slot.box_rows == box_rows) {
+    *map = slot.map;
+    return KF_OK;
+  }
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (!fn) {
+    set_error("cuTensorMapEncodeTiled is not available from the driver");
+    return KF_ERR_UNSUPPORTED;
+  }
+  cuuint64_t dims[3] = {64, (cuuint64_t)heads, (cuuint64_t)rows};
+  cuuint64_t strides[2] = {(cuuint64_t)head_stride * 2, (cuuint64_t)row_stride * 2};
+  cuuint32_t box[3] = {64, 1, (cuuint32_t)box_rows};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled (heads) failed with CUresult %d", (int)r);
+    return KF_ERR_BAD_ARGUMENT;
+  }
+  slot = Slot{base, rows, row_stride, head_stride, heads, box_rows, *map};
+  return KF_OK;
+}
+
+// A [rows, heads, 64] operand as the copies and the stores take it: 16-byte aligned, strides in whole 16-byte units; what has one row or
+// head gets a stride that means nothing.
+int check_heads(const char* what, const kf_heads& t, int64_t rows, int heads, kf_heads* out) {
+  *out = t;
+  if (heads == 1) out->head_stride = 64;
+  if (rows == 1) out->row_stride = (int64_t)64 * heads;
+  KF_REQUIRE(t.ptr && (reinterpret_cast<uintptr_t>(t.ptr) & 15) == 0, "kf_attn_pack: %s must be non-null and 16-byte aligned", what);
+  KF_REQUIRE(out->row_stride >= 64 && out->head_stride >= 64 && out->row_stride % 8 == 0 && out->head_stride % 8 == 0 && out->row_stride < (1ll << 38) &&
+                 out->head_stride < (1ll << 38),
+             "kf_attn_pack: strides of %s (%lld, %lld elements) must be multiples of 8, 64 at least", what, (long long)t.row_stride, (long long)t.head_stride);
+  return KF_OK;
+}
+
+int check_pack(const kf_attn_pack_params* p) {
+  KF_REQUIRE(p, "kf_attn_pack: null parameter block");
+  KF_REQUIRE(p->dtype == KF_BF16 || p->dtype == KF_F16, "kf_attn_pack: dtype must be bf16 or f16");
+  KF_REQUIRE(p->Hq > 0 && p->Hk > 0 && p->Hq % p->Hk == 0, "kf_attn_pack: %d query heads do not share %d key heads evenly", p->Hq, p->Hk);
+  KF_REQUIRE(p->Tq >= 0 && p->Tk >= 0 && p->Tq < (1ll << 31) - 256 && p->Tk < (1ll << 31) - 256, "kf_attn_pack: bad numbers of rows");
+  KF_REQUIRE(p->n_q_tiles >= 0 && p->n_k_tiles >= 0 && (int64_t)p->n_q_tiles * p->Hq < (1ll << 30) && (int64_t)p->n_k_tiles * p->Hk < (1ll << 30),
+             "kf_attn_pack: too many (tile, head) items");
+  KF_REQUIRE(p->scale > 0.f && p->scale < 1e30f && p->cap >= 0.f && p->cap < 1e30f, "kf_attn_pack: scale must be positive and cap not negative, both finite");
+  return KF_OK;
+}
+
+}  // namespace kf
+
+using namespace kf;
+
+extern "C" int kf_attn_pack_fwd(const kf_attn_pack_params* p, void* stream) {
+  int rc = check_pack(p);
+  if (rc != KF_OK) return rc;
+  if (p->n_q_tiles == 0) return KF_OK;
+  KF_REQUIRE(p->Tq > 0 && p->q_tiles && p->lse, "kf_attn_pack_fwd: null pointer");
+  kf_heads q, k, v, o;
+  if ((rc = check_heads("q", p->q, p->Tq, p->Hq, &q)) != KF_OK) return rc;
+  if ((rc = check_heads("o", p->o, p->Tq, p->Hq, &o)) != KF_OK) return rc;
+  k = v = q;
+  int k_heads = p->Hq;
+  int64_t k_rows = p->Tq;
+  if (p->Tk > 0) {                                            // without keys at all the maps are never used
+    if ((rc = check_heads("k", p->k, p->Tk, p->Hk, &k)) != KF_OK) return rc;
+    if ((rc = check_heads("v", p->v, p->Tk, p->Hk, &v)) != KF_OK) return rc;
+    k_heads = p->Hk;
+    k_rows = p->Tk;
+  }
+  CUtensorMap tq, tk, tv;
+  if ((rc = make_tmap_heads(&tq, q.ptr, p->Tq, p->Hq, q.row_stride, q.head_stride, PK_BM)) != KF_OK) return rc;
+  if ((rc = make_tmap_heads(&tk, k.ptr, k_rows, k_heads, k.row_stride, k.head_stride, PK_BN)) != KF_OK) return rc;
+  if ((rc = make_tmap_heads(&tv, v.ptr, k_rows, k_heads, v.row_stride, v.head_stride, PK_BN)) != KF_OK) return rc;
+  using KernelFn = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, PackFwdArgs);
+  static const KernelFn table[2][2][2] = {{{attn_pack_fwd_kernel<0, false, false>, attn_pack_fwd_kernel<0, false, true>}, {attn_pack_fwd_kernel<0, true, false>, attn_pack_fwd_kernel<0, true, true>}},
+                                          {{attn_pack_fwd_kernel<1, false, false>, attn_pack_fwd_kernel<1, false, true>}, {attn_pack_fwd_kernel<1, true, false>, attn_pack_fwd_kernel<1, true, true>}}};
+  const int f = p->dtype == KF_F16, c = p->cap > 0.f, b = p->slopes != nullptr;
+  const KernelFn kern = table[f][c][b];
+  static PerDevice<bool> attr_set[2][2][2];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!attr_set[f][c][b].get(dev)) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PK_SMEM);
+    if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(attn_pack_fwd_kernel)");
+    attr_set[f][c][b].put(dev, true);
+  }
+  constexpr float LOG2E = 1.4426950408889634f;
+  PackFwdArgs a{};
+  a.O = o.ptr; a.o_st = o.row_stride; a.o_sh = o.head_stride; a.lse = p->lse; a.lse_ld = p->Tq;
+  a.tiles = reinterpret_cast<const int4*>(p->q_tiles); a.n_tiles = p->n_q_tiles; a.Hq = p->Hq; a.share = p->Hq / p->Hk;
+  a.scale_log2 = p->scale * LOG2E;
+  if (c) {
+    a.cap_in = 2.f * p->scale * LOG2E / p->cap;
+    a.cap_out = p->cap * LOG2E;
+  }
+  a.slopes = p->slopes;
+  a.wide = ((reinterpret_cast<uintptr_t>(o.ptr) | (uintptr_t)(o.row_stride * 2) | (uintptr_t)(o.head_stride * 2)) & 31) == 0;
+  a.err = dev_error_ptr();
+  KF_REQUIRE(a.err != nullptr, "kf_attn_pack_fwd: device error word unavailable");
+  int sms = 0;
+  if ((rc = device_sm_count(&sms)) != KF_OK) return rc;
+  const int64_t items = (int64_t)p->n_q_tiles * p->Hq;
+  const int grid = items < 2 * sms ? (int)items : 2 * sms;    // two CTAs are resident per SM
+  return cuda_status(launch_maybe_pdl(p->Tq, kern, dim3(grid), dim3(PK_THREADS), PK_SMEM, static_cast<cudaStream_t>(stream), tq, tk, tv, a), "kf_attn_pack_fwd launch");
+}

@@ -407,6 +407,89 @@ def rope_axes(x: torch.Tensor, pos: torch.Tensor, table: RopeTable, *, inverse: 
     return _h.rope_axes(*args) if TIMING is None else _timed("rope_axes", _h.rope_axes, args)
 
 
+class AttnPlan:
+    """Who sees whom in a packed batch: the tables that attn_packed and attn_packed_bwd read, built once per composition of the batch and kept by the
+    caller as long as calls (or captured graphs) use them.
+
+    Sequence d has q_lens[d] queries and k_lens[d] keys (k_lens=None: the same), behind one another in the rows of q and of k and v; rows behind the
+    last sequence belong to none.  Query i of a sequence stands at position i + Lk - Lq of its keys and sees the keys of its own sequence: all of them,
+    or with causal=True key j where j <= its position or j < prefix[d].  Lengths may be 0, and a query may see nothing (Lq > Lk with causal=True).
+
+    A record per 128 rows of queries and of keys, the longest work first: the kernels' CTAs take them in turn."""
+
+    __slots__ = ("q_rows", "k_rows", "causal", "q_tiles", "k_tiles")
+
+    def __init__(self, q_lens, k_lens=None, *, causal: bool = False, prefix=None, device="cuda"):
+        import numpy as np
+
+        lens = [np.asarray([int(n) for n in (q_lens if ls is None else ls)], dtype=np.int64) for ls in (q_lens, k_lens)]
+        lq, lk = lens
+        if len(lq) != len(lk):
+            raise KfError(f"AttnPlan: {len(lq)} sequences of queries, {len(lk)} of keys")
+        if prefix is not None and not causal:
+            raise KfError("AttnPlan: a prefix goes with causal=True (without it every key is seen)")
+        pre = np.asarray([int(n) for n in prefix], dtype=np.int64) if prefix is not None else np.zeros_like(lk)
+        if len(pre) != len(lk):
+            raise KfError(f"AttnPlan: {len(lk)} sequences, {len(pre)} prefixes")
+        if (lq < 0).any() or (lk < 0).any() or (pre < 0).any() or (pre > lk).any():
+            raise KfError("AttnPlan: lengths must not be negative, a prefix not longer than its sequence of keys")
+        if lq.sum() >= 2**31 - 256 or lk.sum() >= 2**31 - 256:
+            raise KfError("AttnPlan: more rows than a call takes")
+        if not causal:
+            pre = lk
+        T = 128
+        q0, k0 = np.cumsum(lq) - lq, np.cumsum(lk) - lk
+        nq, nk = -(-lq // T), -(-lk // T)
+        slot0 = np.cumsum(nq) - nq
+        self.q_rows, self.k_rows, self.causal = int(lq.sum()), int(lk.sum()), bool(causal)
+
+        def tiles(n, first):                               # (sequence, tile of it) of every tile
+            d = np.repeat(np.arange(len(n)), n)
+            return d, np.arange(len(d)) - first[d]
+
+        d, i = tiles(nq, slot0)
+        rows = np.minimum(T, lq[d] - T * i)
+        pos = T * i + lk[d] - lq[d]
+        q = np.stack([q0[d] + T * i, rows, k0[d], lk[d], pos, pre[d], slot0[d] + i, 0 * d], 1)
+        seen = np.clip(np.maximum(pos + rows, pre[d]), 0, lk[d])
+        q = q[np.argsort(-seen, kind="stable")]
+        d, i = tiles(nk, np.cumsum(nk) - nk)
+        off = lk[d] - lq[d]
+        k = np.stack([k0[d] + T * i, np.minimum(T, lk[d] - T * i), q0[d], lq[d], T * i, off, pre[d], slot0[d]], 1)
+        low = np.where(T * i < pre[d], 0, np.maximum(T * i - off, 0))
+        k = k[np.argsort(low - lq[d], kind="stable")]
+        self.q_tiles, self.k_tiles = (torch.from_numpy(np.ascontiguousarray(t, dtype=np.int32)).reshape(-1, 8).to(device) for t in (q, k))
+
+
+def _pack_args(q, k, v, plan: AttnPlan, scale, cap, slopes) -> tuple:
+    return q, k, v, plan.q_tiles, plan.k_tiles, plan.q_rows, plan.k_rows, 0.125 if scale is None else scale, cap, slopes
+
+
+def attn_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: AttnPlan, *, scale: Optional[float] = None, cap: float = 0.0,
+                slopes: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None):
+    """Attention over packed sequences: q [Tq, Hq, 64], k, v [Tk, Hk, 64] (bf16 | f16, Hq a multiple of Hk; channels contiguous, 16-byte aligned rows
+    and heads with any strides, e.g. parts of one projection) -> (out [Tq, Hq, 64], lse fp32 [Hq, Tq]).
+
+    score = scale * q . k (scale 1/8 by default), then cap * tanh(score / cap) with cap > 0, then minus slopes[head] * |distance| (fp32 [Hq]);
+    plan says which keys a query sees.  A query that sees nothing gets 0 and -inf.  Rows behind the last sequence: zero in new tensors, left as they
+    were in a given out.  Keys and values inside a sequence have to be finite; rows outside the sequences may hold anything."""
+    global LAUNCHES
+    LAUNCHES += 1
+    args = (*_pack_args(q, k, v, plan, scale, cap, slopes), out)
+    return _h.attn_packed(*args) if TIMING is None else _timed("attn_packed", _h.attn_packed, args)
+
+
+def attn_packed_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, lse: torch.Tensor, plan: AttnPlan, *,
+                    scale: Optional[float] = None, cap: float = 0.0, slopes: Optional[torch.Tensor] = None, grads=(None, None, None)):
+    """Gradients of attn_packed -> (dq, dk, dv) in the operands' type; the other arguments as the forward took and gave them (slopes have no
+    gradient).  grads: tensors to write instead of new ones, e.g. the parts of one projection's gradient.  f16 gradients have the range of f16: scale
+    the loss as for any f16 product.  No atomics: the same bits from run to run."""
+    global LAUNCHES
+    LAUNCHES += 2
+    args = (*_pack_args(q, k, v, plan, scale, cap, slopes), dout, out, lse, *grads)
+    return _h.attn_packed_bwd(*args) if TIMING is None else _timed("attn_packed_bwd", _h.attn_packed_bwd, args)
+
+
 # ------------------------------------------------------------------------------------------------ patch embed / head / pre / post
 def gemm_tokens(a: torch.Tensor, W: QWeight, bias, out: torch.Tensor, rows_per_image: int, tokens_per_image: int, row_offset: int,
                 round_bf16: bool = False) -> torch.Tensor:
