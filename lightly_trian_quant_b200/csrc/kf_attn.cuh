@@ -103,6 +103,17 @@ __device__ __forceinline__ T load_tile(const int4* tiles, int index) {       // 
   return t;
 }
 
+// Items 0 .. n - 1, the longest first, among the CTAs of the grid: every other round in the opposite order, so that whoever got the longest of a
+// round gets the shortest of the next.
+__device__ __forceinline__ int items_of_cta(int n) {
+  const int g = (int)gridDim.x, rounds = n / g, rest = n - rounds * g;
+  const int place = rounds & 1 ? g - 1 - (int)blockIdx.x : (int)blockIdx.x;
+  return rounds + (place < rest);
+}
+__device__ __forceinline__ int item_of_cta(int it) {
+  return it * (int)gridDim.x + (it & 1 ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x);
+}
+
 __device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* map, int c0, int c1, int c2, uint64_t* bar) {
   asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(smem_dst)), "l"(map),
                "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)

@@ -61,7 +61,7 @@ attn_pack_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   pdl_launch_dependents();
   const int warp = warp_index(), lane = threadIdx.x & 31;
   const int items = a.n_tiles * a.Hq;
-  const int n_my = (int)blockIdx.x < items ? (items - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x : 0;
+  const int n_my = items_of_cta(items);
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -97,8 +97,8 @@ attn_pack_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     a.err[1] = 110;
     a.err[2] = blockIdx.x;
   }
-  auto tile_of = [&](int it) { return load_tile<QTile>(a.tiles, ((int)blockIdx.x + it * (int)gridDim.x) / a.Hq); };
-  auto head_of = [&](int it) { return ((int)blockIdx.x + it * (int)gridDim.x) % a.Hq; };
+  auto tile_of = [&](int it) { return load_tile<QTile>(a.tiles, item_of_cta(it) / a.Hq); };
+  auto head_of = [&](int it) { return item_of_cta(it) % a.Hq; };
   auto key_tiles = [](const QTile& t) { return (t.limit(t.rows - 1) + PK_BN - 1) / PK_BN; };
 
   if (warp >= 4) {
@@ -280,13 +280,19 @@ attn_pack_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       }
     };
     for (int it = 0; it < n_my && ok; ++it) {
-    const QTile tile = tile_of(it);
-    const int h = head_of(it);
-    const int n_kt = key_tiles(tile);
-    const int lim = row < tile.rows ? tile.limit(row) : 0;       // keys this row sees
-    const int warp_lim = tile.limit(warp * 32);                  // the fewest of the warp's rows that exist (rows that do not are not stored)
-    const float slope = BIAS ? __ldg(a.slopes + h) * 1.4426950408889634f : 0.f;
-    const float at = (float)(tile.pos + row);
+    // little of the record lives through the key loop: where the rows go is looked up again behind it
+    int n_kt, lim, warp_lim;                                     // lim: keys this row sees (-1: no row); warp_lim: the fewest of the warp's rows that exist
+    float slope = 0.f, at = 0.f;
+    {
+      const QTile tile = tile_of(it);
+      n_kt = key_tiles(tile);
+      lim = row < tile.rows ? tile.limit(row) : -1;
+      warp_lim = tile.limit(warp * 32);
+      if constexpr (BIAS) {
+        slope = __ldg(a.slopes + head_of(it)) * 1.4426950408889634f;
+        at = (float)(tile.pos + row);
+      }
+    }
     // raw products -> logits in units of the exponent, then the keys that the row does not see
     auto logits = [&](uint32_t (&r)[32], int key0) {
       if constexpr (!RAW) {
@@ -358,7 +364,7 @@ attn_pack_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       exp_half(rc, w + 32, mn2, s0, s1);
       if (prefetch) tmem_ld32(t_lane + buf * PK_BN + 64, rc);
       float sum = (s0.x + s0.y) + (s1.x + s1.y), alpha = 1.f;
-      const bool need = row < tile.rows && !(sum <= PK_SUM_LIMIT);   // rows that are not stored go on with whatever they have
+      const bool need = lim >= 0 && !(sum <= PK_SUM_LIMIT);   // rows that are not stored go on with whatever they have
       if (__any_sync(0xffffffffu, need)) {
         uint32_t r[32];
         float mx = m_run;
@@ -423,7 +429,9 @@ attn_pack_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 #pragma unroll
         for (int i = 0; i < 32; ++i) r0[i] = r1[i] = 0u;
       }
-      if (row < tile.rows) {
+      if (lim >= 0) {
+        const QTile tile = tile_of(it);
+        const int h = head_of(it);
         const bool none = lim == 0;                              // (its sum is not quite 0: the polynomial gives 2^-126 for masked keys)
         const float inv = 1.0f / l_run;
         uint32_t w[32];

@@ -10,47 +10,53 @@
 // memory, in a fixed order.  One pass would add dQ from every key tile to memory by atomics, 32 KB per pair of tiles, in an order that changes
 // from run to run.
 //
-//   CTA      one per SM, persistent over (tile, head) items, the longest first; steps of 128 passing rows
-//   roles    warps 0..7: a thread takes 64 of the 128 columns of one row: S and dP from tensor memory, P and dS in registers, as 16-bit pairs
-//            back over S; warp 8: TMA (row operands in two buffers, passing operands in a ring of four); warp 9: products; warps 10, 11
-//            (ROWS = queries): log-sum-exp and delta of the rows of the next item, also for the second launch
-//   pipeline two S buffers, one dP buffer, the accumulators: S(G + 1) is issued before the end of step G, dP(G + 1) when dP(G) has been read,
-//            the gradients' products of step G behind them
-//   ROWS = keys takes the log-sum-exp and delta of its passing rows from a table with a line of 128 per query tile, +inf where there is no row:
-//            P is 0 there
-//   numerics P and dS are rounded to the 16-bit type of the operands (the products' A operand); everything else fp32
+//   CTA      one per SM, persistent over (tile, head) items, the longest first; steps of 96 passing rows
+//   roles    two groups of four warps take the steps in turn, a thread a row: S and dP from tensor memory, P and dS as 16-bit pairs back over
+//            dP; warp 8: TMA (row operands in two buffers, passing operands in a ring); warps 9, 10, 11: the products S, dP and those of the
+//            gradients; warp 12 (ROWS = queries): log-sum-exp and delta of the rows of the next item, also for the second launch
+//   pipeline two S buffers, two dP buffers, the accumulators (2 x 96 + 2 x 96 + 2 x 64 columns).  A group reads its whole S row at once, so
+//            S(G + 2) is issued while it works on step G; dP(G + 2) goes behind the gradients' products of step G, which read P and dS from
+//            the same buffer, and is needed when the exponentials of step G + 2 are done.  The group of an item's last step writes the
+//            item's gradients, the other one goes on with the next item.
+//   numerics P and dS are rounded to the 16-bit type of the operands (the products' A operand); everything else fp32; three of every four pairs of
+//            exponentials by the special-function unit, the fourth on the FMA pipe
 #include "kf_attn.cuh"
 
 namespace kf {
 
-constexpr int PB_T = 128, PB_D = 64;
-constexpr int PB_THREADS = 384;
-constexpr int PB_REGS_WORK = 208, PB_REGS_LEAN = 88;           // 256 * 208 + 128 * 88 = 384 * 168, the allocation at launch
-constexpr int PB_REGS_LAUNCH = 168;
-static_assert(256 * PB_REGS_WORK + 128 * PB_REGS_LEAN <= PB_THREADS * PB_REGS_LAUNCH, "register split");
-constexpr int PB_RING = 4;
-constexpr int PB_TILE = PB_T * PB_D * 2;                       // 16 KB
-constexpr int PB_OFF_C = 4 * PB_TILE;                          // row operands: two buffers of two tiles; then the ring: two tiles per stage
-constexpr int PB_OFF_STAT = PB_OFF_C + PB_RING * 2 * PB_TILE;  // per ring stage (ROWS = keys) or item buffer: lse2[128], delta[128]
-constexpr int PB_OFF_BAR = PB_OFF_STAT + PB_RING * 1024;
-constexpr size_t PB_SMEM = (size_t)PB_OFF_BAR + 512;
-constexpr int PB_COL_S = 0, PB_COL_DP = 256, PB_COL_A1 = 384, PB_COL_A2 = 448, PB_TMEM_COLS = 512;
+constexpr int PB_T = 128, PB_W = 96, PB_D = 64;                // rows of a tile that stays, rows of a passing one
+constexpr int PB_THREADS = 512;
+constexpr int PB_REGS_WORK = 208, PB_REGS_LEAN = 48;
+constexpr int PB_REGS_LAUNCH = 128;
+static_assert(256 * PB_REGS_WORK + 256 * PB_REGS_LEAN <= PB_THREADS * PB_REGS_LAUNCH, "register split");
+constexpr int PB_RTILE = PB_T * PB_D * 2, PB_CTILE = PB_W * PB_D * 2;     // 16 KB, 12 KB
+// Shared memory: row operands in two buffers (with ROWS = queries also O, for delta), a ring of passing ones, the rows' log-sum-exp and delta
+// (1 KB per stage, or per item buffer), barriers.
+template <bool KEYS>
+struct BwdMem {
+  static constexpr int RING = KEYS ? 6 : 5, RTILES = KEYS ? 2 : 3;
+  static constexpr int OFF_C = 2 * RTILES * PB_RTILE, OFF_STAT = OFF_C + RING * 2 * PB_CTILE, OFF_BAR = OFF_STAT + (KEYS ? RING : 2) * 1024;
+  static constexpr size_t BYTES = (size_t)OFF_BAR + 512;
+  static_assert(BYTES <= 227 * 1024, "shared memory");
+};
+constexpr int PB_COL_S = 0, PB_COL_D = 2 * PB_W, PB_COL_A1 = 4 * PB_W, PB_COL_A2 = PB_COL_A1 + PB_D, PB_TMEM_COLS = 512;
+static_assert(PB_COL_A2 + PB_D <= PB_TMEM_COLS, "TMEM budget");
+constexpr int PB_POLY_K = 3;                                   // element pairs PB_POLY_K .. 3 of every four take the polynomial exponential
 
 struct PackBwdArgs {
   const int4* tiles;
   int n_items, heads, share;     // heads of an item: query heads (ROWS = queries) or key heads
   float scale, scale_log2, cap_in, cap_out;
   const float* slopes;
-  float* stats;                  // [Hq][n_q_tiles][2][128]
-  int n_q_tiles;
+  float *lse2, *delta;           // [Hq][n_q_tiles * 128], a sequence's rows from its first tile's slot on
+  int64_t stat_ld;
   // ROWS = queries
-  const void *O, *dO;
-  int64_t o_st, o_sh, do_st, do_sh;
   const float* lse;
   int64_t lse_ld;
   // outputs: dQ, or dK and dV
   void *g1, *g2;
   int64_t g1_st, g1_sh, g2_st, g2_sh;
+  int wide;                      // rows of the outputs are 32-byte aligned
   unsigned int* err;
 };
 
@@ -70,76 +76,81 @@ struct BwdItem<false> {
   __device__ __forceinline__ void load(const PackBwdArgs& a, int item) {
     t = load_tile<QTile>(a.tiles, item / a.heads);
     head = item % a.heads;
-    n = (t.limit(t.rows - 1) + PB_T - 1) / PB_T;
+    n = (t.limit(t.rows - 1) + PB_W - 1) / PB_W;
   }
   __device__ __forceinline__ int rows() const { return t.rows; }
   __device__ __forceinline__ int row0() const { return t.row; }
-  __device__ __forceinline__ int slot(int) const { return t.slot; }
+  __device__ __forceinline__ int slot() const { return t.slot; }
 };
 template <>
 struct BwdItem<true> {
   KTile t;
-  int head, n, per, first;                                      // per: query tiles per query head, from tile `first` of the sequence on
+  int head, n, per, first;                                      // per: passing tiles per query head, from tile `first` of the sequence on
   __device__ __forceinline__ void load(const PackBwdArgs& a, int item) {
     t = load_tile<KTile>(a.tiles, item / a.heads);
     head = item % a.heads;
-    first = t.lowest(0) / PB_T;
-    const int tiles = (t.q_len + PB_T - 1) / PB_T;
+    first = t.lowest(0) / PB_W;
+    const int tiles = (t.q_len + PB_W - 1) / PB_W;
     per = tiles > first ? tiles - first : 0;
     n = per * a.share;
   }
   __device__ __forceinline__ int rows() const { return t.rows; }
   __device__ __forceinline__ int row0() const { return t.row; }
-  __device__ __forceinline__ int slot(int tile) const { return t.slot0 + tile; }
+  __device__ __forceinline__ int slot() const { return t.slot0; }
 };
 // Where a step's passing tile lies: first row in the batch, head, index of its first row in the sequence, rows that belong to the sequence.
 struct BwdStep {
-  int row, head, index, valid, tile;
+  int row, head, index, valid;
 };
 __device__ __forceinline__ BwdStep step_of(const PackBwdArgs& a, const BwdItem<false>& i, int j) {
-  return {i.t.k_row + j * PB_T, i.head / a.share, j * PB_T, i.t.k_len - j * PB_T, 0};
+  return {i.t.k_row + j * PB_W, i.head / a.share, j * PB_W, i.t.k_len - j * PB_W};
 }
 __device__ __forceinline__ BwdStep step_of(const PackBwdArgs& a, const BwdItem<true>& i, int j) {
   const int hh = j / i.per, qt = i.first + j - hh * i.per;
-  return {i.t.q_row + qt * PB_T, i.head * a.share + hh, qt * PB_T, i.t.q_len - qt * PB_T, qt};
+  return {i.t.q_row + qt * PB_W, i.head * a.share + hh, qt * PB_W, i.t.q_len - qt * PB_W};
 }
 
 template <int F16, bool KEYS, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(PB_THREADS, 1)
-attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constant__ CUtensorMap tmR2, const __grid_constant__ CUtensorMap tmC1,
-                     const __grid_constant__ CUtensorMap tmC2, const __grid_constant__ PackBwdArgs a) {
+attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constant__ CUtensorMap tmR2, const __grid_constant__ CUtensorMap tmR3,
+                     const __grid_constant__ CUtensorMap tmC1, const __grid_constant__ CUtensorMap tmC2, const __grid_constant__ PackBwdArgs a) {
+  using Mem = BwdMem<KEYS>;
+  constexpr int PB_RING = Mem::RING, RTILES = Mem::RTILES, PB_OFF_C = Mem::OFF_C, PB_OFF_STAT = Mem::OFF_STAT, PB_OFF_BAR = Mem::OFF_BAR;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + PB_OFF_BAR);
   uint64_t *r_full = bars, *r_empty = r_full + 2, *c1_full = r_empty + 2, *c2_full = c1_full + PB_RING, *c_empty = c2_full + PB_RING, *st_full = c_empty + PB_RING,
-           *st_empty = st_full + PB_RING, *s_full = st_empty + 2, *ds_full = s_full + 2, *dp_full = ds_full + 2, *dp_free = dp_full + 1, *acc_full = dp_free + 1;
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(acc_full + 1);
+           *st_empty = st_full + PB_RING, *s_full = st_empty + 2, *s_free = s_full + 2, *dp_full = s_free + 2, *ds_full = dp_full + 2, *d_free = ds_full + 2,
+           *acc_full = d_free + 2, *acc_free = acc_full + 2;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(acc_free + 1);
   volatile uint32_t* abort_flag = tmem_holder + 1;
 
   pdl_launch_dependents();
   const int warp = warp_index(), lane = threadIdx.x & 31;
-  const int n_my = (int)blockIdx.x < a.n_items ? (a.n_items - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x : 0;
+  const int n_my = items_of_cta(a.n_items);
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&r_full[i], 1);
-      mbar_init(&r_empty[i], 1);
+      mbar_init(&r_empty[i], RTILES);                             // S, dP, and whoever reads O
       mbar_init(&s_full[i], 1);
-      mbar_init(&ds_full[i], 256);
+      mbar_init(&s_free[i], 128);
+      mbar_init(&dp_full[i], 1);
+      mbar_init(&ds_full[i], 128);
+      mbar_init(&d_free[i], 1);
       mbar_init(&st_empty[i], 256);
+      mbar_init(&acc_full[i], 1);                                // items in turn: a group may ask for its item before the other's is complete
     }
     for (int i = 0; i < PB_RING; ++i) {
       mbar_init(&c1_full[i], 1);
       mbar_init(&c2_full[i], 1);
       mbar_init(&c_empty[i], 1);
-      mbar_init(&st_full[i], KEYS ? 1 : 64);
+      mbar_init(&st_full[i], 1);
     }
-    mbar_init(dp_full, 1);
-    mbar_init(dp_free, 256);
-    mbar_init(acc_full, 1);
+    mbar_init(acc_free, 128);
     *abort_flag = 0u;
     fence_mbar_init();
   }
-  if (warp == 9) {
+  if (warp == 9) {                                         // (the whole warp)
     tmem_alloc(tmem_holder, PB_TMEM_COLS);
     tmem_relinquish();
   }
@@ -147,7 +158,7 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
   __syncthreads();
   tc_fence_after();
   pdl_wait();
-  const uint32_t tmem_base = *tmem_holder;
+  const uint32_t tmem_base = (uint32_t)uniform_int((int)*tmem_holder);
   const WaitCtx ctx{abort_flag, a.err};
   const bool bad_align = (smem_u32(smem) & 1023u) != 0;
   if (bad_align && threadIdx.x == 0 && atomicCAS(&a.err[0], 0u, 99u) == 0u) {
@@ -155,7 +166,7 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
     a.err[2] = blockIdx.x;
   }
   using Item = BwdItem<KEYS>;
-  auto load_item = [&](Item& i, int it) { i.load(a, (int)blockIdx.x + it * (int)gridDim.x); };
+  auto load_item = [&](Item& i, int it) { i.load(a, item_of_cta(it)); };
 
   if (warp >= 8) {
   setmaxnreg_dec<PB_REGS_LEAN>();
@@ -179,10 +190,11 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
       const uint32_t rb = ri & 1;
       if (!mbar_wait_warp(&r_empty[rb], ((ri >> 1) & 1) ^ 1, ctx, 60)) break;
       if (elect_one()) {
-        uint8_t* to = smem + rb * 2 * PB_TILE;
-        mbar_expect_tx(&r_full[rb], 2 * PB_TILE);
+        uint8_t* to = smem + rb * RTILES * PB_RTILE;
+        mbar_expect_tx(&r_full[rb], RTILES * PB_RTILE);
         tma_load_3d(to, &tmR1, 0, I.head, I.row0(), &r_full[rb]);
-        tma_load_3d(to + PB_TILE, &tmR2, 0, I.head, I.row0(), &r_full[rb]);
+        tma_load_3d(to + PB_RTILE, &tmR2, 0, I.head, I.row0(), &r_full[rb]);
+        if (!KEYS) tma_load_3d(to + 2 * PB_RTILE, &tmR3, 0, I.head, I.row0(), &r_full[rb]);
       }
       __syncwarp();
       ++ri;
@@ -190,15 +202,17 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
         const BwdStep s = step_of(a, I, j);
         if (!mbar_wait_warp(&c_empty[st], ph, ctx, 61)) { ok = false; break; }
         if (elect_one()) {
-          uint8_t* to = smem + PB_OFF_C + st * 2 * PB_TILE;
-          mbar_expect_tx(&c1_full[st], PB_TILE);
+          uint8_t* to = smem + PB_OFF_C + st * 2 * PB_CTILE;
+          mbar_expect_tx(&c1_full[st], PB_CTILE + (KEYS ? 2 * PB_W * 4 : 0));
           tma_load_3d(to, &tmC1, 0, s.head, s.row, &c1_full[st]);
-          if (KEYS) {
-            mbar_expect_tx(&st_full[st], 1024);
-            bulk_load_1d(smem + PB_OFF_STAT + st * 1024, a.stats + ((size_t)s.head * a.n_q_tiles + I.slot(s.tile)) * 256, 1024, &st_full[st]);
+          if (KEYS) {                                                         // 96 values each; what is behind the sequence's end is put right by the issuer
+            const int64_t at = s.head * a.stat_ld + (int64_t)I.slot() * PB_T + s.index;
+            uint8_t* sm = smem + PB_OFF_STAT + st * 1024;
+            bulk_load_1d(sm, a.lse2 + at, PB_W * 4, &c1_full[st]);
+            bulk_load_1d(sm + 512, a.delta + at, PB_W * 4, &c1_full[st]);
           }
-          mbar_expect_tx(&c2_full[st], PB_TILE);
-          tma_load_3d(to + PB_TILE, &tmC2, 0, s.head, s.row, &c2_full[st]);
+          mbar_expect_tx(&c2_full[st], PB_CTILE);
+          tma_load_3d(to + PB_CTILE, &tmC2, 0, s.head, s.row, &c2_full[st]);
         }
         __syncwarp();
         if (++st == PB_RING) {
@@ -207,344 +221,370 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
         }
       }
     }
-  } else if (warp == 9) {
-    // ------------------------------------------------------------------ MMA issuer
-    const uint32_t fmt = F16 ? 0u : 1u;
-    const uint32_t idesc_s = idesc_f16(fmt, PB_T), idesc_a = idesc_f16(fmt, PB_D) | (1u << 16);     // the passing operand of a gradient is MN-major
+  } else if (warp <= 11) {
+    // ------------------------------------------------------------------ MMA issuers: warp 9 S, warp 10 dP, warp 11 the gradients
+    // One warp for all three spent 1700 clk per step on waiting, addresses and issue, twice the time of the products.
+    // Everything the products take is worked out by the whole warp, in front of the branch that one lane takes: behind it each address would
+    // be one lane's, moved to a uniform register in front of every instruction.
     const bool leader = elect_one();
-    struct Cursor {
-      Item i;
-      int it, j;
-      uint32_t ri;                                                            // items with steps so far
-    };
-    auto settle = [&](Cursor& c) {
-      c.j = 0;
-      for (; c.it < n_my; ++c.it) {
-        load_item(c.i, c.it);
-        if (c.i.n > 0) return;
+    int it = 0, next_n = -1, next_per = 0, next_rows = 0;                     // the item behind this one is asked for ahead
+    auto fetch = [&]() {
+      next_n = -1;
+      if (it < n_my) {
+        Item I;
+        load_item(I, it++);
+        next_n = I.n;
+        if constexpr (KEYS) {
+          next_per = I.per;
+          next_rows = I.t.q_len - I.first * PB_W;
+        } else {
+          next_per = I.n;
+          next_rows = I.t.k_len;
+        }
       }
     };
-    auto advance = [&](Cursor& c) {
-      if (++c.j == c.i.n) {
-        ++c.it;
-        ++c.ri;
-        settle(c);
-      }
+    int j, n, jj, per, rows;                                                  // step of the item and their number (-1: no item left); step of the sequence, their number, its rows
+    uint32_t G = 0, ri = 0, st = 0, ph = 0;                                   // steps and items before, ring stage and its parity
+    auto open = [&]() {                                                       // the next item that has steps
+      do {
+        n = uniform_int(next_n);
+        per = uniform_int(next_per);
+        rows = uniform_int(next_rows);
+        fetch();
+      } while (n == 0);
+      j = jj = 0;
     };
-    Cursor x;                                                                 // the next S and dP products
-    x.it = 0;
-    x.ri = 0;
-    settle(x);
-    uint32_t x_st = 0, x_ph = 0;                                              // their ring stage
-    uint32_t G = 0;                                                           // steps whose S has been issued
-    bool ok = true;
-    auto product = [&](uint32_t t_d, uint32_t which) {                        // row operand `which` times the passing one, 128 x 128 x 64
-      const uint64_t rdesc = smem_desc_sw128(smem_u32(smem + ((x.ri & 1) * 2 + which) * PB_TILE));
-      const uint64_t cdesc = smem_desc_sw128(smem_u32(smem + PB_OFF_C + (x_st * 2 + which) * PB_TILE));
-#pragma unroll
-      for (int kk = 0; kk < PB_D / 16; ++kk) mma_f16(t_d, rdesc + 2 * kk, cdesc + 2 * kk, idesc_s, kk != 0);
-    };
-    auto issue_s = [&]() {
-      ok = (x.j != 0 || mbar_wait_warp(&r_full[x.ri & 1], (x.ri >> 1) & 1, ctx, 62)) && mbar_wait_warp(&c1_full[x_st], x_ph, ctx, 63);
-      if (!ok) return;
-      const int valid = step_of(a, x.i, x.j).valid;
-      if (valid < PB_T) zero_rows(smem + PB_OFF_C + x_st * 2 * PB_TILE, valid, PB_T, lane);
-      tc_fence_after();
-      if (leader) {
-        product(tmem_base + PB_COL_S + (G & 1) * PB_T, 0);
-        tc_commit(&s_full[G & 1]);
-      }
-      __syncwarp();
-    };
-    auto issue_dp = [&]() {                                                   // and on to the next step
-      ok = mbar_wait_warp(&c2_full[x_st], x_ph, ctx, 64) && (G == 0 || mbar_wait_warp(dp_free, (G - 1) & 1, ctx, 65));
-      if (!ok) return;
-      const int valid = step_of(a, x.i, x.j).valid;
-      if (valid < PB_T) zero_rows(smem + PB_OFF_C + (x_st * 2 + 1) * PB_TILE, valid, PB_T, lane);
-      tc_fence_after();
-      if (leader) {
-        product(tmem_base + PB_COL_DP, 1);
-        tc_commit(dp_full);
-      }
-      __syncwarp();
+    auto advance = [&]() {
       ++G;
-      if (++x_st == PB_RING) {
-        x_st = 0;
-        x_ph ^= 1;
+      if (++st == PB_RING) {
+        st = 0;
+        ph ^= 1;
+      }
+      if (++jj == per) jj = 0;
+      if (++j == n) {
+        ++ri;
+        open();
       }
     };
-    int a_j = 0, a_n = x.it < n_my ? x.i.n : 0;                               // the gradients' products: step and number of steps of their item
-    uint32_t a_ri = 0, a_st = 0, A = 0;
-    bool more = x.it < n_my;
-    if (more) {
-      issue_s();
-      if (ok) issue_dp();
-      if (ok) advance(x);
-    }
-    while (more && ok) {
-      const bool next = x.it < n_my;
-      const int n_next = x.j == 0 ? x.i.n : 0;                                // the item of step A + 1, where that is its first
-      if (next) {
-        issue_s();
-        if (ok) issue_dp();
-        if (!ok) break;
-        advance(x);
-      }
-      if (!mbar_wait_warp(&ds_full[A & 1], (A >> 1) & 1, ctx, 66)) break;
-      tc_fence_after();
-      if (leader) {
-        const uint32_t t_p = tmem_base + PB_COL_S + (A & 1) * PB_T;
-        const uint64_t c1 = smem_desc_sw128(smem_u32(smem + PB_OFF_C + a_st * 2 * PB_TILE)), c2 = smem_desc_sw128(smem_u32(smem + PB_OFF_C + (a_st * 2 + 1) * PB_TILE));
+    fetch();
+    open();
+    const uint32_t fmt = F16 ? 0u : 1u;
+    if (warp < 11) {
+      // row operand `which` times the passing one, 128 x 96 x 64, into the buffer that the step before the last has left
+      const uint32_t which = warp - 9;
+      const uint32_t idesc = idesc_f16(fmt, PB_W), col = which ? PB_COL_D : PB_COL_S;
+      uint64_t *const c_full = which ? c2_full : c1_full, *const room = which ? d_free : s_free, *const full = which ? dp_full : s_full;
+      while (n > 0) {
+        const uint32_t b = G & 1, b_ph = ((G >> 1) & 1) ^ 1;
+        if (j == 0 && !mbar_wait_warp(&r_full[ri & 1], (ri >> 1) & 1, ctx, 62)) break;
+        if (!mbar_wait_warp3(&c_full[st], ph, &room[b], b_ph, &room[b], b_ph, ctx, 63)) break;
+        uint8_t* const tile = smem + PB_OFF_C + (st * 2 + which) * PB_CTILE;
+        const int valid = rows - jj * PB_W;
+        if (valid < PB_W) {                                                   // what the tile holds behind the end of the sequence becomes zero
+          if (KEYS && which == 0) {                                           // the rows' values there: P = 0
+            float* sm = reinterpret_cast<float*>(smem + PB_OFF_STAT + st * 1024);
+            for (int i = valid + lane; i < PB_W; i += 32) {
+              sm[i] = INFINITY;
+              sm[128 + i] = 0.f;
+            }
+          }
+          zero_rows(tile, valid, PB_W, lane);
+        }
+        if (KEYS && which == 0 && lane == 0) mbar_arrive(&st_full[st]);
+        const uint32_t d = tmem_base + col + b * PB_W;
+        const uint64_t r = smem_desc_sw128(smem_u32(smem + ((ri & 1) * RTILES + which) * PB_RTILE)), p = smem_desc_sw128(smem_u32(tile));
+        uint64_t *const done = &full[b], *const r_done = &r_empty[ri & 1];
+        const bool last = j + 1 == n;
+        tc_fence_after();
+        if (leader) {
 #pragma unroll
-        for (int kk = 0; kk < PB_T / 16; ++kk) {                              // 16 columns: 8 words of the half that their threads wrote
-          const uint32_t p = t_p + (kk >> 2) * 64 + (kk & 3) * 8;
-          if (KEYS) mma_f16_ta(tmem_base + PB_COL_A2, p, c2 + (uint64_t)(kk * (2048 >> 4)), idesc_a, (a_j | kk) != 0);
-          mma_f16_ta(tmem_base + PB_COL_A1, p + 32, c1 + (uint64_t)(kk * (2048 >> 4)), idesc_a, (a_j | kk) != 0);
+          for (int kk = 0; kk < PB_D / 16; ++kk) mma_f16(d, r + 2 * kk, p + 2 * kk, idesc, kk != 0);
+          tc_commit(done);
+          if (last) tc_commit(r_done);
         }
-        tc_commit(&c_empty[a_st]);
-        if (a_j + 1 == a_n) {
-          tc_commit(acc_full);
-          tc_commit(&r_empty[a_ri & 1]);
+        __syncwarp();
+        advance();
+      }
+    } else {
+      const uint32_t idesc = idesc_f16(fmt, PB_D) | (1u << 16);               // the passing operand is MN-major
+      while (n > 0) {
+        const uint32_t b = G & 1;
+        if (!mbar_wait_warp(&ds_full[b], (G >> 1) & 1, ctx, 67)) break;
+        if (j == 0 && ri > 0 && !mbar_wait_warp(acc_free, (ri - 1) & 1, ctx, 68)) break;   // the last item's gradients have been read
+        tc_fence_after();
+        const uint32_t t_d = tmem_base + PB_COL_D + b * PB_W;
+        const uint64_t c1 = smem_desc_sw128(smem_u32(smem + PB_OFF_C + st * 2 * PB_CTILE)), c2 = c1 + (PB_CTILE >> 4);
+        uint64_t *const c_done = &c_empty[st], *const d_done = &d_free[b], *const a_done = &acc_full[ri & 1];
+        const bool last = j + 1 == n;
+        const uint32_t more = j != 0;
+        if (leader) {
+#pragma unroll
+          for (int kk = 0; kk < PB_W / 16; ++kk) {                            // 32 columns of dP hold 16 words of dS and 16 of P
+            const uint32_t d = t_d + (kk >> 1) * 32 + (kk & 1) * 8;
+            if (KEYS) mma_f16_ta(tmem_base + PB_COL_A2, d + 16, c2 + (uint64_t)(kk * (2048 >> 4)), idesc, kk ? 1u : more);
+            mma_f16_ta(tmem_base + PB_COL_A1, d, c1 + (uint64_t)(kk * (2048 >> 4)), idesc, kk ? 1u : more);
+          }
+          tc_commit(d_done);
+          tc_commit(c_done);
+          if (last) tc_commit(a_done);
         }
+        __syncwarp();
+        advance();
       }
-      __syncwarp();
-      ++A;
-      if (++a_st == PB_RING) a_st = 0;
-      if (++a_j == a_n) {
-        a_j = 0;
-        a_n = n_next;
-        ++a_ri;
-      }
-      more = next;
     }
-  } else if (!KEYS) {
-    // ------------------------------------------------------------------ log-sum-exp and delta of the rows: two per thread
-    bool ok = true;
-    for (int it = 0; it < n_my && ok; ++it) {
+  } else if (!KEYS && warp == 12) {
+    // ------------------------------------------------------------------ log-sum-exp and delta of the rows: four per lane, dO and O from shared memory
+    uint32_t ri = 0;
+    for (int it = 0; it < n_my; ++it) {
       Item I;
       load_item(I, it);
       const int b = it & 1;
-      ok = mbar_wait_warp(&st_empty[b], ((it >> 1) & 1) ^ 1, ctx, 67);
-      if (!ok) break;
-      float* sm = reinterpret_cast<float*>(smem + PB_OFF_STAT + b * 1024);
-      float* gl = a.stats + ((size_t)I.head * a.n_q_tiles + I.slot(0)) * 256;
-#pragma unroll 1
-      for (int r = (warp - 10) * 32 + lane; r < PB_T; r += 64) {
-        float lse2 = INFINITY, delta = 0.f;
-        if (r < I.rows()) {
-          const int64_t row = I.row0() + r;
-          const float l = __ldg(a.lse + (int64_t)I.head * a.lse_ld + row);
-          if (l != -INFINITY) lse2 = l * 1.4426950408889634f;
-          const uint4* o = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.O) + 2 * (row * a.o_st + (int64_t)I.head * a.o_sh));
-          const uint4* d = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.dO) + 2 * (row * a.do_st + (int64_t)I.head * a.do_sh));
+      const float* l = a.lse + (int64_t)I.head * a.lse_ld + I.row0();
+      float lse2[4], delta[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) lse2[k] = 32 * k + lane < I.rows() ? __ldg(l + 32 * k + lane) : -INFINITY;
+      if (I.n > 0) {
+        if (!mbar_wait_warp(&r_full[ri & 1], (ri >> 1) & 1, ctx, 65)) break;
+        const uint8_t* d = smem + ((ri & 1) * RTILES + 1) * PB_RTILE;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int r = 32 * k + lane;
           float2 s = make_float2(0.f, 0.f);
 #pragma unroll
-          for (int i = 0; i < PB_D / 8; ++i) {
-            const uint4 u = __ldg(o + i), v = __ldg(d + i);
-            const uint32_t uw[4] = {u.x, u.y, u.z, u.w}, vw[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) s = fma2(unpack16<F16>(uw[k]), unpack16<F16>(vw[k]), s);
+          for (int c = 0; c < 8; ++c) {
+            const int at = r * 128 + ((c ^ (r & 7)) << 4);                    // the swizzle of the tile
+            const uint4 u = *reinterpret_cast<const uint4*>(d + at), v = *reinterpret_cast<const uint4*>(d + PB_RTILE + at);
+            s = fma2(unpack16<F16>(u.x), unpack16<F16>(v.x), s);
+            s = fma2(unpack16<F16>(u.y), unpack16<F16>(v.y), s);
+            s = fma2(unpack16<F16>(u.z), unpack16<F16>(v.z), s);
+            s = fma2(unpack16<F16>(u.w), unpack16<F16>(v.w), s);
           }
-          delta = s.x + s.y;
+          if (r < I.rows()) delta[k] = s.x + s.y;
         }
-        sm[r] = lse2;
-        sm[128 + r] = delta;
-        gl[r] = lse2;
-        gl[128 + r] = delta;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&r_empty[ri & 1]);
+        ++ri;
       }
-      mbar_arrive(&st_full[b]);
+      if (!mbar_wait_warp(&st_empty[b], ((it >> 1) & 1) ^ 1, ctx, 69)) break;
+      float* sm = reinterpret_cast<float*>(smem + PB_OFF_STAT + b * 1024);
+      const int64_t at = I.head * a.stat_ld + (int64_t)I.slot() * PB_T;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int r = 32 * k + lane;
+        lse2[k] = lse2[k] == -INFINITY ? INFINITY : lse2[k] * 1.4426950408889634f;
+        sm[r] = a.lse2[at + r] = lse2[k];
+        sm[128 + r] = a.delta[at + r] = delta[k];
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&st_full[b]);
     }
   }
   } else {
     setmaxnreg_inc<PB_REGS_WORK>();
     if (!bad_align) {
-    // ------------------------------------------------------------------ thread = half a row
-    const int wg = warp >> 2, row = (warp & 3) * 32 + lane, c0 = wg * 64;
+    // ------------------------------------------------------------------ a thread a row, the groups take the steps in turn
+    const uint32_t wg = warp >> 2;
+    const int row = (warp & 3) * 32 + lane;
     const uint32_t t_lane = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t t_s = t_lane + PB_COL_S + wg * PB_W, t_d = t_lane + PB_COL_D + wg * PB_W;     // step G uses buffer G & 1, which is the group
     bool ok = true;
-    uint32_t G = 0, st = 0, st_ph = 0, acc_ph = 0;
+    uint32_t G0 = 0, ph = 0, acc_n = 0;                          // steps before this item; parity of this group's next step; items with steps
+    uint32_t st = wg, st_ph = 0;                                 // ring stage of this group's next step and its parity
     for (int it = 0; it < n_my && ok; ++it) {
       Item I;
       load_item(I, it);
-      float lse2 = 0.f, delta = 0.f;
+      float nlse2 = 0.f, ndelta = 0.f;
       if (!KEYS) {
-        if (!mbar_wait_warp(&st_full[it & 1], (it >> 1) & 1, ctx, 68)) { ok = false; break; }
+        if (!mbar_wait_warp(&st_full[it & 1], (it >> 1) & 1, ctx, 69)) break;
         const float* sm = reinterpret_cast<const float*>(smem + PB_OFF_STAT + (it & 1) * 1024);
-        lse2 = sm[row];
-        delta = sm[128 + row];
+        nlse2 = -sm[row];
+        ndelta = -sm[128 + row];
         mbar_arrive(&st_empty[it & 1]);
       }
-      // ROWS = queries: columns below `edge` are seen; ROWS = keys: columns from `edge` on
+      // ROWS = queries: the row sees columns below `edge`; ROWS = keys: from `edge` on
       int edge, warp_edge;
-      float at;
+      float at;                                                  // ROWS = queries: position; ROWS = keys: the query that stands at the key
       if constexpr (KEYS) {
         edge = row < I.rows() ? I.t.lowest(row) : 0;
         warp_edge = I.t.lowest((warp & 3) * 32 + 31);            // the largest of the warp's
-        at = (float)(I.t.first + row - I.t.off);                 // the query at whose position the key is
+        at = (float)(I.t.first + row - I.t.off);
       } else {
         edge = row < I.rows() ? I.t.limit(row) : 0x7fffffff;
         warp_edge = I.t.limit((warp & 3) * 32);
         at = (float)(I.t.pos + row);
       }
       float slope = 0.f;
-      for (int j = 0; j < I.n; ++j, ++G) {
-        const BwdStep s = step_of(a, I, j);
-        const uint32_t buf = G & 1, t_s = t_lane + PB_COL_S + buf * PB_T + c0;
-        if (BIAS && (KEYS || j == 0)) slope = __ldg(a.slopes + (KEYS ? s.head : I.head)) * 1.4426950408889634f;
-        uint32_t p[64];
-        if (!mbar_wait_warp(&s_full[buf], (G >> 1) & 1, ctx, 69)) { ok = false; break; }
+      if (BIAS && !KEYS) slope = __ldg(a.slopes + I.head) * 1.4426950408889634f;
+      const int n = I.n;
+      int index, end, head = 0;                                  // of the passing rows: first one in its sequence, end of the sequence, head
+      if constexpr (KEYS) {
+        index = I.first * PB_W;
+        end = I.t.q_len;
+        head = I.head * a.share;
+      } else {
+        index = 0;
+        end = 0x7fffffff;
+      }
+      auto move = [&](int steps) {                               // from one query head to the next one that shares the keys
+        index += steps * PB_W;
+        if constexpr (KEYS) {
+          while (index >= end && head + 1 < (I.head + 1) * a.share) {
+            index -= I.per * PB_W;
+            ++head;
+          }
+        }
+      };
+      const int j0 = (int)((G0 + wg) & 1);
+      if (j0 < n) move(j0);
+      for (int j = j0; j < n; j += 2, move(2)) {
+        if (BIAS && KEYS) slope = __ldg(a.slopes + head) * 1.4426950408889634f;
+        uint32_t p[96];
+        if (!mbar_wait_warp(&s_full[wg], ph, ctx, 70)) { ok = false; break; }
         tc_fence_after();
         {
           uint32_t(&p0)[32] = *reinterpret_cast<uint32_t(*)[32]>(p);
           uint32_t(&p1)[32] = *reinterpret_cast<uint32_t(*)[32]>(p + 32);
+          uint32_t(&p2)[32] = *reinterpret_cast<uint32_t(*)[32]>(p + 64);
           tmem_ld32(t_s, p0);
           tmem_ld32(t_s + 32, p1);
+          tmem_ld32(t_s + 64, p2);
           tmem_ld_wait();
           tmem_ld_fence(p0);
           tmem_ld_fence(p1);
+          tmem_ld_fence(p2);
         }
-        const float* stat = reinterpret_cast<const float*>(smem + PB_OFF_STAT + st * 1024) + c0;
-        if (KEYS && !mbar_wait_warp(&st_full[st], st_ph, ctx, 70)) { ok = false; break; }
-        const float gap = at - (float)(s.index + c0);
+        if (!CAP) {
+          tc_fence_before();
+          mbar_arrive(&s_free[wg]);
+        }
+        const float* stat = reinterpret_cast<const float*>(smem + PB_OFF_STAT + st * 1024);
+        if (KEYS && !mbar_wait_warp(&st_full[st], st_ph, ctx, 71)) { ok = false; break; }
+        const float gap = at - (float)index;
 #pragma unroll
-        for (int i = 0; i < 64; i += 4) {
-          float2 l[2];
+        for (int i = 0; i < 96; i += 8) {
+          uint32_t f[8];                                         // with a cap: 1 - tanh^2 = 4 r (1 - r), r = 1 / (1 + e^2y)
+          float v[8];
           if (KEYS) {
-            const float4 v = *reinterpret_cast<const float4*>(stat + i);
-            l[0] = make_float2(-v.x, -v.y);
-            l[1] = make_float2(-v.z, -v.w);
-          } else {
-            l[0] = l[1] = splat2(-lse2);
+            *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(stat + i);
+            *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(stat + i + 4);
           }
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
+          for (int k = 0; k < 4; ++k) {
             const int c = i + 2 * k;
+            float2 l = KEYS ? make_float2(-v[2 * k], -v[2 * k + 1]) : splat2(nlse2);
             float2 x = make_float2(__uint_as_float(p[c]), __uint_as_float(p[c + 1]));
             if constexpr (CAP) {
-              const float2 rc = make_float2(rcp_approx(1.f + ex2(x.x * a.cap_in)), rcp_approx(1.f + ex2(x.y * a.cap_in)));
-              x = fma2(rc, splat2(-2.f * a.cap_out), splat2(a.cap_out));
+              const float2 r = make_float2(rcp_approx(1.f + ex2(x.x * a.cap_in)), rcp_approx(1.f + ex2(x.y * a.cap_in)));
+              const float2 r4 = mul2(r, splat2(4.f));
+              const float2 d = fma2(make_float2(-r4.x, -r4.y), r, r4);
+              f[2 * k] = __float_as_uint(d.x);
+              f[2 * k + 1] = __float_as_uint(d.y);
+              x = fma2(r, splat2(-2.f * a.cap_out), splat2(a.cap_out));
             } else if constexpr (BIAS) {
               x = mul2(x, splat2(a.scale_log2));
             }
             if constexpr (BIAS) {
-              l[k].x = fmaf(-slope, fabsf(gap - (float)c), l[k].x);
-              l[k].y = fmaf(-slope, fabsf(gap - (float)(c + 1)), l[k].y);
+              l.x = fmaf(-slope, fabsf(gap - (float)c), l.x);
+              l.y = fmaf(-slope, fabsf(gap - (float)(c + 1)), l.y);
             }
-            x = CAP || BIAS ? add2(x, l[k]) : fma2(x, splat2(a.scale_log2), l[k]);
-            p[c] = __float_as_uint(ex2(x.x));
-            p[c + 1] = __float_as_uint(ex2(x.y));
+            x = CAP || BIAS ? add2(x, l) : fma2(x, splat2(a.scale_log2), l);
+            x = k >= PB_POLY_K ? ex2_poly2_fine(x) : make_float2(ex2(x.x), ex2(x.y));
+            p[c] = __float_as_uint(x.x);
+            p[c + 1] = __float_as_uint(x.y);
           }
+          if constexpr (CAP) tmem_st8(t_s + i, f);               // over S, for the other half of the step
         }
-        const bool masked = KEYS ? s.index + c0 < warp_edge : s.index + c0 + 64 > warp_edge;
-        if (KEYS && masked) {
+        if constexpr (CAP) tmem_st_wait();
+        // the columns that the row sees (operands behind the end of a sequence are zero, so that P = 0 is enough)
+        if (KEYS ? index < warp_edge || end - index < PB_W : index + PB_W > warp_edge) {
+          const int lo = KEYS ? edge - index : 0, hi = KEYS ? end - index : edge - index;
 #pragma unroll
-          for (int i = 0; i < 64; ++i)
-            if (s.index + c0 + i < edge) p[i] = 0u;
+          for (int i = 0; i < 96; ++i)
+            if (i < lo || i >= hi) p[i] = 0u;
         }
-        if (!mbar_wait_warp(dp_full, G & 1, ctx, 71)) { ok = false; break; }
+        if (!mbar_wait_warp(&dp_full[wg], ph, ctx, 72)) { ok = false; break; }
         tc_fence_after();
-        uint32_t d[64];
-        {
-          uint32_t(&d0)[32] = *reinterpret_cast<uint32_t(*)[32]>(d);
-          uint32_t(&d1)[32] = *reinterpret_cast<uint32_t(*)[32]>(d + 32);
-          tmem_ld32(t_lane + PB_COL_DP + c0, d0);
-          tmem_ld32(t_lane + PB_COL_DP + c0 + 32, d1);
+#pragma unroll
+        for (int q = 0; q < 3; ++q) {                            // 32 columns: dP in, dS and P out in its place
+          uint32_t d[32], f[CAP ? 32 : 1];
+          tmem_ld32(t_d + 32 * q, d);
+          if constexpr (CAP) tmem_ld32(t_s + 32 * q, f);
           tmem_ld_wait();
-          tmem_ld_fence(d0);
-          tmem_ld_fence(d1);
-        }
-        tc_fence_before();
-        mbar_arrive(dp_free);
+          tmem_ld_fence(d);
+          if constexpr (CAP) tmem_ld_fence(f);
+          uint32_t w[32];
+          float u[4];
 #pragma unroll
-        for (int i = 0; i < 64; i += 4) {
-          float2 m[2];
-          if (KEYS) {
-            const float4 v = *reinterpret_cast<const float4*>(stat + 128 + i);
-            m[0] = make_float2(-v.x, -v.y);
-            m[1] = make_float2(-v.z, -v.w);
-          } else {
-            m[0] = m[1] = splat2(-delta);
+          for (int i = 0; i < 32; i += 2) {
+            const int c = 32 * q + i;
+            if (KEYS && i % 4 == 0) *reinterpret_cast<float4*>(u) = *reinterpret_cast<const float4*>(stat + 128 + c);
+            const float2 m = KEYS ? make_float2(-u[i % 4], -u[i % 4 + 1]) : splat2(ndelta);
+            const float2 pp = make_float2(__uint_as_float(p[c]), __uint_as_float(p[c + 1]));
+            float2 v = mul2(add2(make_float2(__uint_as_float(d[i]), __uint_as_float(d[i + 1])), m), pp);
+            if constexpr (CAP) v = mul2(v, make_float2(__uint_as_float(f[i]), __uint_as_float(f[i + 1])));
+            w[i >> 1] = pack16(v.x, v.y, F16);
+            if (KEYS) w[16 + (i >> 1)] = pack16(pp.x, pp.y, F16);
           }
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const int c = i + 2 * k;
-            float2 g = add2(make_float2(__uint_as_float(d[c]), __uint_as_float(d[c + 1])), m[k]);
-            g = mul2(g, make_float2(__uint_as_float(p[c]), __uint_as_float(p[c + 1])));
-            d[c] = __float_as_uint(g.x);
-            d[c + 1] = __float_as_uint(g.y);
-          }
-        }
-        if constexpr (CAP) {                                     // S is still in tensor memory: the factor from it again, 4 r (1 - r), r = 1 / (1 + e^2y)
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            uint32_t y[32];
-            tmem_ld32(t_s + 32 * half, y);
-            tmem_ld_wait();
-            tmem_ld_fence(y);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const float r = rcp_approx(1.f + ex2(__uint_as_float(y[i]) * a.cap_in));
-              d[32 * half + i] = __float_as_uint(__uint_as_float(d[32 * half + i]) * (4.f * r * (1.f - r)));
-            }
-          }
-        }
-        if (masked) {                                            // 0 * something that is no number
-#pragma unroll
-          for (int i = 0; i < 64; ++i)
-            if (KEYS ? s.index + c0 + i < edge : s.index + c0 + i >= edge) d[i] = 0u;
-        }
-        uint32_t w[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) w[i] = pack16(__uint_as_float(d[2 * i]), __uint_as_float(d[2 * i + 1]), F16);
-        tmem_st32(t_s + 32, w);
-        if (KEYS) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) w[i] = pack16(__uint_as_float(p[2 * i]), __uint_as_float(p[2 * i + 1]), F16);
-          tmem_st32(t_s, w);
-          if (++st == PB_RING) {
-            st = 0;
-            st_ph ^= 1;
-          }
+          if (KEYS) tmem_st32(t_d + 32 * q, w);
+          else tmem_st16(t_d + 32 * q, w);
         }
         tmem_st_wait();
         tc_fence_before();
-        mbar_arrive(&ds_full[buf]);
-      }
-      if (!ok) break;
-      if (I.n > 0) {
-        if (!mbar_wait_warp(acc_full, acc_ph, ctx, 72)) { ok = false; break; }
-        acc_ph ^= 1;
-        tc_fence_after();
-      }
-      // ROWS = queries: 32 columns of dQ per thread; ROWS = keys: dK by one half of the threads, dV by the other
-      constexpr int COLS = KEYS ? 64 : 32;
-#pragma unroll
-      for (int half = 0; half < COLS / 32; ++half) {
-        uint32_t r[32];
-        const uint32_t col = KEYS ? (wg ? PB_COL_A2 : PB_COL_A1) + 32 * half : PB_COL_A1 + 32 * wg;
-        if (I.n > 0) {
-          tmem_ld32(t_lane + col, r);
-          tmem_ld_wait();
-          tmem_ld_fence(r);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) r[i] = 0u;
-        }
-        if (row < I.rows()) {
-          const float f = KEYS && wg ? 1.f : a.scale;
-          uint8_t* dst;
-          if (KEYS && wg) dst = static_cast<uint8_t*>(a.g2) + 2 * ((int64_t)(I.row0() + row) * a.g2_st + (int64_t)I.head * a.g2_sh + 32 * half);
-          else dst = static_cast<uint8_t*>(a.g1) + 2 * ((int64_t)(I.row0() + row) * a.g1_st + (int64_t)I.head * a.g1_sh + (KEYS ? 32 * half : 32 * wg));
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t w[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) w[k] = pack16(__uint_as_float(r[8 * i + 2 * k]) * f, __uint_as_float(r[8 * i + 2 * k + 1]) * f, F16);
-            *reinterpret_cast<uint4*>(dst + 16 * i) = make_uint4(w[0], w[1], w[2], w[3]);
+        if (CAP) mbar_arrive(&s_free[wg]);
+        mbar_arrive(&ds_full[wg]);
+        ph ^= 1;
+        if (KEYS) {
+          st += 2;
+          if (st >= PB_RING) {
+            st -= PB_RING;
+            st_ph ^= 1;
           }
         }
       }
-      tc_fence_before();                                         // the accumulators have been read when the next step is handed over
+      if (!ok) break;
+      G0 += n;
+      // the group of the last step writes the item's gradients, those of an item without steps (zeros) group 0
+      if (n > 0) ++acc_n;
+      if (wg != (n > 0 ? (G0 - 1) & 1 : 0u)) continue;
+      if (n > 0) {
+        if (!mbar_wait_warp(&acc_full[(acc_n - 1) & 1], ((acc_n - 1) >> 1) & 1, ctx, 73)) { ok = false; break; }
+        tc_fence_after();
+      }
+      load_item(I, it);
+      // 64 columns of dQ, or of dK and then dV: all of them into registers, then the accumulators are the next item's
+      constexpr int PIECES = KEYS ? 4 : 2;
+      uint32_t r[PIECES][32];
+      if (n > 0) {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) tmem_ld32(t_lane + PB_COL_A1 + 32 * i, r[i]);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) tmem_ld_fence(r[i]);
+        tc_fence_before();
+        mbar_arrive(acc_free);
+      } else {
+#pragma unroll
+        for (int i = 0; i < PIECES * 32; ++i) r[i / 32][i % 32] = 0u;
+      }
+      if (row < I.rows()) {
+#pragma unroll
+        for (int half = 0; half < PIECES; ++half) {
+          const float f = half >= 2 ? 1.f : a.scale;
+          uint8_t* dst;
+          if (half >= 2) dst = static_cast<uint8_t*>(a.g2) + 2 * ((int64_t)(I.row0() + row) * a.g2_st + (int64_t)I.head * a.g2_sh + 32 * (half - 2));
+          else dst = static_cast<uint8_t*>(a.g1) + 2 * ((int64_t)(I.row0() + row) * a.g1_st + (int64_t)I.head * a.g1_sh + 32 * half);
+          uint32_t w[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) w[i] = pack16(__uint_as_float(r[half][2 * i]) * f, __uint_as_float(r[half][2 * i + 1]) * f, F16);
+          if (a.wide) {
+            stg8w(dst, w);
+            stg8w(dst + 32, w + 8);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) reinterpret_cast<uint4*>(dst)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+          }
+        }
+      }
     }
     }
   }
@@ -560,15 +600,19 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
   }
 }
 
-using BwdFn = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, PackBwdArgs);
+using BwdFn = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, PackBwdArgs);
 template <int F16, bool KEYS>
 static BwdFn bwd_kernel(bool cap, bool bias) {
   if (cap) return bias ? attn_pack_bwd_kernel<F16, KEYS, true, true> : attn_pack_bwd_kernel<F16, KEYS, true, false>;
   return bias ? attn_pack_bwd_kernel<F16, KEYS, false, true> : attn_pack_bwd_kernel<F16, KEYS, false, false>;
 }
 
+static int wide_rows(const kf_heads& t) {
+  return ((reinterpret_cast<uintptr_t>(t.ptr) | (uintptr_t)(t.row_stride * 2) | (uintptr_t)(t.head_stride * 2)) & 31) == 0;
+}
+
 // The register split draws on what the block was launched with: a build that allocates less is refused here, it would wait forever.
-static int bwd_ready(BwdFn kern, int which) {
+static int bwd_ready(BwdFn kern, int which, size_t smem) {
   static PerDevice<bool> ready[16];
   int dev = 0;
   cudaGetDevice(&dev);
@@ -577,7 +621,7 @@ static int bwd_ready(BwdFn kern, int which) {
   cudaError_t e = cudaFuncGetAttributes(&attr, kern);
   if (e != cudaSuccess) return cuda_status(e, "cudaFuncGetAttributes(attn_pack_bwd_kernel)");
   KF_REQUIRE(attr.numRegs >= PB_REGS_LAUNCH, "kf_attn_pack_bwd: the kernel was built with %d registers per thread, its split needs %d", attr.numRegs, PB_REGS_LAUNCH);
-  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PB_SMEM);
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(attn_pack_bwd_kernel)");
   ready[which].put(dev, true);
   return KF_OK;
@@ -592,7 +636,7 @@ extern "C" int64_t kf_attn_pack_ws_bytes(int Hq, int n_q_tiles) {
     set_error("kf_attn_pack_ws_bytes: bad argument Hq=%d n_q_tiles=%d", Hq, n_q_tiles);
     return KF_ERR_BAD_ARGUMENT;
   }
-  return (int64_t)Hq * n_q_tiles * 256 * 4;
+  return 2 * ((int64_t)Hq * n_q_tiles + 1) * PB_T * 4;         // the last passing tile may reach behind the last row
 }
 
 extern "C" int kf_attn_pack_bwd(const kf_attn_pack_params* p, void* stream) {
@@ -601,33 +645,28 @@ extern "C" int kf_attn_pack_bwd(const kf_attn_pack_params* p, void* stream) {
   if (p->n_q_tiles == 0 && p->n_k_tiles == 0) return KF_OK;
   constexpr float LOG2E = 1.4426950408889634f;
   kf_heads q{}, k{}, v{}, o{}, go{}, gq{}, gk{}, gv{};
-  if (p->n_q_tiles > 0) {
-    KF_REQUIRE(p->Tq > 0 && p->q_tiles && p->lse, "kf_attn_pack_bwd: null pointer");
+  const bool any_q = p->n_q_tiles > 0, any_k = p->n_k_tiles > 0;
+  KF_REQUIRE((!any_q || (p->Tq > 0 && p->q_tiles && p->lse)) && (!any_k || (p->Tk > 0 && p->k_tiles)), "kf_attn_pack_bwd: null pointer");
+  if (p->Tq > 0) {
     if ((rc = check_heads("q", p->q, p->Tq, p->Hq, &q)) != KF_OK) return rc;
     if ((rc = check_heads("o", p->o, p->Tq, p->Hq, &o)) != KF_OK) return rc;
     if ((rc = check_heads("dout", p->dout, p->Tq, p->Hq, &go)) != KF_OK) return rc;
     if ((rc = check_heads("dq", p->dq, p->Tq, p->Hq, &gq)) != KF_OK) return rc;
-    KF_REQUIRE(p->ws && (reinterpret_cast<uintptr_t>(p->ws) & 15) == 0 && p->ws_bytes >= kf_attn_pack_ws_bytes(p->Hq, p->n_q_tiles),
-               "kf_attn_pack_bwd: workspace of %lld bytes, needs %lld, 16-byte aligned", (long long)p->ws_bytes, (long long)kf_attn_pack_ws_bytes(p->Hq, p->n_q_tiles));
   }
-  if (p->n_k_tiles > 0) {
-    KF_REQUIRE(p->Tk > 0 && p->k_tiles, "kf_attn_pack_bwd: null pointer");
+  if (p->Tk > 0) {
     if ((rc = check_heads("k", p->k, p->Tk, p->Hk, &k)) != KF_OK) return rc;
     if ((rc = check_heads("v", p->v, p->Tk, p->Hk, &v)) != KF_OK) return rc;
     if ((rc = check_heads("dk", p->dk, p->Tk, p->Hk, &gk)) != KF_OK) return rc;
     if ((rc = check_heads("dv", p->dv, p->Tk, p->Hk, &gv)) != KF_OK) return rc;
   }
-  // without queries (or keys) at all the maps over them are never used: they then describe the other side
-  const bool any_q = p->n_q_tiles > 0, any_k = p->n_k_tiles > 0;
-  CUtensorMap tq, tgo, tk, tv;
-  auto maps = [&](const kf_heads& x, const kf_heads& y, int64_t rows, int heads, CUtensorMap* mx, CUtensorMap* my) {
-    const int r = make_tmap_heads(mx, x.ptr, rows, heads, x.row_stride, x.head_stride, PB_T);
-    return r != KF_OK ? r : make_tmap_heads(my, y.ptr, rows, heads, y.row_stride, y.head_stride, PB_T);
+  KF_REQUIRE(p->ws && (reinterpret_cast<uintptr_t>(p->ws) & 15) == 0 && p->ws_bytes >= kf_attn_pack_ws_bytes(p->Hq, p->n_q_tiles),
+             "kf_attn_pack_bwd: workspace of %lld bytes, needs %lld, 16-byte aligned", (long long)p->ws_bytes, (long long)kf_attn_pack_ws_bytes(p->Hq, p->n_q_tiles));
+  CUtensorMap r1, r2, r3, c1, c2;
+  // (a side stays in boxes of 128 rows in one launch and passes in boxes of 96 in the other)
+  auto maps = [&](const kf_heads& x, const kf_heads& y, int64_t rows, int heads, int box, CUtensorMap* mx, CUtensorMap* my) {
+    const int r = make_tmap_heads(mx, x.ptr, rows, heads, x.row_stride, x.head_stride, box);
+    return r != KF_OK ? r : make_tmap_heads(my, y.ptr, rows, heads, y.row_stride, y.head_stride, box);
   };
-  if (any_q && (rc = maps(q, go, p->Tq, p->Hq, &tq, &tgo)) != KF_OK) return rc;
-  if (any_k && (rc = maps(k, v, p->Tk, p->Hk, &tk, &tv)) != KF_OK) return rc;
-  if (!any_q) { tq = tk; tgo = tv; }
-  if (!any_k) { tk = tq; tv = tgo; }
   int sms = 0;
   if ((rc = device_sm_count(&sms)) != KF_OK) return rc;
   const bool f = p->dtype == KF_F16, c = p->cap > 0.f, b = p->slopes != nullptr;
@@ -640,8 +679,9 @@ extern "C" int kf_attn_pack_bwd(const kf_attn_pack_params* p, void* stream) {
     a.cap_out = p->cap * LOG2E;
   }
   a.slopes = p->slopes;
-  a.stats = static_cast<float*>(p->ws);
-  a.n_q_tiles = p->n_q_tiles;
+  a.stat_ld = (int64_t)p->n_q_tiles * PB_T;
+  a.lse2 = static_cast<float*>(p->ws);
+  a.delta = a.lse2 + a.stat_ld * p->Hq + PB_T;
   a.err = dev_error_ptr();
   KF_REQUIRE(a.err != nullptr, "kf_attn_pack_bwd: device error word unavailable");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -649,13 +689,20 @@ extern "C" int kf_attn_pack_bwd(const kf_attn_pack_params* p, void* stream) {
     a.tiles = reinterpret_cast<const int4*>(p->q_tiles);
     a.heads = p->Hq;
     a.n_items = p->n_q_tiles * p->Hq;
-    a.O = o.ptr; a.o_st = o.row_stride; a.o_sh = o.head_stride;
-    a.dO = go.ptr; a.do_st = go.row_stride; a.do_sh = go.head_stride;
     a.lse = p->lse; a.lse_ld = p->Tq;
     a.g1 = gq.ptr; a.g1_st = gq.row_stride; a.g1_sh = gq.head_stride;
+    a.wide = wide_rows(gq);
+    if ((rc = maps(q, go, p->Tq, p->Hq, PB_T, &r1, &r2)) != KF_OK) return rc;
+    if ((rc = make_tmap_heads(&r3, o.ptr, p->Tq, p->Hq, o.row_stride, o.head_stride, PB_T)) != KF_OK) return rc;
+    if (p->Tk > 0) {
+      if ((rc = maps(k, v, p->Tk, p->Hk, PB_W, &c1, &c2)) != KF_OK) return rc;
+    } else {                                                  // nothing passes: never used
+      c1 = r1;
+      c2 = r2;
+    }
     const BwdFn kern = f ? bwd_kernel<1, false>(c, b) : bwd_kernel<0, false>(c, b);
-    if ((rc = bwd_ready(kern, f * 8 + c * 2 + b)) != KF_OK) return rc;
-    const cudaError_t e = launch_maybe_pdl(p->Tq, kern, dim3(a.n_items < sms ? a.n_items : sms), dim3(PB_THREADS), PB_SMEM, st, tq, tgo, tk, tv, a);
+    if ((rc = bwd_ready(kern, f * 8 + c * 2 + b, BwdMem<false>::BYTES)) != KF_OK) return rc;
+    const cudaError_t e = launch_maybe_pdl(p->Tq, kern, dim3(a.n_items < sms ? a.n_items : sms), dim3(PB_THREADS), BwdMem<false>::BYTES, st, r1, r2, r3, c1, c2, a);
     if (e != cudaSuccess) return cuda_status(e, "kf_attn_pack_bwd launch (queries)");
   }
   if (any_k) {
@@ -664,9 +711,17 @@ extern "C" int kf_attn_pack_bwd(const kf_attn_pack_params* p, void* stream) {
     a.n_items = p->n_k_tiles * p->Hk;
     a.g1 = gk.ptr; a.g1_st = gk.row_stride; a.g1_sh = gk.head_stride;
     a.g2 = gv.ptr; a.g2_st = gv.row_stride; a.g2_sh = gv.head_stride;
+    a.wide = wide_rows(gk) && wide_rows(gv);
+    if ((rc = maps(k, v, p->Tk, p->Hk, PB_T, &r1, &r2)) != KF_OK) return rc;
+    if (p->Tq > 0) {
+      if ((rc = maps(q, go, p->Tq, p->Hq, PB_W, &c1, &c2)) != KF_OK) return rc;
+    } else {
+      c1 = r1;
+      c2 = r2;
+    }
     const BwdFn kern = f ? bwd_kernel<1, true>(c, b) : bwd_kernel<0, true>(c, b);
-    if ((rc = bwd_ready(kern, f * 8 + 4 + c * 2 + b)) != KF_OK) return rc;
-    const cudaError_t e = launch_maybe_pdl(p->Tk, kern, dim3(a.n_items < sms ? a.n_items : sms), dim3(PB_THREADS), PB_SMEM, st, tk, tv, tq, tgo, a);
+    if ((rc = bwd_ready(kern, f * 8 + 4 + c * 2 + b, BwdMem<true>::BYTES)) != KF_OK) return rc;
+    const cudaError_t e = launch_maybe_pdl(p->Tk, kern, dim3(a.n_items < sms ? a.n_items : sms), dim3(PB_THREADS), BwdMem<true>::BYTES, st, r1, r2, r1, c1, c2, a);
     if (e != cudaSuccess) return cuda_status(e, "kf_attn_pack_bwd launch (keys)");
   }
   return KF_OK;
