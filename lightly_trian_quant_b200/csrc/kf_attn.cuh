@@ -59,6 +59,19 @@ __device__ __forceinline__ float2 ex2_poly2_fine(float2 t) {
   return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(r.x) << 23)), __int_as_float(__float_as_int(p.y) + (__float_as_int(r.y) << 23)));
 }
 
+// The quartic for t that is not above 0 (but for rounding): one clamp, and the power of two goes in by a multiplication, which keeps what is no number.
+__device__ __forceinline__ float2 ex2_poly2_neg(float2 t) {
+  asm("max.NaN.f32 %0, %0, 0fC2FC0000;\n\tmax.NaN.f32 %1, %1, 0fC2FC0000;" : "+f"(t.x), "+f"(t.y));
+  const float2 r = add2(t, splat2(12582912.f));
+  const float2 n = add2(r, splat2(-12582912.f));
+  const float2 f = fma2(n, splat2(-1.f), t);
+  float2 p = fma2(f, splat2(0x1.3997d4p-7f), splat2(0x1.ca1440p-5f));
+  p = fma2(p, f, splat2(0x1.ec06dap-3f));
+  p = fma2(p, f, splat2(0x1.62e0dcp-1f));
+  p = fma2(p, f, splat2(0x1.ffffe8p-1f));
+  return mul2(p, make_float2(__int_as_float((__float_as_int(r.x) << 23) + 0x3f800000), __int_as_float((__float_as_int(r.y) << 23) + 0x3f800000)));
+}
+
 __device__ __forceinline__ float rcp_approx(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

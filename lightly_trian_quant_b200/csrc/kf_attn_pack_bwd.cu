@@ -11,13 +11,13 @@
 // from run to run.
 //
 //   CTA      one per SM, persistent over (tile, head) items, the longest first; steps of 96 passing rows
-//   roles    two groups of four warps take the steps in turn, a thread a row: S and dP from tensor memory, P and dS as 16-bit pairs back over
-//            dP; warp 8: TMA (row operands in two buffers, passing operands in a ring); warps 9, 10, 11: the products S, dP and those of the
-//            gradients; warp 12 (ROWS = queries): log-sum-exp and delta of the rows of the next item, also for the second launch
-//   pipeline two S buffers, two dP buffers, the accumulators (2 x 96 + 2 x 96 + 2 x 64 columns).  A group reads its whole S row at once, so
+//   roles    two pairs of groups of four warps take the steps in turn, a thread half a row: S and dP from tensor memory, P and dS as 16-bit
+//            pairs back over dP; warp 16: TMA (row operands in two buffers, passing operands in a ring); warps 17, 18, 19: the products S, dP
+//            and those of the gradients
+//   pipeline two S buffers, two dP buffers, the accumulators (2 x 96 + 2 x 96 + 2 x 64 columns).  The groups read their S at once, so
 //            S(G + 2) is issued while it works on step G; dP(G + 2) goes behind the gradients' products of step G, which read P and dS from
-//            the same buffer, and is needed when the exponentials of step G + 2 are done.  The group of an item's last step writes the
-//            item's gradients, the other one goes on with the next item.
+//            the same buffer, and is needed when the exponentials of step G + 2 are done.  The groups of an item's last step write the
+//            item's gradients, the others go on with the next item.
 //   numerics P and dS are rounded to the 16-bit type of the operands (the products' A operand); everything else fp32; three of every four pairs of
 //            exponentials by the special-function unit, the fourth on the FMA pipe
 #include "kf_attn.cuh"
@@ -25,30 +25,30 @@
 namespace kf {
 
 constexpr int PB_T = 128, PB_W = 96, PB_D = 64;                // rows of a tile that stays, rows of a passing one
-constexpr int PB_THREADS = 512;
-constexpr int PB_REGS_WORK = 208, PB_REGS_LEAN = 48;
-constexpr int PB_REGS_LAUNCH = 128;
-static_assert(256 * PB_REGS_WORK + 256 * PB_REGS_LEAN <= PB_THREADS * PB_REGS_LAUNCH, "register split");
+constexpr int PB_THREADS = 640;
+constexpr int PB_REGS_WORK = 104, PB_REGS_LEAN = 64;
+constexpr int PB_REGS_LAUNCH = 96;
+static_assert(512 * PB_REGS_WORK + 128 * PB_REGS_LEAN <= PB_THREADS * PB_REGS_LAUNCH, "register split");
 constexpr int PB_RTILE = PB_T * PB_D * 2, PB_CTILE = PB_W * PB_D * 2;     // 16 KB, 12 KB
-// Shared memory: row operands in two buffers (with ROWS = queries also O, for delta), a ring of passing ones, the rows' log-sum-exp and delta
-// (1 KB per stage, or per item buffer), barriers.
+// Shared memory: row operands in two buffers (with ROWS = queries also O, for delta), a ring of passing ones, with ROWS = keys the log-sum-exp
+// and delta of the passing rows (1 KB per stage), barriers.
 template <bool KEYS>
 struct BwdMem {
   static constexpr int RING = KEYS ? 6 : 5, RTILES = KEYS ? 2 : 3;
-  static constexpr int OFF_C = 2 * RTILES * PB_RTILE, OFF_STAT = OFF_C + RING * 2 * PB_CTILE, OFF_BAR = OFF_STAT + (KEYS ? RING : 2) * 1024;
+  static constexpr int OFF_C = 2 * RTILES * PB_RTILE, OFF_STAT = OFF_C + RING * 2 * PB_CTILE, OFF_BAR = OFF_STAT + (KEYS ? RING * 1024 : 0);
   static constexpr size_t BYTES = (size_t)OFF_BAR + 512;
   static_assert(BYTES <= 227 * 1024, "shared memory");
 };
 constexpr int PB_COL_S = 0, PB_COL_D = 2 * PB_W, PB_COL_A1 = 4 * PB_W, PB_COL_A2 = PB_COL_A1 + PB_D, PB_TMEM_COLS = 512;
 static_assert(PB_COL_A2 + PB_D <= PB_TMEM_COLS, "TMEM budget");
-constexpr int PB_POLY_K = 3;                                   // element pairs PB_POLY_K .. 3 of every four take the polynomial exponential
+constexpr int PB_POLY = 0x88, PB_POLY_CAP = 0xaa;               // which of eight element pairs take the polynomial exponential
 
 struct PackBwdArgs {
   const int4* tiles;
   int n_items, heads, share;     // heads of an item: query heads (ROWS = queries) or key heads
   float scale, scale_log2, cap_in, cap_out;
   const float* slopes;
-  float *lse2, *delta;           // [Hq][n_q_tiles * 128], a sequence's rows from its first tile's slot on
+  float *lse2, *delta;           // -lse * log2(e) (-inf: no row, or one that sees nothing) and -delta: [Hq][n_q_tiles * 128], a sequence's rows from its first tile's slot on
   int64_t stat_ld;
   // ROWS = queries
   const float* lse;
@@ -119,8 +119,8 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + PB_OFF_BAR);
   uint64_t *r_full = bars, *r_empty = r_full + 2, *c1_full = r_empty + 2, *c2_full = c1_full + PB_RING, *c_empty = c2_full + PB_RING, *st_full = c_empty + PB_RING,
-           *st_empty = st_full + PB_RING, *s_full = st_empty + 2, *s_free = s_full + 2, *dp_full = s_free + 2, *ds_full = dp_full + 2, *d_free = ds_full + 2,
-           *acc_full = d_free + 2, *acc_free = acc_full + 2;
+           *s_full = st_full + PB_RING, *s_free = s_full + 2, *dp_full = s_free + 2, *ds_full = dp_full + 2, *d_free = ds_full + 2, *acc_full = d_free + 2,
+           *acc_free = acc_full + 2;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(acc_free + 1);
   volatile uint32_t* abort_flag = tmem_holder + 1;
 
@@ -131,13 +131,12 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&r_full[i], 1);
-      mbar_init(&r_empty[i], RTILES);                             // S, dP, and whoever reads O
+      mbar_init(&r_empty[i], KEYS ? 2 : 2 + 16);                  // S, dP; the warps that read O and dO
       mbar_init(&s_full[i], 1);
-      mbar_init(&s_free[i], 128);
+      mbar_init(&s_free[i], 256);
       mbar_init(&dp_full[i], 1);
-      mbar_init(&ds_full[i], 128);
+      mbar_init(&ds_full[i], 256);
       mbar_init(&d_free[i], 1);
-      mbar_init(&st_empty[i], 256);
       mbar_init(&acc_full[i], 1);                                // items in turn: a group may ask for its item before the other's is complete
     }
     for (int i = 0; i < PB_RING; ++i) {
@@ -146,11 +145,11 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
       mbar_init(&c_empty[i], 1);
       mbar_init(&st_full[i], 1);
     }
-    mbar_init(acc_free, 128);
+    mbar_init(acc_free, 256);
     *abort_flag = 0u;
     fence_mbar_init();
   }
-  if (warp == 9) {                                         // (the whole warp)
+  if (warp == 16) {
     tmem_alloc(tmem_holder, PB_TMEM_COLS);
     tmem_relinquish();
   }
@@ -168,11 +167,11 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
   using Item = BwdItem<KEYS>;
   auto load_item = [&](Item& i, int it) { i.load(a, item_of_cta(it)); };
 
-  if (warp >= 8) {
+  if (warp >= 16) {
   setmaxnreg_dec<PB_REGS_LEAN>();
   if (bad_align) {
     // nothing was issued; fall through to the teardown
-  } else if (warp == 8) {
+  } else if (warp == 16) {
     // ------------------------------------------------------------------ TMA producer
     if (elect_one()) {
       prefetch_tmap(&tmR1);
@@ -221,8 +220,8 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
         }
       }
     }
-  } else if (warp <= 11) {
-    // ------------------------------------------------------------------ MMA issuers: warp 9 S, warp 10 dP, warp 11 the gradients
+  } else {
+    // ------------------------------------------------------------------ MMA issuers: warp 17 S, warp 18 dP, warp 19 the gradients
     // One warp for all three spent 1700 clk per step on waiting, addresses and issue, twice the time of the products.
     // Everything the products take is worked out by the whole warp, in front of the branch that one lane takes: behind it each address would
     // be one lane's, moved to a uniform register in front of every instruction.
@@ -269,9 +268,9 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
     fetch();
     open();
     const uint32_t fmt = F16 ? 0u : 1u;
-    if (warp < 11) {
+    if (warp < 19) {
       // row operand `which` times the passing one, 128 x 96 x 64, into the buffer that the step before the last has left
-      const uint32_t which = warp - 9;
+      const uint32_t which = warp - 17;
       const uint32_t idesc = idesc_f16(fmt, PB_W), col = which ? PB_COL_D : PB_COL_S;
       uint64_t *const c_full = which ? c2_full : c1_full, *const room = which ? d_free : s_free, *const full = which ? dp_full : s_full;
       while (n > 0) {
@@ -284,7 +283,7 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
           if (KEYS && which == 0) {                                           // the rows' values there: P = 0
             float* sm = reinterpret_cast<float*>(smem + PB_OFF_STAT + st * 1024);
             for (int i = valid + lane; i < PB_W; i += 32) {
-              sm[i] = INFINITY;
+              sm[i] = -INFINITY;
               sm[128 + i] = 0.f;
             }
           }
@@ -319,9 +318,9 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
         const uint32_t more = j != 0;
         if (leader) {
 #pragma unroll
-          for (int kk = 0; kk < PB_W / 16; ++kk) {                            // 32 columns of dP hold 16 words of dS and 16 of P
-            const uint32_t d = t_d + (kk >> 1) * 32 + (kk & 1) * 8;
-            if (KEYS) mma_f16_ta(tmem_base + PB_COL_A2, d + 16, c2 + (uint64_t)(kk * (2048 >> 4)), idesc, kk ? 1u : more);
+          for (int kk = 0; kk < PB_W / 16; ++kk) {                            // 16 columns of dP hold 8 words of dS and 8 of P
+            const uint32_t d = t_d + kk * 16;
+            if (KEYS) mma_f16_ta(tmem_base + PB_COL_A2, d + 8, c2 + (uint64_t)(kk * (2048 >> 4)), idesc, kk ? 1u : more);
             mma_f16_ta(tmem_base + PB_COL_A1, d, c1 + (uint64_t)(kk * (2048 >> 4)), idesc, kk ? 1u : more);
           }
           tc_commit(d_done);
@@ -332,74 +331,51 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
         advance();
       }
     }
-  } else if (!KEYS && warp == 12) {
-    // ------------------------------------------------------------------ log-sum-exp and delta of the rows: four per lane, dO and O from shared memory
-    uint32_t ri = 0;
-    for (int it = 0; it < n_my; ++it) {
+  }
+  } else {
+    setmaxnreg_inc<PB_REGS_WORK>();
+    if (!bad_align) {
+    // ------------------------------------------------------------------ a thread half a row of every other step
+    const uint32_t par = (warp >> 2) & 1, half = warp >> 3;
+    const int row = (warp & 3) * 32 + lane;
+    constexpr int COLS = PB_W / 2;
+    const int c0 = (int)half * COLS;
+    const uint32_t t_lane = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t t_s = t_lane + PB_COL_S + par * PB_W + c0, t_d = t_lane + PB_COL_D + par * PB_W + c0;     // step G uses buffers G & 1
+    bool ok = true;
+    uint32_t G0 = 0, ph = 0, ri = 0;                             // steps before this item; parity of the next step of this kind; items with steps
+    uint32_t st = par, st_ph = 0;                                // ring stage of the next step and its parity
+    for (int it = 0; it < n_my && ok; ++it) {
       Item I;
       load_item(I, it);
-      const int b = it & 1;
-      const float* l = a.lse + (int64_t)I.head * a.lse_ld + I.row0();
-      float lse2[4], delta[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) lse2[k] = 32 * k + lane < I.rows() ? __ldg(l + 32 * k + lane) : -INFINITY;
-      if (I.n > 0) {
-        if (!mbar_wait_warp(&r_full[ri & 1], (ri >> 1) & 1, ctx, 65)) break;
-        const uint8_t* d = smem + ((ri & 1) * RTILES + 1) * PB_RTILE;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int r = 32 * k + lane;
+      const int n = I.n;
+      // ROWS = queries: the row's log-sum-exp and delta (negated: they are added), also for the second launch
+      float nlse2 = 0.f, ndelta = 0.f;
+      if constexpr (!KEYS) {
+        nlse2 = row < I.rows() ? __ldg(a.lse + (int64_t)I.head * a.lse_ld + I.row0() + row) : -INFINITY;
+        if (n > 0) {
+          if (!mbar_wait_warp(&r_full[ri & 1], (ri >> 1) & 1, ctx, 65)) break;
+          const uint8_t* d = smem + ((ri & 1) * RTILES + 1) * PB_RTILE + row * 128;
           float2 s = make_float2(0.f, 0.f);
-#pragma unroll
+#pragma unroll 4
           for (int c = 0; c < 8; ++c) {
-            const int at = r * 128 + ((c ^ (r & 7)) << 4);                    // the swizzle of the tile
-            const uint4 u = *reinterpret_cast<const uint4*>(d + at), v = *reinterpret_cast<const uint4*>(d + PB_RTILE + at);
+            const int o = (c ^ (row & 7)) << 4;                  // the swizzle of the tile
+            const uint4 u = *reinterpret_cast<const uint4*>(d + o), v = *reinterpret_cast<const uint4*>(d + PB_RTILE + o);
             s = fma2(unpack16<F16>(u.x), unpack16<F16>(v.x), s);
             s = fma2(unpack16<F16>(u.y), unpack16<F16>(v.y), s);
             s = fma2(unpack16<F16>(u.z), unpack16<F16>(v.z), s);
             s = fma2(unpack16<F16>(u.w), unpack16<F16>(v.w), s);
           }
-          if (r < I.rows()) delta[k] = s.x + s.y;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&r_empty[ri & 1]);
+          if (row < I.rows()) ndelta = -(s.x + s.y);
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&r_empty[ri & 1]);
-        ++ri;
-      }
-      if (!mbar_wait_warp(&st_empty[b], ((it >> 1) & 1) ^ 1, ctx, 69)) break;
-      float* sm = reinterpret_cast<float*>(smem + PB_OFF_STAT + b * 1024);
-      const int64_t at = I.head * a.stat_ld + (int64_t)I.slot() * PB_T;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int r = 32 * k + lane;
-        lse2[k] = lse2[k] == -INFINITY ? INFINITY : lse2[k] * 1.4426950408889634f;
-        sm[r] = a.lse2[at + r] = lse2[k];
-        sm[128 + r] = a.delta[at + r] = delta[k];
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&st_full[b]);
-    }
-  }
-  } else {
-    setmaxnreg_inc<PB_REGS_WORK>();
-    if (!bad_align) {
-    // ------------------------------------------------------------------ a thread a row, the groups take the steps in turn
-    const uint32_t wg = warp >> 2;
-    const int row = (warp & 3) * 32 + lane;
-    const uint32_t t_lane = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t t_s = t_lane + PB_COL_S + wg * PB_W, t_d = t_lane + PB_COL_D + wg * PB_W;     // step G uses buffer G & 1, which is the group
-    bool ok = true;
-    uint32_t G0 = 0, ph = 0, acc_n = 0;                          // steps before this item; parity of this group's next step; items with steps
-    uint32_t st = wg, st_ph = 0;                                 // ring stage of this group's next step and its parity
-    for (int it = 0; it < n_my && ok; ++it) {
-      Item I;
-      load_item(I, it);
-      float nlse2 = 0.f, ndelta = 0.f;
-      if (!KEYS) {
-        if (!mbar_wait_warp(&st_full[it & 1], (it >> 1) & 1, ctx, 69)) break;
-        const float* sm = reinterpret_cast<const float*>(smem + PB_OFF_STAT + (it & 1) * 1024);
-        nlse2 = -sm[row];
-        ndelta = -sm[128 + row];
-        mbar_arrive(&st_empty[it & 1]);
+        nlse2 = nlse2 == -INFINITY ? -INFINITY : nlse2 * -1.4426950408889634f;
+        if (warp < 4) {
+          const int64_t o = I.head * a.stat_ld + (int64_t)I.slot() * PB_T + row;
+          a.lse2[o] = nlse2;
+          a.delta[o] = ndelta;
+        }
       }
       // ROWS = queries: the row sees columns below `edge`; ROWS = keys: from `edge` on
       int edge, warp_edge;
@@ -415,53 +391,44 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
       }
       float slope = 0.f;
       if (BIAS && !KEYS) slope = __ldg(a.slopes + I.head) * 1.4426950408889634f;
-      const int n = I.n;
-      int index, end, head = 0;                                  // of the passing rows: first one in its sequence, end of the sequence, head
+      int index = c0, end = 0x7fffffff, head = 0, per_rows = 0;  // of this thread's first column: its place in the sequence; the sequence's end; head
       if constexpr (KEYS) {
-        index = I.first * PB_W;
+        index += I.first * PB_W;
         end = I.t.q_len;
         head = I.head * a.share;
-      } else {
-        index = 0;
-        end = 0x7fffffff;
+        per_rows = I.per * PB_W;
       }
+      const int start = index;
       auto move = [&](int steps) {                               // from one query head to the next one that shares the keys
         index += steps * PB_W;
         if constexpr (KEYS) {
-          while (index >= end && head + 1 < (I.head + 1) * a.share) {
-            index -= I.per * PB_W;
+          while (index >= start + per_rows) {
+            index -= per_rows;
             ++head;
           }
         }
       };
-      const int j0 = (int)((G0 + wg) & 1);
+      const int j0 = (int)((G0 + par) & 1);
       if (j0 < n) move(j0);
-      for (int j = j0; j < n; j += 2, move(2)) {
+      for (int j = j0; j < n; j += 2) {
         if (BIAS && KEYS) slope = __ldg(a.slopes + head) * 1.4426950408889634f;
-        uint32_t p[96];
-        if (!mbar_wait_warp(&s_full[wg], ph, ctx, 70)) { ok = false; break; }
+        uint32_t p[3][16];
+        if (!mbar_wait_warp(&s_full[par], ph, ctx, 70)) { ok = false; break; }
         tc_fence_after();
-        {
-          uint32_t(&p0)[32] = *reinterpret_cast<uint32_t(*)[32]>(p);
-          uint32_t(&p1)[32] = *reinterpret_cast<uint32_t(*)[32]>(p + 32);
-          uint32_t(&p2)[32] = *reinterpret_cast<uint32_t(*)[32]>(p + 64);
-          tmem_ld32(t_s, p0);
-          tmem_ld32(t_s + 32, p1);
-          tmem_ld32(t_s + 64, p2);
-          tmem_ld_wait();
-          tmem_ld_fence(p0);
-          tmem_ld_fence(p1);
-          tmem_ld_fence(p2);
-        }
+#pragma unroll
+        for (int q = 0; q < 3; ++q) tmem_ld16(t_s + 16 * q, p[q]);
+        tmem_ld_wait();
+#pragma unroll
+        for (int q = 0; q < 3; ++q) tmem_ld_fence(p[q]);
         if (!CAP) {
           tc_fence_before();
-          mbar_arrive(&s_free[wg]);
+          mbar_arrive(&s_free[par]);
         }
-        const float* stat = reinterpret_cast<const float*>(smem + PB_OFF_STAT + st * 1024);
+        const float* stat = reinterpret_cast<const float*>(smem + PB_OFF_STAT + st * 1024) + c0;
         if (KEYS && !mbar_wait_warp(&st_full[st], st_ph, ctx, 71)) { ok = false; break; }
         const float gap = at - (float)index;
 #pragma unroll
-        for (int i = 0; i < 96; i += 8) {
+        for (int i = 0; i < COLS; i += 8) {
           uint32_t f[8];                                         // with a cap: 1 - tanh^2 = 4 r (1 - r), r = 1 / (1 + e^2y)
           float v[8];
           if (KEYS) {
@@ -471,8 +438,8 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const int c = i + 2 * k;
-            float2 l = KEYS ? make_float2(-v[2 * k], -v[2 * k + 1]) : splat2(nlse2);
-            float2 x = make_float2(__uint_as_float(p[c]), __uint_as_float(p[c + 1]));
+            float2 l = KEYS ? make_float2(v[2 * k], v[2 * k + 1]) : splat2(nlse2);
+            float2 x = make_float2(__uint_as_float(p[c / 16][c % 16]), __uint_as_float(p[c / 16][c % 16 + 1]));
             if constexpr (CAP) {
               const float2 r = make_float2(rcp_approx(1.f + ex2(x.x * a.cap_in)), rcp_approx(1.f + ex2(x.y * a.cap_in)));
               const float2 r4 = mul2(r, splat2(4.f));
@@ -488,50 +455,49 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
               l.y = fmaf(-slope, fabsf(gap - (float)(c + 1)), l.y);
             }
             x = CAP || BIAS ? add2(x, l) : fma2(x, splat2(a.scale_log2), l);
-            x = k >= PB_POLY_K ? ex2_poly2_fine(x) : make_float2(ex2(x.x), ex2(x.y));
-            p[c] = __float_as_uint(x.x);
-            p[c + 1] = __float_as_uint(x.y);
+            x = ((CAP ? PB_POLY_CAP : PB_POLY) >> ((i / 2 + k) % 8)) & 1 ? ex2_poly2_neg(x) : make_float2(ex2(x.x), ex2(x.y));
+            p[c / 16][c % 16] = __float_as_uint(x.x);
+            p[c / 16][c % 16 + 1] = __float_as_uint(x.y);
           }
           if constexpr (CAP) tmem_st8(t_s + i, f);               // over S, for the other half of the step
         }
         if constexpr (CAP) tmem_st_wait();
         // the columns that the row sees (operands behind the end of a sequence are zero, so that P = 0 is enough)
-        if (KEYS ? index < warp_edge || end - index < PB_W : index + PB_W > warp_edge) {
+        if (KEYS ? index < warp_edge || end - index < COLS : index + COLS > warp_edge) {
           const int lo = KEYS ? edge - index : 0, hi = KEYS ? end - index : edge - index;
 #pragma unroll
-          for (int i = 0; i < 96; ++i)
-            if (i < lo || i >= hi) p[i] = 0u;
+          for (int i = 0; i < COLS; ++i)
+            if (i < lo || i >= hi) p[i / 16][i % 16] = 0u;
         }
-        if (!mbar_wait_warp(&dp_full[wg], ph, ctx, 72)) { ok = false; break; }
+        if (!mbar_wait_warp(&dp_full[par], ph, ctx, 72)) { ok = false; break; }
         tc_fence_after();
 #pragma unroll
-        for (int q = 0; q < 3; ++q) {                            // 32 columns: dP in, dS and P out in its place
-          uint32_t d[32], f[CAP ? 32 : 1];
-          tmem_ld32(t_d + 32 * q, d);
-          if constexpr (CAP) tmem_ld32(t_s + 32 * q, f);
+        for (int q = 0; q < 3; ++q) {                            // 16 columns: dP in, dS and P out in its place
+          uint32_t d[16], f[CAP ? 16 : 1];
+          tmem_ld16(t_d + 16 * q, d);
+          if constexpr (CAP) tmem_ld16(t_s + 16 * q, f);
           tmem_ld_wait();
           tmem_ld_fence(d);
           if constexpr (CAP) tmem_ld_fence(f);
-          uint32_t w[32];
+          uint32_t w[16];
           float u[4];
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const int c = 32 * q + i;
-            if (KEYS && i % 4 == 0) *reinterpret_cast<float4*>(u) = *reinterpret_cast<const float4*>(stat + 128 + c);
-            const float2 m = KEYS ? make_float2(-u[i % 4], -u[i % 4 + 1]) : splat2(ndelta);
-            const float2 pp = make_float2(__uint_as_float(p[c]), __uint_as_float(p[c + 1]));
+          for (int i = 0; i < 16; i += 2) {
+            if (KEYS && i % 4 == 0) *reinterpret_cast<float4*>(u) = *reinterpret_cast<const float4*>(stat + 128 + 16 * q + i);
+            const float2 m = KEYS ? make_float2(u[i % 4], u[i % 4 + 1]) : splat2(ndelta);
+            const float2 pp = make_float2(__uint_as_float(p[q][i]), __uint_as_float(p[q][i + 1]));
             float2 v = mul2(add2(make_float2(__uint_as_float(d[i]), __uint_as_float(d[i + 1])), m), pp);
             if constexpr (CAP) v = mul2(v, make_float2(__uint_as_float(f[i]), __uint_as_float(f[i + 1])));
             w[i >> 1] = pack16(v.x, v.y, F16);
-            if (KEYS) w[16 + (i >> 1)] = pack16(pp.x, pp.y, F16);
+            if (KEYS) w[8 + (i >> 1)] = pack16(pp.x, pp.y, F16);
           }
-          if (KEYS) tmem_st32(t_d + 32 * q, w);
-          else tmem_st16(t_d + 32 * q, w);
+          if (KEYS) tmem_st16(t_d + 16 * q, w);
+          else tmem_st8(t_d + 16 * q, *reinterpret_cast<const uint32_t(*)[8]>(w));
         }
         tmem_st_wait();
         tc_fence_before();
-        if (CAP) mbar_arrive(&s_free[wg]);
-        mbar_arrive(&ds_full[wg]);
+        if (CAP) mbar_arrive(&s_free[par]);
+        mbar_arrive(&ds_full[par]);
         ph ^= 1;
         if (KEYS) {
           st += 2;
@@ -540,48 +506,53 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
             st_ph ^= 1;
           }
         }
+        move(2);
       }
       if (!ok) break;
       G0 += n;
-      // the group of the last step writes the item's gradients, those of an item without steps (zeros) group 0
-      if (n > 0) ++acc_n;
-      if (wg != (n > 0 ? (G0 - 1) & 1 : 0u)) continue;
+      if (n > 0) ++ri;
+      // the groups of the last step write the item's gradients, those of an item without steps (zeros) groups 0
+      if (par != (n > 0 ? (G0 - 1) & 1 : 0u)) continue;
       if (n > 0) {
-        if (!mbar_wait_warp(&acc_full[(acc_n - 1) & 1], ((acc_n - 1) >> 1) & 1, ctx, 73)) { ok = false; break; }
+        if (!mbar_wait_warp(&acc_full[(ri - 1) & 1], ((ri - 1) >> 1) & 1, ctx, 73)) { ok = false; break; }
         tc_fence_after();
       }
       load_item(I, it);
-      // 64 columns of dQ, or of dK and then dV: all of them into registers, then the accumulators are the next item's
-      constexpr int PIECES = KEYS ? 4 : 2;
-      uint32_t r[PIECES][32];
+      // ROWS = queries: 32 columns of dQ; ROWS = keys: 64 of dK or of dV.  All of them packed in registers, then the accumulators are the next item's.
+      constexpr int PIECES = KEYS ? 2 : 1;
+      uint32_t w[PIECES][16];
+      const uint32_t t_a = t_lane + PB_COL_A1 + half * (32 * PIECES);
+      const float scale = KEYS && half ? 1.f : a.scale;
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) {
+        uint32_t r[32];
+        if (n > 0) {
+          tmem_ld32(t_a + 32 * i, r);
+          tmem_ld_wait();
+          tmem_ld_fence(r);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) r[k] = 0u;
+        }
+#pragma unroll
+        for (int k = 0; k < 16; ++k) w[i][k] = pack16(__uint_as_float(r[2 * k]) * scale, __uint_as_float(r[2 * k + 1]) * scale, F16);
+      }
       if (n > 0) {
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i) tmem_ld32(t_lane + PB_COL_A1 + 32 * i, r[i]);
-        tmem_ld_wait();
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i) tmem_ld_fence(r[i]);
         tc_fence_before();
         mbar_arrive(acc_free);
-      } else {
-#pragma unroll
-        for (int i = 0; i < PIECES * 32; ++i) r[i / 32][i % 32] = 0u;
       }
       if (row < I.rows()) {
+        const int64_t r = I.row0() + row;
+        uint8_t* dst = KEYS && half ? static_cast<uint8_t*>(a.g2) + 2 * (r * a.g2_st + (int64_t)I.head * a.g2_sh)
+                                    : static_cast<uint8_t*>(a.g1) + 2 * (r * a.g1_st + (int64_t)I.head * a.g1_sh + (KEYS ? 0 : 32 * (int)half));
 #pragma unroll
-        for (int half = 0; half < PIECES; ++half) {
-          const float f = half >= 2 ? 1.f : a.scale;
-          uint8_t* dst;
-          if (half >= 2) dst = static_cast<uint8_t*>(a.g2) + 2 * ((int64_t)(I.row0() + row) * a.g2_st + (int64_t)I.head * a.g2_sh + 32 * (half - 2));
-          else dst = static_cast<uint8_t*>(a.g1) + 2 * ((int64_t)(I.row0() + row) * a.g1_st + (int64_t)I.head * a.g1_sh + 32 * half);
-          uint32_t w[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) w[i] = pack16(__uint_as_float(r[half][2 * i]) * f, __uint_as_float(r[half][2 * i + 1]) * f, F16);
+        for (int i = 0; i < PIECES; ++i) {
           if (a.wide) {
-            stg8w(dst, w);
-            stg8w(dst + 32, w + 8);
+            stg8w(dst + 64 * i, w[i]);
+            stg8w(dst + 64 * i + 32, w[i] + 8);
           } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) reinterpret_cast<uint4*>(dst)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+            for (int k = 0; k < 4; ++k) reinterpret_cast<uint4*>(dst + 64 * i)[k] = make_uint4(w[i][4 * k], w[i][4 * k + 1], w[i][4 * k + 2], w[i][4 * k + 3]);
           }
         }
       }
@@ -594,7 +565,7 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
   if (*abort_flag && !bad_align) {
     for (int i = 0; i < 64; ++i) __nanosleep(2000);
   }
-  if (warp == 9) {
+  if (warp == 16) {
     tc_fence_after();
     tmem_dealloc(tmem_base, PB_TMEM_COLS);
   }
