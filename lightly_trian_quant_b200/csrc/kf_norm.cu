@@ -4,11 +4,13 @@
 //   g  = dy * w;  dx = rstd * (g - mean(g) - xh * mean(g * xh)) (+ dres);  dw = sum over rows of dy * xh;  db = sum over rows of dy
 //
 // A row belongs to a group of W warps (1, 2, 4 or 8 of a CTA's 8), its values stay in registers between the statistics and their use: one
-// pass over memory in either direction.  Chunks of 8 values where width, strides and addresses allow 16-byte accesses, single values
-// otherwise.  Statistics, sums and products in fp32 whatever the tensors' types.
+// pass over memory in either direction, which is what bounds both.  Rows come through shared memory by bulk copies, one row ahead of the one
+// that a group works on: loads into registers left the memory idle while a warp reduced (22 470 x 1024, fp32 rows: backward 140 us).  A
+// copy takes the 16-byte units that hold the row, whatever its address; they are read in chunks of 8 values where width, strides and
+// addresses allow 16-byte accesses and one value per lane otherwise.  Statistics, sums and products in fp32 whatever the tensors' types.
 // The weight's gradient is summed in registers over the rows of a group, over the groups of a CTA through shared memory in their order, and
 // over the CTAs by a second launch: no atomics, the same bits from run to run.
-#include "kf_common.cuh"
+#include "kf_sm100.cuh"
 
 namespace kf {
 
@@ -35,12 +37,12 @@ __device__ __forceinline__ float2 ln_unpack2(uint32_t w) {
 template <int CH, typename T>
 __device__ __forceinline__ void ln_load(const T* p, float (&v)[CH]) {
   if constexpr (CH == 1) {
-    v[0] = ln_to_float(__ldg(p));
+    v[0] = ln_to_float(*p);
   } else if constexpr (sizeof(T) == 4) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
   } else {
-    const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -90,17 +92,65 @@ struct LnArgs {
   float* part;                       // backward: [gridDim.x][2][d]
   int64_t ldx, lddy, ldres;
   int rows, d, W;
+  int slot_x, slot_y, slot_r;        // bytes of a row's place in shared memory, per tensor (multiples of 16; 0: not there)
   float eps, inv_d;
+  unsigned int* err;
 };
+
+constexpr int LN_RING = 2;
+
+// Row `row` of a [rows, d] tensor on its way to shared memory: the 16-byte units that hold it (they lie in the same allocation, whose
+// granularity is coarser); values of the row start at byte (address & 15) of the copy.
+template <typename T>
+__device__ __forceinline__ uint32_t ln_row_bytes(const T* p, int d) { return (uint32_t)(((reinterpret_cast<uintptr_t>(p) & 15) + (size_t)d * sizeof(T) + 15) & ~(size_t)15); }
+template <typename T>
+__device__ __forceinline__ void ln_row_copy(uint8_t* dst, const T* p, int d, uint64_t* bar) {
+  bulk_load_1d(dst, reinterpret_cast<const void*>(reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)15), ln_row_bytes(p, d), bar);
+}
+template <typename T>
+__device__ __forceinline__ const T* ln_row_at(const uint8_t* slot, const T* p) { return reinterpret_cast<const T*>(slot + (reinterpret_cast<uintptr_t>(p) & 15)); }
+
+// Behind a wait that ran out: time for the copies in flight, before the shared memory may be another CTA's.
+__device__ __forceinline__ void ln_drain(bool ok) {
+  if (!ok)
+    for (int i = 0; i < 64; ++i) __nanosleep(2000);
+}
 
 template <typename TI, typename TO, int CH, int NC>
 __global__ void __launch_bounds__(LN_THREADS) layer_norm_fwd_kernel(const __grid_constant__ LnArgs a) {
+  extern __shared__ __align__(128) uint8_t ln_smem[];
   __shared__ float2 red[2][LN_WARPS];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __shared__ uint64_t bars[LN_WARPS][LN_RING];
+  __shared__ volatile uint32_t abort_flag;
+  const int lane = threadIdx.x & 31, warp = warp_index();
   const int group = warp / a.W, groups = LN_WARPS / a.W, t = (warp - group * a.W) * 32 + lane, step = a.W * 32;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < LN_WARPS; ++i)
+      for (int k = 0; k < LN_RING; ++k) mbar_init(&bars[i][k], 1);
+    abort_flag = 0u;
+    fence_mbar_init();
+  }
+  __syncthreads();
   pdl_wait();
-  for (int64_t row = (int64_t)blockIdx.x * groups + group; row < a.rows; row += (int64_t)gridDim.x * groups) {
-    const TI* x = static_cast<const TI*>(a.x) + row * a.ldx;
+  const WaitCtx ctx{&abort_flag, a.err};
+  uint8_t* ring = ln_smem + (size_t)group * LN_RING * a.slot_x;
+  const TI* const x0 = static_cast<const TI*>(a.x);
+  const int64_t first = (int64_t)blockIdx.x * groups + group, stride = (int64_t)gridDim.x * groups;
+  bool ok = true;                                                // a group whose wait ran out goes on, without asking for more: its warps meet at barriers
+  auto request = [&](int64_t row, int slot) {                    // one lane of the group
+    if (t == 0 && row < a.rows && ok) {
+      const TI* p = x0 + row * a.ldx;
+      mbar_expect_tx(&bars[group][slot], ln_row_bytes(p, a.d));
+      ln_row_copy(ring + slot * a.slot_x, p, a.d, &bars[group][slot]);
+    }
+  };
+  request(first, 0);
+  int k = 0;
+  for (int64_t row = first; row < a.rows; row += stride, ++k) {
+    const int slot = k % LN_RING;
+    if (a.W == 1) request(row + stride, (k + 1) % LN_RING);      // (a group of several warps asks behind the barrier of its sums)
+    ok = mbar_wait_warp(&bars[group][slot], (k / LN_RING) & 1, ctx, 80) && ok;
+    const TI* x = ln_row_at(ring + slot * a.slot_x, x0 + row * a.ldx);
     float v[NC][CH];
     float2 s = make_float2(0.f, 0.f);
 #pragma unroll
@@ -118,6 +168,7 @@ __global__ void __launch_bounds__(LN_THREADS) layer_norm_fwd_kernel(const __grid
 #pragma unroll
       for (int j = 0; j < CH; ++j) s.x += v[i][j];
     const float mean = ln_group_sum(s, a.W, group, warp, lane, red[0]).x * a.inv_d;
+    if (a.W > 1) request(row + stride, (k + 1) % LN_RING);       // every warp is through with the row before
     s.x = 0.f;
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
@@ -151,16 +202,47 @@ __global__ void __launch_bounds__(LN_THREADS) layer_norm_fwd_kernel(const __grid
       a.mean[row] = mean;
       a.rstd[row] = rstd;
     }
+    __syncwarp();                                                // the slot's values have been read by all lanes
   }
+  ln_drain(ok);
 }
 
 template <typename TI, typename TO, int CH, int NC>
 __global__ void __launch_bounds__(LN_THREADS) layer_norm_bwd_kernel(const __grid_constant__ LnArgs a) {
-  extern __shared__ float colsum[];  // [2][d], where a CTA has more than one group
+  extern __shared__ __align__(128) uint8_t ln_smem[];
   __shared__ float2 red[2][LN_WARPS];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __shared__ uint64_t bars[LN_WARPS][LN_RING];
+  __shared__ volatile uint32_t abort_flag;
+  const int lane = threadIdx.x & 31, warp = warp_index();
   const int group = warp / a.W, groups = LN_WARPS / a.W, t = (warp - group * a.W) * 32 + lane, step = a.W * 32;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < LN_WARPS; ++i)
+      for (int k = 0; k < LN_RING; ++k) mbar_init(&bars[i][k], 1);
+    abort_flag = 0u;
+    fence_mbar_init();
+  }
+  __syncthreads();
   pdl_wait();
+  const WaitCtx ctx{&abort_flag, a.err};
+  const int slot_bytes = a.slot_x + a.slot_y + a.slot_r;
+  uint8_t* ring = ln_smem + (size_t)group * LN_RING * slot_bytes;
+  const TI *const x0 = static_cast<const TI*>(a.x), *const r0 = static_cast<const TI*>(a.dres);
+  const TO* const y0 = static_cast<const TO*>(a.dy);
+  const int64_t first = (int64_t)blockIdx.x * groups + group, stride = (int64_t)gridDim.x * groups;
+  bool ok = true;                                                // a group whose wait ran out goes on, without asking for more: its warps meet at barriers
+  auto request = [&](int64_t row, int slot) {                    // one lane of the group
+    if (t == 0 && row < a.rows && ok) {
+      const TI* p = x0 + row * a.ldx;
+      const TO* q = y0 + row * a.lddy;
+      uint64_t* bar = &bars[group][slot];
+      uint8_t* to = ring + slot * slot_bytes;
+      mbar_expect_tx(bar, ln_row_bytes(p, a.d) + ln_row_bytes(q, a.d) + (r0 ? ln_row_bytes(r0 + row * a.ldres, a.d) : 0));
+      ln_row_copy(to, p, a.d, bar);
+      ln_row_copy(to + a.slot_x, q, a.d, bar);
+      if (r0) ln_row_copy(to + a.slot_x + a.slot_y, r0 + row * a.ldres, a.d, bar);
+    }
+  };
+  request(first, 0);
   float w[NC][CH], aw[NC][CH], ab[NC][CH];
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
@@ -174,11 +256,17 @@ __global__ void __launch_bounds__(LN_THREADS) layer_norm_bwd_kernel(const __grid
 #pragma unroll
     for (int j = 0; j < CH; ++j) aw[i][j] = ab[i][j] = 0.f;
   }
-  int turn = 0;
-  for (int64_t row = (int64_t)blockIdx.x * groups + group; row < a.rows; row += (int64_t)gridDim.x * groups, turn ^= 1) {
-    const TI* x = static_cast<const TI*>(a.x) + row * a.ldx;
-    const TO* dy = static_cast<const TO*>(a.dy) + row * a.lddy;
-    const float mean = __ldg(a.mean + row), rstd = __ldg(a.rstd + row);
+  int k = 0;
+  float mean = first < a.rows ? __ldg(a.mean + first) : 0.f, rstd = first < a.rows ? __ldg(a.rstd + first) : 0.f;
+  for (int64_t row = first; row < a.rows; row += stride, ++k) {
+    const int slot = k % LN_RING;
+    if (a.W == 1) request(row + stride, (k + 1) % LN_RING);
+    const bool more = row + stride < a.rows;
+    const float next_mean = more ? __ldg(a.mean + row + stride) : 0.f, next_rstd = more ? __ldg(a.rstd + row + stride) : 0.f;
+    ok = mbar_wait_warp(&bars[group][slot], (k / LN_RING) & 1, ctx, 81) && ok;
+    const uint8_t* from = ring + slot * slot_bytes;
+    const TI* x = ln_row_at(from, x0 + row * a.ldx);
+    const TO* dy = ln_row_at(from + a.slot_x, y0 + row * a.lddy);
     float xh[NC][CH], g[NC][CH];
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
@@ -206,10 +294,11 @@ __global__ void __launch_bounds__(LN_THREADS) layer_norm_bwd_kernel(const __grid
         s.x += g[i][j];
         s.y = fmaf(g[i][j], xh[i][j], s.y);
       }
-    s = ln_group_sum(s, a.W, group, warp, lane, red[turn]);
+    s = ln_group_sum(s, a.W, group, warp, lane, red[k & 1]);
+    if (a.W > 1) request(row + stride, (k + 1) % LN_RING);       // every warp is through with the row before
     const float m1 = s.x * a.inv_d, m2 = s.y * a.inv_d;
     TI* dx = static_cast<TI*>(a.dx) + row * a.d;
-    const TI* dres = a.dres ? static_cast<const TI*>(a.dres) + row * a.ldres : nullptr;
+    const TI* dres = r0 ? ln_row_at(from + a.slot_x + a.slot_y, r0 + row * a.ldres) : nullptr;
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       const int c = (t + i * step) * CH;
@@ -223,20 +312,27 @@ __global__ void __launch_bounds__(LN_THREADS) layer_norm_bwd_kernel(const __grid
         ln_store<CH>(dx + c, r);
       }
     }
+    mean = next_mean;
+    rstd = next_rstd;
+    __syncwarp();                                                // the slot's values have been read by all lanes
   }
-  // the groups of this CTA, in their order; then the CTA's line of the partial sums
+  // the groups of this CTA, in their order, where the ring was; then the CTA's line of the partial sums
+  ln_drain(ok);
+  __syncthreads();
+  if (abort_flag) return;
+  float* colsum = reinterpret_cast<float*>(ln_smem);             // [2][d], where a CTA has more than one group
   float* part = a.part + (size_t)blockIdx.x * 2 * a.d;
-  for (int k = 0; k < groups; ++k) {
-    if (group == k) {
-      float* to = k == groups - 1 ? part : colsum;
+  for (int g = 0; g < groups; ++g) {
+    if (group == g) {
+      float* to = g == groups - 1 ? part : colsum;
 #pragma unroll
       for (int i = 0; i < NC; ++i) {
         const int c = (t + i * step) * CH;
         if (c < a.d) {
 #pragma unroll
           for (int j = 0; j < CH; ++j) {
-            to[c + j] = k ? colsum[c + j] + aw[i][j] : aw[i][j];
-            to[a.d + c + j] = k ? colsum[a.d + c + j] + ab[i][j] : ab[i][j];
+            to[c + j] = g ? colsum[c + j] + aw[i][j] : aw[i][j];
+            to[a.d + c + j] = g ? colsum[a.d + c + j] + ab[i][j] : ab[i][j];
           }
         }
       }
@@ -245,40 +341,72 @@ __global__ void __launch_bounds__(LN_THREADS) layer_norm_bwd_kernel(const __grid
   }
 }
 
-// dw, db = the sum of `n` lines [2][d]: 32 columns per CTA, 8 threads per column
-__global__ void __launch_bounds__(256) layer_norm_cols_kernel(const float* __restrict__ part, int n, int d, float* __restrict__ dw, float* __restrict__ db) {
-  __shared__ float sm[8][33];
+// dw, db = the sum of `n` lines [2][d]: 32 columns per CTA, 32 threads per column
+__global__ void __launch_bounds__(1024) layer_norm_cols_kernel(const float* __restrict__ part, int n, int d, float* __restrict__ dw, float* __restrict__ db) {
+  __shared__ float sm[32][33];
   pdl_wait();
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int64_t c = (int64_t)blockIdx.x * 32 + tx;
   float s = 0.f;
   if (c < 2 * (int64_t)d) {
-#pragma unroll 4
-    for (int i = ty; i < n; i += 8) s += part[(size_t)i * 2 * d + c];
+#pragma unroll 8
+    for (int i = ty; i < n; i += 32) s += part[(size_t)i * 2 * d + c];
   }
   sm[ty][tx] = s;
   __syncthreads();
-  if (ty == 0 && c < 2 * (int64_t)d) {
+  s = sm[tx][ty];                                                // a warp per column
 #pragma unroll
-    for (int k = 1; k < 8; ++k) s += sm[k][tx];
-    if (c < d) dw[c] = s;
-    else if (db) db[c - d] = s;
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  const int64_t col = (int64_t)blockIdx.x * 32 + ty;
+  if (tx == 0 && col < 2 * (int64_t)d) {
+    if (col < d) dw[col] = s;
+    else if (db) db[col - d] = s;
   }
 }
 
 // warps per row: at most 32 values per thread
 static int ln_warps(int d) { return d <= 1024 ? 1 : d <= 2048 ? 2 : d <= 4096 ? 4 : 8; }
 
-static int ln_grid(int64_t rows, int d, int per_sm, int* grid) {
+// CTAs: as many as the device holds at once with this much shared memory each, or as there are rows for
+constexpr int LN_SMEM_SM = 222 * 1024, LN_MAX_PER_SM = 4;       // shared memory of an SM less what the CTAs take beside their rings; registers allow no more
+static int ln_slot(int64_t d, int64_t size) { return (int)((d * size + 15 + 15) & ~15ll); }      // wherever the row starts in its first 16 bytes
+static size_t ln_smem_bytes(int d, int slot_bytes, bool cols) {
+  const int groups = LN_WARPS / ln_warps(d);
+  const size_t ring = (size_t)groups * LN_RING * slot_bytes, sums = cols && groups > 1 ? (size_t)2 * d * 4 : 0;
+  return ring > sums ? ring : sums;
+}
+static int ln_grid(int64_t rows, int d, size_t smem, int regs, int* grid) {
   int sms = 0;
   const int rc = device_sm_count(&sms);
   if (rc != KF_OK) return rc;
   const int groups = LN_WARPS / ln_warps(d);
+  int per_sm = (int)(LN_SMEM_SM / (smem + 2048));
+  if (regs > 0 && per_sm > 65536 / (regs * LN_THREADS)) per_sm = 65536 / (regs * LN_THREADS);
+  per_sm = per_sm < 1 ? 1 : per_sm > LN_MAX_PER_SM ? LN_MAX_PER_SM : per_sm;
   const int64_t blocks = (rows + groups - 1) / groups, most = (int64_t)sms * per_sm;
   *grid = (int)(blocks < most ? blocks : most);
   return KF_OK;
 }
-constexpr int LN_FWD_PER_SM = 8, LN_BWD_PER_SM = 2;
+
+// ws_bytes: room for the lines of the partial sums (backward; -1: none are made); *grid: the CTAs that were launched
+template <void (*kern)(const LnArgs)>
+static int ln_launch(const char* what, int64_t rows, size_t smem, cudaStream_t st, const LnArgs& a, int64_t ws_bytes, int* grid) {
+  static PerDevice<int> kept;                                     // registers per thread of this instantiation
+  int dev = 0;
+  cudaGetDevice(&dev);
+  int regs = kept.get(dev);
+  if (!regs) {
+    cudaFuncAttributes attr;
+    cudaError_t e = cudaFuncGetAttributes(&attr, kern);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024);
+    if (e != cudaSuccess) return cuda_status(e, "attributes of layer_norm");
+    kept.put(dev, regs = attr.numRegs);
+  }
+  const int rc = ln_grid(rows, a.d, smem, regs, grid);
+  if (rc != KF_OK) return rc;
+  KF_REQUIRE(ws_bytes < 0 || ws_bytes >= (int64_t)*grid * 2 * a.d * 4, "kf_layer_norm_bwd: workspace of %lld bytes, needs %lld", (long long)ws_bytes, (long long)*grid * 2 * a.d * 4);
+  return cuda_status(launch_maybe_pdl(rows, kern, dim3(*grid), dim3(LN_THREADS), smem, st, a), what);
+}
 
 // f(TI, TO, CH, NC) for the types, the access width and the values per thread of a call
 template <typename TI, typename TO, typename F>
@@ -323,7 +451,7 @@ extern "C" int64_t kf_layer_norm_ws_bytes(int64_t rows, int d) {
     return KF_ERR_BAD_ARGUMENT;
   }
   int grid = 0;
-  const int rc = ln_grid(rows, d, LN_BWD_PER_SM, &grid);
+  const int rc = ln_grid(rows, d, 0, 0, &grid);                  // no launch makes more lines
   if (rc != KF_OK) return rc > 0 ? KF_ERR_UNSUPPORTED : rc;
   return (int64_t)grid * 2 * d * 4;
 }
@@ -336,14 +464,15 @@ extern "C" int kf_layer_norm_fwd(int in_dtype, const void* x, int64_t ldx, const
   KF_REQUIRE(x && w && y && mean && rstd, "kf_layer_norm_fwd: null pointer");
   LnArgs a{};
   a.x = x; a.ldx = ldx; a.w = w; a.b = b; a.mean = mean; a.rstd = rstd; a.y = y; a.rows = rows; a.d = d; a.W = ln_warps(d); a.eps = eps; a.inv_d = 1.0f / (float)d;
+  a.slot_x = ln_slot(d, ln_size(in_dtype));
+  a.err = dev_error_ptr();
+  KF_REQUIRE(a.err != nullptr, "kf_layer_norm_fwd: device error word unavailable");
   const bool wide = d % 8 == 0 && ln_aligned(x, ldx * ln_size(in_dtype)) && ln_aligned(y, 0) && ln_aligned(w, 0) && ln_aligned(b, 0);
+  const size_t smem = ln_smem_bytes(d, a.slot_x, false);
   int grid = 0;
-  const int rc = ln_grid(rows, d, LN_FWD_PER_SM, &grid);
-  if (rc != KF_OK) return rc;
   return ln_by_type(in_dtype, out_dtype, wide, d, [&](auto ti, auto to, auto ch, auto nc) {
-    return cuda_status(launch_maybe_pdl(rows, layer_norm_fwd_kernel<decltype(ti), decltype(to), decltype(ch)::value, decltype(nc)::value>, dim3(grid), dim3(LN_THREADS), 0,
-                                        static_cast<cudaStream_t>(stream), a),
-                       "kf_layer_norm_fwd launch");
+    return ln_launch<layer_norm_fwd_kernel<decltype(ti), decltype(to), decltype(ch)::value, decltype(nc)::value>>("kf_layer_norm_fwd launch", rows, smem,
+                     static_cast<cudaStream_t>(stream), a, -1, &grid);
   });
 }
 
@@ -361,21 +490,22 @@ extern "C" int kf_layer_norm_bwd(int in_dtype, const void* x, int64_t ldx, int d
     return cuda_status(e, "kf_layer_norm_bwd memset");
   }
   KF_REQUIRE(x && dy && mean && rstd && dx && ws, "kf_layer_norm_bwd: null pointer");
-  int grid = 0;
-  int rc = ln_grid(rows, d, LN_BWD_PER_SM, &grid);
-  if (rc != KF_OK) return rc;
-  KF_REQUIRE(ws_bytes >= (int64_t)grid * 2 * d * 4, "kf_layer_norm_bwd: workspace of %lld bytes, needs %lld", (long long)ws_bytes, (long long)grid * 2 * d * 4);
   LnArgs a{};
   a.x = x; a.ldx = ldx; a.dy = dy; a.lddy = lddy; a.dres = dres; a.ldres = ldres; a.w = w; a.mean = const_cast<float*>(mean); a.rstd = const_cast<float*>(rstd);
   a.dx = dx; a.part = static_cast<float*>(ws); a.rows = rows; a.d = d; a.W = ln_warps(d); a.inv_d = 1.0f / (float)d;
+  a.slot_x = ln_slot(d, ln_size(in_dtype));
+  a.slot_y = ln_slot(d, ln_size(dy_dtype));
+  a.slot_r = dres ? a.slot_x : 0;
+  a.err = dev_error_ptr();
+  KF_REQUIRE(a.err != nullptr, "kf_layer_norm_bwd: device error word unavailable");
+  const size_t smem = ln_smem_bytes(d, a.slot_x + a.slot_y + a.slot_r, true);
+  int grid = 0;
   const bool wide = d % 8 == 0 && ln_aligned(x, ldx * ln_size(in_dtype)) && ln_aligned(dy, lddy * ln_size(dy_dtype)) && ln_aligned(dres, ldres * ln_size(in_dtype)) &&
                     ln_aligned(dx, 0) && ln_aligned(w, 0);
-  const size_t smem = a.W < LN_WARPS ? (size_t)2 * d * 4 : 0;
-  rc = ln_by_type(in_dtype, dy_dtype, wide, d, [&](auto ti, auto to, auto ch, auto nc) {
-    return cuda_status(launch_maybe_pdl(rows, layer_norm_bwd_kernel<decltype(ti), decltype(to), decltype(ch)::value, decltype(nc)::value>, dim3(grid), dim3(LN_THREADS), smem, st, a),
-                       "kf_layer_norm_bwd launch");
+  const int rc = ln_by_type(in_dtype, dy_dtype, wide, d, [&](auto ti, auto to, auto ch, auto nc) {
+    return ln_launch<layer_norm_bwd_kernel<decltype(ti), decltype(to), decltype(ch)::value, decltype(nc)::value>>("kf_layer_norm_bwd launch", rows, smem, st, a, ws_bytes, &grid);
   });
   if (rc != KF_OK) return rc;
-  return cuda_status(launch_maybe_pdl(rows, layer_norm_cols_kernel, dim3((2 * d + 31) / 32), dim3(256), 0, st, static_cast<const float*>(ws), grid, d, dw, db),
+  return cuda_status(launch_maybe_pdl(1, layer_norm_cols_kernel, dim3((2 * d + 31) / 32), dim3(1024), 0, st, static_cast<const float*>(ws), grid, d, dw, db),
                      "kf_layer_norm_bwd column sums launch");
 }

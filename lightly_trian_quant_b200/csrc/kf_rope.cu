@@ -6,13 +6,13 @@
 //
 // Bound by memory: x is read once and y written once.  An angle is worked out once per token and pair for all heads: the product in fp64
 // and reduced to half turns there (a position of 10^6 times a frequency of 1 leaves fp32 with less than two digits of the angle), sine and
-// cosine of the reduced angle in fp32 with its rounding put right to first order.  A thread owns one chunk of a head's channels, keeps
-// its sines and cosines in registers and goes through the heads.
+// cosine of the reduced angle in fp32 with its rounding put right to first order.  A CTA takes a few tokens; its threads ask for their
+// first chunks of x, then work out the angles of the tokens while those are on their way.
 #include "kf_common.cuh"
 
 namespace kf {
 
-constexpr int ROPE_THREADS = 256, ROPE_MAX_PAIRS = 128, ROPE_TOKENS = 8;
+constexpr int ROPE_THREADS = 256, ROPE_MAX_PAIRS = 128, ROPE_MAX_TOKENS = 16, ROPE_ITEMS = 4;     // chunks (or pairs of chunks) per thread in flight
 
 struct RopeArgs {
   const void *x, *pos;
@@ -22,7 +22,8 @@ struct RopeArgs {
   int64_t xs_g, xs_t, xs_h, ys_g, ys_t, ys_h;   // strides in elements: outer, token, head
   int64_t ps_t, ps_a;                // strides of pos
   int G, T, H, D, P;
-  int inverse;
+  int inverse, tokens;               // tokens per CTA
+  uint64_t by_chunks, by_heads;      // 2^32 / n rounded up: a division of less than 2^16 by a multiplication
 };
 
 template <typename T, int V>
@@ -32,71 +33,77 @@ struct alignas(sizeof(T) * V < 16 ? sizeof(T) * V : 16) RopeVec {
 
 template <typename T, typename TP, int V, bool INTER>
 __global__ void __launch_bounds__(ROPE_THREADS) rope_axes_kernel(const __grid_constant__ RopeArgs a) {
-  __shared__ float2 turn[ROPE_TOKENS * ROPE_MAX_PAIRS];            // (cos, sin)
+  extern __shared__ float2 turn[];                                 // (cos, sin) [tokens][P]
   pdl_wait();
-  // chunks of a head: half layout: P / V pairs of chunks, then what passes through; interleaved: 2P / V chunks, then what passes through
+  using Vec = RopeVec<T, V>;
+  // items of a head: half layout: P / V pairs of chunks, then what passes through; interleaved: 2P / V chunks, then what passes through
   const int rot = INTER ? 2 * a.P / V : a.P / V, nc = rot + (a.D - 2 * a.P) / V;
-  const int per = ROPE_THREADS / nc;                               // heads in flight
-  const int c = threadIdx.x % nc, h0 = threadIdx.x / nc;
-  for (int64_t t0 = (int64_t)blockIdx.x * ROPE_TOKENS; t0 < a.T; t0 += (int64_t)gridDim.x * ROPE_TOKENS) {
-    const int nt = a.T - t0 < ROPE_TOKENS ? (int)(a.T - t0) : ROPE_TOKENS;
-    for (int i = threadIdx.x; i < nt * a.P; i += ROPE_THREADS) {
-      const int k = i / a.P, p = i - k * a.P;
-      const double half = (double)static_cast<const TP*>(a.pos)[(t0 + k) * a.ps_t + a.axis[p] * a.ps_a] * a.freq[p];
-      const double r = half - 2.0 * rint(0.5 * half);              // [-1, 1]
-      const float rf = (float)r;
-      const float rest = (float)(r - (double)rf) * 3.14159265358979f;
-      float s, co;
-      sincospif(rf, &s, &co);
-      turn[k * a.P + p] = make_float2(fmaf(-s, rest, co), a.inverse ? -fmaf(co, rest, s) : fmaf(co, rest, s));
-    }
-    __syncthreads();
-    if (h0 < per) {
-      for (int k = 0; k < nt; ++k) {
-        const T* xt = static_cast<const T*>(a.x) + (t0 + k) * a.xs_t;
-        T* yt = static_cast<T*>(a.y) + (t0 + k) * a.ys_t;
-        if (c >= rot) {
-          const int e = 2 * a.P + (c - rot) * V;
-          for (int g = 0; g < a.G; ++g)
-            for (int h = h0; h < a.H; h += per)
-              *reinterpret_cast<RopeVec<T, V>*>(yt + g * a.ys_g + h * a.ys_h + e) = *reinterpret_cast<const RopeVec<T, V>*>(xt + g * a.xs_g + h * a.xs_h + e);
-        } else if constexpr (INTER) {
-          float2 cs[V / 2];
+  const int64_t t0 = (int64_t)blockIdx.x * a.tokens;
+  const int nt = a.T - t0 < a.tokens ? (int)(a.T - t0) : a.tokens, items = nt * a.H * nc;
+  const T* const x0 = static_cast<const T*>(a.x) + blockIdx.y * a.xs_g + t0 * a.xs_t;
+  T* const y0 = static_cast<T*>(a.y) + blockIdx.y * a.ys_g + t0 * a.ys_t;
+  Vec lo[ROPE_ITEMS], hi[INTER ? 1 : ROPE_ITEMS];
+  int at_c[ROPE_ITEMS], at_k[ROPE_ITEMS];
+  int64_t to[ROPE_ITEMS];
+  auto load = [&](int base) {
 #pragma unroll
-          for (int j = 0; j < V / 2; ++j) cs[j] = turn[k * a.P + c * (V / 2) + j];
-          for (int g = 0; g < a.G; ++g)
-            for (int h = h0; h < a.H; h += per) {
-              RopeVec<T, V> u = *reinterpret_cast<const RopeVec<T, V>*>(xt + g * a.xs_g + h * a.xs_h + c * V);
-#pragma unroll
-              for (int j = 0; j < V / 2; ++j) {
-                const float p = (float)u.v[2 * j], q = (float)u.v[2 * j + 1];
-                u.v[2 * j] = (T)(p * cs[j].x - q * cs[j].y);
-                u.v[2 * j + 1] = (T)(q * cs[j].x + p * cs[j].y);
-              }
-              *reinterpret_cast<RopeVec<T, V>*>(yt + g * a.ys_g + h * a.ys_h + c * V) = u;
-            }
-        } else {
-          float2 cs[V];
-#pragma unroll
-          for (int j = 0; j < V; ++j) cs[j] = turn[k * a.P + c * V + j];
-          for (int g = 0; g < a.G; ++g)
-            for (int h = h0; h < a.H; h += per) {
-              const T* xp = xt + g * a.xs_g + h * a.xs_h + c * V;
-              RopeVec<T, V> lo = *reinterpret_cast<const RopeVec<T, V>*>(xp), hi = *reinterpret_cast<const RopeVec<T, V>*>(xp + a.P);
-#pragma unroll
-              for (int j = 0; j < V; ++j) {
-                const float p = (float)lo.v[j], q = (float)hi.v[j];
-                lo.v[j] = (T)(p * cs[j].x - q * cs[j].y);
-                hi.v[j] = (T)(q * cs[j].x + p * cs[j].y);
-              }
-              T* yp = yt + g * a.ys_g + h * a.ys_h + c * V;
-              *reinterpret_cast<RopeVec<T, V>*>(yp) = lo;
-              *reinterpret_cast<RopeVec<T, V>*>(yp + a.P) = hi;
-            }
+    for (int u = 0; u < ROPE_ITEMS; ++u) {
+      const uint32_t i = base + u * ROPE_THREADS + threadIdx.x;
+      if ((int)i < items) {
+        const uint32_t th = (uint32_t)(i * a.by_chunks >> 32), c = i - th * nc, k = (uint32_t)(th * a.by_heads >> 32), h = th - k * a.H;
+        const int e = (int)c < rot ? c * V : 2 * a.P + ((int)c - rot) * V;
+        const T* p = x0 + k * a.xs_t + h * a.xs_h + e;
+        lo[u] = *reinterpret_cast<const Vec*>(p);
+        if constexpr (!INTER) {
+          if ((int)c < rot) hi[u] = *reinterpret_cast<const Vec*>(p + a.P);
         }
+        at_c[u] = c;
+        at_k[u] = k;
+        to[u] = k * a.ys_t + h * a.ys_h + e;
       }
     }
-    __syncthreads();
+  };
+  load(0);
+  for (int i = threadIdx.x; i < nt * a.P; i += ROPE_THREADS) {
+    const int k = i / a.P, p = i - k * a.P;
+    const double half = (double)static_cast<const TP*>(a.pos)[(t0 + k) * a.ps_t + a.axis[p] * a.ps_a] * a.freq[p];
+    const double r = half - 2.0 * rint(0.5 * half);                // [-1, 1]
+    const float rf = (float)r;
+    const float rest = (float)(r - (double)rf) * 3.14159265358979f;
+    float s, co;
+    sincospif(rf, &s, &co);
+    turn[i] = make_float2(fmaf(-s, rest, co), a.inverse ? -fmaf(co, rest, s) : fmaf(co, rest, s));
+  }
+  __syncthreads();
+  for (int base = 0; base < items; base += ROPE_ITEMS * ROPE_THREADS) {
+    if (base) load(base);
+#pragma unroll
+    for (int u = 0; u < ROPE_ITEMS; ++u) {
+      if ((int)(base + u * ROPE_THREADS + threadIdx.x) >= items) break;
+      T* q = y0 + to[u];
+      if (at_c[u] < rot) {
+        const float2* cs = turn + at_k[u] * a.P + at_c[u] * (INTER ? V / 2 : V);
+        if constexpr (INTER) {
+#pragma unroll
+          for (int j = 0; j < V / 2; ++j) {
+            const float2 t = cs[j];
+            const float m = (float)lo[u].v[2 * j], n = (float)lo[u].v[2 * j + 1];
+            lo[u].v[2 * j] = (T)(m * t.x - n * t.y);
+            lo[u].v[2 * j + 1] = (T)(n * t.x + m * t.y);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            const float2 t = cs[j];
+            const float m = (float)lo[u].v[j], n = (float)hi[u].v[j];
+            lo[u].v[j] = (T)(m * t.x - n * t.y);
+            hi[u].v[j] = (T)(n * t.x + m * t.y);
+          }
+          *reinterpret_cast<Vec*>(q + a.P) = hi[u];
+        }
+      }
+      *reinterpret_cast<Vec*>(q) = lo[u];
+    }
   }
 }
 
@@ -105,29 +112,30 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_axes_kernel(const __grid_co
 using namespace kf;
 
 template <typename T, typename TP, int V>
-static int rope_launch(const RopeArgs& a, int interleaved, int grid, cudaStream_t st) {
+static int rope_launch(const RopeArgs& a, int interleaved, dim3 grid, cudaStream_t st) {
   cudaError_t e;
+  const size_t smem = (size_t)a.tokens * a.P * sizeof(float2);
   if (interleaved) {
     if constexpr (V == 1) {
       set_error("kf_rope_axes: interleaved pairs need an even alignment");
       return KF_ERR_BAD_ARGUMENT;
     } else {
-      e = launch_maybe_pdl(a.T, rope_axes_kernel<T, TP, V, true>, dim3(grid), dim3(ROPE_THREADS), 0, st, a);
+      e = launch_maybe_pdl((int64_t)a.T * a.G, rope_axes_kernel<T, TP, V, true>, grid, dim3(ROPE_THREADS), smem, st, a);
     }
   } else {
-    e = launch_maybe_pdl(a.T, rope_axes_kernel<T, TP, V, false>, dim3(grid), dim3(ROPE_THREADS), 0, st, a);
+    e = launch_maybe_pdl((int64_t)a.T * a.G, rope_axes_kernel<T, TP, V, false>, grid, dim3(ROPE_THREADS), smem, st, a);
   }
   return cuda_status(e, "kf_rope_axes launch");
 }
 template <typename T, typename TP>
-static int rope_by_width(const RopeArgs& a, int interleaved, int V, int grid, cudaStream_t st) {
+static int rope_by_width(const RopeArgs& a, int interleaved, int V, dim3 grid, cudaStream_t st) {
   if (V == 8) return rope_launch<T, TP, 8>(a, interleaved, grid, st);
   if (V == 4) return rope_launch<T, TP, 4>(a, interleaved, grid, st);
   if (V == 2) return rope_launch<T, TP, 2>(a, interleaved, grid, st);
   return rope_launch<T, TP, 1>(a, interleaved, grid, st);
 }
 template <typename T>
-static int rope_by_pos(const RopeArgs& a, int pos_kind, int interleaved, int V, int grid, cudaStream_t st) {
+static int rope_by_pos(const RopeArgs& a, int pos_kind, int interleaved, int V, dim3 grid, cudaStream_t st) {
   if (pos_kind == KF_POS_I32) return rope_by_width<T, int32_t>(a, interleaved, V, grid, st);
   if (pos_kind == KF_POS_I64) return rope_by_width<T, int64_t>(a, interleaved, V, grid, st);
   return rope_by_width<T, float>(a, interleaved, V, grid, st);
@@ -151,7 +159,7 @@ extern "C" int kf_rope_axes(const kf_rope_params* p, void* stream) {
   const int64_t strides = p->xs_g | p->xs_t | p->xs_h | p->ys_g | p->ys_t | p->ys_h;
   const uintptr_t base = reinterpret_cast<uintptr_t>(p->x) | reinterpret_cast<uintptr_t>(p->y);
   auto fits = [&](int v) {
-    return ((strides % v) | (p->D % v) | ((p->interleaved ? 2 * p->P : p->P) % v)) == 0 && base % (uintptr_t)(v * size) == 0 && p->D / v <= ROPE_THREADS;
+    return ((strides % v) | (p->D % v) | ((p->interleaved ? 2 * p->P : p->P) % v)) == 0 && base % (uintptr_t)(v * size) == 0;
   };
   while (V > 1 && !fits(V)) V >>= 1;
   KF_REQUIRE(base % (uintptr_t)size == 0, "kf_rope_axes: misaligned tensor");
@@ -161,8 +169,18 @@ extern "C" int kf_rope_axes(const kf_rope_params* p, void* stream) {
   int sms = 0;
   const int rc = device_sm_count(&sms);
   if (rc != KF_OK) return rc;
-  const int64_t blocks = ((int64_t)p->T + ROPE_TOKENS - 1) / ROPE_TOKENS;
-  const int grid = (int)(blocks < 8 * sms ? blocks : 8 * sms);
+  // Tokens per CTA: its threads' first items, but not so many that a short batch leaves SMs without one
+  const int nc = (p->interleaved ? 2 * p->P : p->P) / V + (p->D - 2 * p->P) / V;
+  KF_REQUIRE((int64_t)p->H * nc < 65536, "kf_rope_axes: %d heads of %d channels are more than a token may have", p->H, p->D);
+  KF_REQUIRE(p->G < 65536, "kf_rope_axes: outer dimension of %d", p->G);
+  int64_t tokens = (int64_t)ROPE_ITEMS * ROPE_THREADS / ((int64_t)p->H * nc);
+  const int64_t spread = ((int64_t)p->T * p->G + 2 * sms - 1) / (2 * sms);
+  tokens = tokens < spread ? tokens : spread;
+  tokens = tokens < 1 ? 1 : tokens > ROPE_MAX_TOKENS ? ROPE_MAX_TOKENS : tokens;
+  a.tokens = (int)tokens;
+  a.by_chunks = ((1ull << 32) + nc - 1) / nc;
+  a.by_heads = ((1ull << 32) + p->H - 1) / p->H;
+  const dim3 grid((unsigned)(((int64_t)p->T + tokens - 1) / tokens), (unsigned)p->G);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (p->dtype == KF_F32) return rope_by_pos<float>(a, p->pos_kind, p->interleaved, V, grid, st);
   if (p->dtype == KF_BF16) return rope_by_pos<__nv_bfloat16>(a, p->pos_kind, p->interleaved, V, grid, st);
