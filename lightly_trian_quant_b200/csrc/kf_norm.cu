@@ -145,6 +145,17 @@ __global__ void __launch_bounds__(LN_THREADS) layer_norm_fwd_kernel(const __grid
     }
   };
   request(first, 0);
+  float w[NC][CH], b[NC][CH];                                    // read once: per row they are twice the bytes of the row
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    const int c = (t + i * step) * CH;
+#pragma unroll
+    for (int j = 0; j < CH; ++j) w[i][j] = b[i][j] = 0.f;
+    if (c < a.d) {
+      ln_load<CH>(a.w + c, w[i]);
+      if (a.b) ln_load<CH>(a.b + c, b[i]);
+    }
+  }
   int k = 0;
   for (int64_t row = first; row < a.rows; row += stride, ++k) {
     const int slot = k % LN_RING;
@@ -185,16 +196,8 @@ __global__ void __launch_bounds__(LN_THREADS) layer_norm_fwd_kernel(const __grid
     for (int i = 0; i < NC; ++i) {
       const int c = (t + i * step) * CH;
       if (c < a.d) {
-        float w[CH], b[CH];
-        ln_load<CH>(a.w + c, w);
-        if (a.b) {
-          ln_load<CH>(a.b + c, b);
-        } else {
 #pragma unroll
-          for (int j = 0; j < CH; ++j) b[j] = 0.f;
-        }
-#pragma unroll
-        for (int j = 0; j < CH; ++j) v[i][j] = fmaf(v[i][j] * rstd, w[j], b[j]);
+        for (int j = 0; j < CH; ++j) v[i][j] = fmaf(v[i][j] * rstd, w[i][j], b[i][j]);
         ln_store<CH>(y + c, v[i]);
       }
     }
@@ -364,22 +367,26 @@ __global__ void __launch_bounds__(1024) layer_norm_cols_kernel(const float* __re
   }
 }
 
-// warps per row: at most 32 values per thread
-static int ln_warps(int d) { return d <= 1024 ? 1 : d <= 2048 ? 2 : d <= 4096 ? 4 : 8; }
+// Warps per row: at most 32 values per thread; in the backward pass, which keeps four arrays of them, 16 where eight warps are enough for that
+// (22 470 x 1024: one warp per row 72 us)
+static int ln_warps(int d, bool bwd) {
+  if (bwd) return d <= 512 ? 1 : d <= 1024 ? 2 : d <= 2048 ? 4 : 8;
+  return d <= 1024 ? 1 : d <= 2048 ? 2 : d <= 4096 ? 4 : 8;
+}
 
 // CTAs: as many as the device holds at once with this much shared memory each, or as there are rows for
 constexpr int LN_SMEM_SM = 222 * 1024, LN_MAX_PER_SM = 4;       // shared memory of an SM less what the CTAs take beside their rings; registers allow no more
 static int ln_slot(int64_t d, int64_t size) { return (int)((d * size + 15 + 15) & ~15ll); }      // wherever the row starts in its first 16 bytes
 static size_t ln_smem_bytes(int d, int slot_bytes, bool cols) {
-  const int groups = LN_WARPS / ln_warps(d);
+  const int groups = LN_WARPS / ln_warps(d, cols);
   const size_t ring = (size_t)groups * LN_RING * slot_bytes, sums = cols && groups > 1 ? (size_t)2 * d * 4 : 0;
   return ring > sums ? ring : sums;
 }
-static int ln_grid(int64_t rows, int d, size_t smem, int regs, int* grid) {
+static int ln_grid(int64_t rows, int W, size_t smem, int regs, int* grid) {
   int sms = 0;
   const int rc = device_sm_count(&sms);
   if (rc != KF_OK) return rc;
-  const int groups = LN_WARPS / ln_warps(d);
+  const int groups = LN_WARPS / W;
   int per_sm = (int)(LN_SMEM_SM / (smem + 2048));
   if (regs > 0 && per_sm > 65536 / (regs * LN_THREADS)) per_sm = 65536 / (regs * LN_THREADS);
   per_sm = per_sm < 1 ? 1 : per_sm > LN_MAX_PER_SM ? LN_MAX_PER_SM : per_sm;
@@ -402,7 +409,7 @@ static int ln_launch(const char* what, int64_t rows, size_t smem, cudaStream_t s
     if (e != cudaSuccess) return cuda_status(e, "attributes of layer_norm");
     kept.put(dev, regs = attr.numRegs);
   }
-  const int rc = ln_grid(rows, a.d, smem, regs, grid);
+  const int rc = ln_grid(rows, a.W, smem, regs, grid);
   if (rc != KF_OK) return rc;
   KF_REQUIRE(ws_bytes < 0 || ws_bytes >= (int64_t)*grid * 2 * a.d * 4, "kf_layer_norm_bwd: workspace of %lld bytes, needs %lld", (long long)ws_bytes, (long long)*grid * 2 * a.d * 4);
   return cuda_status(launch_maybe_pdl(rows, kern, dim3(*grid), dim3(LN_THREADS), smem, st, a), what);
@@ -410,8 +417,8 @@ static int ln_launch(const char* what, int64_t rows, size_t smem, cudaStream_t s
 
 // f(TI, TO, CH, NC) for the types, the access width and the values per thread of a call
 template <typename TI, typename TO, typename F>
-static int ln_by_width(bool wide, int d, F&& f) {
-  const int lanes = ln_warps(d) * 32;
+static int ln_by_width(bool wide, int d, int W, F&& f) {
+  const int lanes = W * 32;
   if (wide) {
     const int n = (d / 8 + lanes - 1) / lanes;
     if (n <= 1) return f(TI{}, TO{}, std::integral_constant<int, 8>{}, std::integral_constant<int, 1>{});
@@ -425,16 +432,16 @@ static int ln_by_width(bool wide, int d, F&& f) {
   return f(TI{}, TO{}, std::integral_constant<int, 1>{}, std::integral_constant<int, 32>{});
 }
 template <typename TI, typename F>
-static int ln_by_out(int out_dtype, bool wide, int d, F&& f) {
-  if (out_dtype == KF_F32) return ln_by_width<TI, float>(wide, d, f);
-  if (out_dtype == KF_BF16) return ln_by_width<TI, __nv_bfloat16>(wide, d, f);
-  return ln_by_width<TI, __half>(wide, d, f);
+static int ln_by_out(int out_dtype, bool wide, int d, int W, F&& f) {
+  if (out_dtype == KF_F32) return ln_by_width<TI, float>(wide, d, W, f);
+  if (out_dtype == KF_BF16) return ln_by_width<TI, __nv_bfloat16>(wide, d, W, f);
+  return ln_by_width<TI, __half>(wide, d, W, f);
 }
 template <typename F>
-static int ln_by_type(int in_dtype, int out_dtype, bool wide, int d, F&& f) {
-  if (in_dtype == KF_F32) return ln_by_out<float>(out_dtype, wide, d, f);
-  if (in_dtype == KF_BF16) return ln_by_out<__nv_bfloat16>(out_dtype, wide, d, f);
-  return ln_by_out<__half>(out_dtype, wide, d, f);
+static int ln_by_type(int in_dtype, int out_dtype, bool wide, int d, int W, F&& f) {
+  if (in_dtype == KF_F32) return ln_by_out<float>(out_dtype, wide, d, W, f);
+  if (in_dtype == KF_BF16) return ln_by_out<__nv_bfloat16>(out_dtype, wide, d, W, f);
+  return ln_by_out<__half>(out_dtype, wide, d, W, f);
 }
 
 static bool ln_aligned(const void* p, int64_t pitch_bytes) { return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)pitch_bytes) & 15) == 0; }
@@ -451,7 +458,7 @@ extern "C" int64_t kf_layer_norm_ws_bytes(int64_t rows, int d) {
     return KF_ERR_BAD_ARGUMENT;
   }
   int grid = 0;
-  const int rc = ln_grid(rows, d, 0, 0, &grid);                  // no launch makes more lines
+  const int rc = ln_grid(rows, ln_warps(d, true), 0, 0, &grid);                  // no launch makes more lines
   if (rc != KF_OK) return rc > 0 ? KF_ERR_UNSUPPORTED : rc;
   return (int64_t)grid * 2 * d * 4;
 }
@@ -463,14 +470,14 @@ extern "C" int kf_layer_norm_fwd(int in_dtype, const void* x, int64_t ldx, const
   if (rows == 0) return KF_OK;
   KF_REQUIRE(x && w && y && mean && rstd, "kf_layer_norm_fwd: null pointer");
   LnArgs a{};
-  a.x = x; a.ldx = ldx; a.w = w; a.b = b; a.mean = mean; a.rstd = rstd; a.y = y; a.rows = rows; a.d = d; a.W = ln_warps(d); a.eps = eps; a.inv_d = 1.0f / (float)d;
+  a.x = x; a.ldx = ldx; a.w = w; a.b = b; a.mean = mean; a.rstd = rstd; a.y = y; a.rows = rows; a.d = d; a.W = ln_warps(d, false); a.eps = eps; a.inv_d = 1.0f / (float)d;
   a.slot_x = ln_slot(d, ln_size(in_dtype));
   a.err = dev_error_ptr();
   KF_REQUIRE(a.err != nullptr, "kf_layer_norm_fwd: device error word unavailable");
   const bool wide = d % 8 == 0 && ln_aligned(x, ldx * ln_size(in_dtype)) && ln_aligned(y, 0) && ln_aligned(w, 0) && ln_aligned(b, 0);
   const size_t smem = ln_smem_bytes(d, a.slot_x, false);
   int grid = 0;
-  return ln_by_type(in_dtype, out_dtype, wide, d, [&](auto ti, auto to, auto ch, auto nc) {
+  return ln_by_type(in_dtype, out_dtype, wide, d, a.W, [&](auto ti, auto to, auto ch, auto nc) {
     return ln_launch<layer_norm_fwd_kernel<decltype(ti), decltype(to), decltype(ch)::value, decltype(nc)::value>>("kf_layer_norm_fwd launch", rows, smem,
                      static_cast<cudaStream_t>(stream), a, -1, &grid);
   });
@@ -492,7 +499,7 @@ extern "C" int kf_layer_norm_bwd(int in_dtype, const void* x, int64_t ldx, int d
   KF_REQUIRE(x && dy && mean && rstd && dx && ws, "kf_layer_norm_bwd: null pointer");
   LnArgs a{};
   a.x = x; a.ldx = ldx; a.dy = dy; a.lddy = lddy; a.dres = dres; a.ldres = ldres; a.w = w; a.mean = const_cast<float*>(mean); a.rstd = const_cast<float*>(rstd);
-  a.dx = dx; a.part = static_cast<float*>(ws); a.rows = rows; a.d = d; a.W = ln_warps(d); a.inv_d = 1.0f / (float)d;
+  a.dx = dx; a.part = static_cast<float*>(ws); a.rows = rows; a.d = d; a.W = ln_warps(d, true); a.inv_d = 1.0f / (float)d;
   a.slot_x = ln_slot(d, ln_size(in_dtype));
   a.slot_y = ln_slot(d, ln_size(dy_dtype));
   a.slot_r = dres ? a.slot_x : 0;
@@ -502,7 +509,7 @@ extern "C" int kf_layer_norm_bwd(int in_dtype, const void* x, int64_t ldx, int d
   int grid = 0;
   const bool wide = d % 8 == 0 && ln_aligned(x, ldx * ln_size(in_dtype)) && ln_aligned(dy, lddy * ln_size(dy_dtype)) && ln_aligned(dres, ldres * ln_size(in_dtype)) &&
                     ln_aligned(dx, 0) && ln_aligned(w, 0);
-  const int rc = ln_by_type(in_dtype, dy_dtype, wide, d, [&](auto ti, auto to, auto ch, auto nc) {
+  const int rc = ln_by_type(in_dtype, dy_dtype, wide, d, a.W, [&](auto ti, auto to, auto ch, auto nc) {
     return ln_launch<layer_norm_bwd_kernel<decltype(ti), decltype(to), decltype(ch)::value, decltype(nc)::value>>("kf_layer_norm_bwd launch", rows, smem, st, a, ws_bytes, &grid);
   });
   if (rc != KF_OK) return rc;
