@@ -78,6 +78,40 @@ __device__ __forceinline__ float rcp_approx(float x) {
   return y;
 }
 
+// Capped scores in units of the exponent, cap * tanh(x * scale / cap) * log2(e) of raw products x.  Anywhere: tanh(y) = 1 - 2 / (1 + e^2y), two
+// operations of the special-function unit, absolute error ~1e-7 (tanh.approx would leave 2^-11, which the cap scales).  Where every score of a
+// piece lies within half the cap, which is what a cap leaves alone: x times a polynomial in x^2 (minimax for the relative error of
+// tanh(y) / y, |y| <= 0.5: 2.8e-8), six packed operations per pair.
+struct Cap {
+  float in, out;            // 2 * scale * log2(e) / cap, cap * log2(e)
+  float flat;               // raw products up to here in size take the polynomial
+  float inv_out;
+  float c[5];               // with scale and log2(e) in them
+  __host__ void set(float scale, float cap) {
+    constexpr double LOG2E = 1.4426950408889634;
+    const double a[5] = {0x1.0000000000000p+0, -0x1.5554a4p-2, 0x1.10e438p-3, -0x1.b20fdap-5, 0x1.18bd6ep-6}, r = (double)scale / cap;
+    in = (float)(2 * r * LOG2E);
+    out = (float)(cap * LOG2E);
+    inv_out = 1.f / out;
+    flat = (float)(0.5 / r < 1e18 ? 0.5 / r : 1e18);
+    double m = scale * LOG2E;
+    for (int i = 0; i < 5; ++i, m *= r * r) c[i] = (float)(a[i] * m);
+  }
+};
+__device__ __forceinline__ float2 cap_flat(const Cap& k, float2 x) {
+  const float2 t = mul2(x, x);
+  float2 p = fma2(t, splat2(k.c[4]), splat2(k.c[3]));
+  p = fma2(p, t, splat2(k.c[2]));
+  p = fma2(p, t, splat2(k.c[1]));
+  p = fma2(p, t, splat2(k.c[0]));
+  return mul2(x, p);
+}
+
+__device__ __forceinline__ float2 cap_any(const Cap& k, float2 x) {
+  const float2 r = make_float2(rcp_approx(1.f + ex2(x.x * k.in)), rcp_approx(1.f + ex2(x.y * k.in)));
+  return fma2(r, splat2(-2.f * k.out), splat2(k.out));
+}
+
 // ------------------------------------------------------------------------------------------------ packed batches
 // One 128-row tile of queries of one sequence (a record of eight 32-bit words, built by the host; see kf_attn_pack_params).  Query r of the
 // tile is at position pos + r of its keys and sees keys [0, limit(r)): all of them (prefix = k_len), or those up to itself and the prefix.

@@ -11,8 +11,10 @@
 //     possible: every role steps from item to item with its own cursor
 //   - a tile may reach behind the end of its sequence: the scores there are masked one by one, the rows of V are set to zero in shared
 //     memory by the warp that issues the products (P is 0 there, but 0 * NaN is not)
-//   - with a cap or slopes the scores are brought to the exponent's scale in registers before the maximum; tanh(y) = 1 - 2 / (1 + e^2y):
-//     absolute error ~1e-7, which the cap scales (tanh.approx would leave 2^-11)
+//   - with a cap or slopes the scores are brought to the exponent's scale in registers before the maximum
+//   - with slopes the key tiles start at the one where the first query stands, go up to the last and then down to the first: scores mostly
+//     fall with the distance, and a maximum that rises from tile to tile sends every tile down the slow path (200 queries behind 1605
+//     keys, slope 1/16: 49 us in the keys' order)
 //   - the polynomial exponential is a degree finer, for the log-sum-exp
 #include <type_traits>
 
@@ -41,7 +43,7 @@ struct PackFwdArgs {
   const int4* tiles;        // QTile records
   int n_tiles, Hq, share;   // share = query heads per key head
   float scale_log2;         // scale * log2(e)
-  float cap_in, cap_out;    // 2 * scale * log2(e) / cap, cap * log2(e)
+  Cap cap;
   const float* slopes;      // [Hq]
   int wide;                 // rows of O are 32-byte aligned
   unsigned int* err;
@@ -90,7 +92,7 @@ attn_pack_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   __syncthreads();
   tc_fence_after();
   pdl_wait();
-  const uint32_t tmem_base = *tmem_holder;
+  const uint32_t tmem_base = (uint32_t)uniform_int((int)*tmem_holder);
   const WaitCtx ctx{abort_flag, a.err};
   const bool bad_align = (smem_u32(smem) & 1023u) != 0;
   if (bad_align && threadIdx.x == 0 && atomicCAS(&a.err[0], 0u, 99u) == 0u) {
@@ -100,6 +102,9 @@ attn_pack_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   auto tile_of = [&](int it) { return load_tile<QTile>(a.tiles, item_of_cta(it) / a.Hq); };
   auto head_of = [&](int it) { return item_of_cta(it) % a.Hq; };
   auto key_tiles = [](const QTile& t) { return (t.limit(t.rows - 1) + PK_BN - 1) / PK_BN; };
+  // the order of an item's n key tiles: from tile `start` up, then from the one in front of it down
+  auto start_of = [](const QTile& t, int n) { return !BIAS || t.pos < 0 ? 0 : t.pos / PK_BN < n ? t.pos / PK_BN : n - 1; };
+  auto tile_at = [](int i, int start, int n) { return !BIAS ? i : start + i < n ? start + i : n - 1 - i; };
 
   if (warp >= 4) {
   setmaxnreg_dec<PK_REGS_LEAN>();
@@ -118,7 +123,7 @@ attn_pack_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     uint32_t qi = 0;                                                              // items with keys so far
     for (int it = 0; it < n_my && ok; ++it) {
       const QTile t = tile_of(it);
-      const int n_kt = key_tiles(t), h = head_of(it), hk = h / a.share;
+      const int n_kt = key_tiles(t), h = head_of(it), hk = h / a.share, start = start_of(t, n_kt);
       if (n_kt == 0) continue;
       const uint32_t qb = qi & 1;
       if (!mbar_wait_warp(&q_empty[qb], ((qi >> 1) & 1) ^ 1, ctx, 40)) break;
@@ -128,17 +133,18 @@ attn_pack_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       }
       __syncwarp();
       ++qi;
-      for (int j = 0; j < n_kt; ++j) {
+      for (int i = 0; i < n_kt; ++i) {
+        const int key = t.k_row + tile_at(i, start, n_kt) * PK_BN;
         if (!mbar_wait_warp(&k_empty[st], ph, ctx, 41)) { ok = false; break; }
         if (elect_one()) {
           mbar_expect_tx(&k_full[st], PK_KTILE);
-          tma_load_3d(smem + PK_OFF_K + st * PK_KTILE, &tmK, 0, hk, t.k_row + j * PK_BN, &k_full[st]);
+          tma_load_3d(smem + PK_OFF_K + st * PK_KTILE, &tmK, 0, hk, key, &k_full[st]);
         }
         __syncwarp();
         if (!mbar_wait_warp(&v_empty[st], ph, ctx, 42)) { ok = false; break; }
         if (elect_one()) {
           mbar_expect_tx(&v_full[st], PK_KTILE);
-          tma_load_3d(smem + PK_OFF_V + st * PK_KTILE, &tmV, 0, hk, t.k_row + j * PK_BN, &v_full[st]);
+          tma_load_3d(smem + PK_OFF_V + st * PK_KTILE, &tmV, 0, hk, key, &v_full[st]);
         }
         __syncwarp();
         if (++st == PK_KV) {
@@ -154,25 +160,33 @@ attn_pack_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     const uint32_t t_o = tmem_base + PK_COL_O;
     const bool leader = elect_one();
     struct Cursor {                                                          // a key tile of an item; items without keys are stepped over
-      int it, j, n, k_len;
+      int it, next_n, next_len, next_start;                                  // the item behind this one: asked for ahead
+      int j, n, k_len, start;                                                // n = -1: no item left
     };
-    auto settle = [&](Cursor& c) {                                           // c.it: the first item at or behind it that has keys
-      for (; c.it < n_my; ++c.it) {
-        const QTile t = tile_of(c.it);
-        c.j = 0;
-        c.n = key_tiles(t);
-        c.k_len = t.k_len;
-        if (c.n > 0) return;
+    auto fetch = [&](Cursor& c) {
+      c.next_n = -1;
+      if (c.it < n_my) {
+        const QTile t = tile_of(c.it++);
+        c.next_n = key_tiles(t);
+        c.next_len = t.k_len;
+        c.next_start = start_of(t, c.next_n);
       }
+    };
+    auto open = [&](Cursor& c) {
+      do {
+        c.n = uniform_int(c.next_n);
+        c.k_len = uniform_int(c.next_len);
+        if (BIAS) c.start = uniform_int(c.next_start);
+        fetch(c);
+      } while (c.n == 0);
+      c.j = 0;
     };
     auto advance = [&](Cursor& c) {
-      if (++c.j == c.n) {
-        ++c.it;
-        settle(c);
-      }
+      if (++c.j == c.n) open(c);
     };
-    Cursor s{0, 0, 0, 0};                                                    // the next S product
-    settle(s);
+    Cursor s{};                                                              // the next S product
+    fetch(s);
+    open(s);
     Cursor v = s;                                                            // the next PV product
     uint32_t s_qi = 0, k_st = 0, k_ph = 0;
     auto issue_s = [&](uint32_t buf) {
@@ -196,16 +210,16 @@ attn_pack_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       }
     };
     bool ok = true;
-    for (uint32_t G = 0; G < PK_SBUF && s.it < n_my && ok; ++G) {
+    for (uint32_t G = 0; G < PK_SBUF && s.n > 0 && ok; ++G) {
       ok = (s.j != 0 || mbar_wait_warp(&q_full[s_qi & 1], (s_qi >> 1) & 1, ctx, 43)) && mbar_wait_warp(&k_full[k_st], k_ph, ctx, 44);
       tc_fence_after();
       if (ok) issue_s(G);
     }
     uint32_t buf = 0, pph = 0, st = 0, vph = 0;
-    while (v.it < n_my && ok) {
-      const bool more = s.it < n_my;
+    while (v.n > 0 && ok) {
+      const bool more = s.n > 0;
       if (more && s.j == 0 && !mbar_wait_warp(&q_full[s_qi & 1], (s_qi >> 1) & 1, ctx, 43)) break;
-      const int valid = v.k_len - v.j * PK_BN;                               // rows of this V tile that belong to the sequence
+      const int valid = v.k_len - tile_at(v.j, v.start, v.n) * PK_BN;                               // rows of this V tile that belong to the sequence
       if (valid < PK_BN) {
         if (!mbar_wait_warp(&v_full[st], vph, ctx, 45)) break;
         zero_rows(smem + PK_OFF_V + st * PK_KTILE, valid, PK_BN, lane);
@@ -218,10 +232,11 @@ attn_pack_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       tc_fence_after();
       const uint32_t t_p = tmem_base + buf * PK_BN;
       const uint64_t vdesc = smem_desc_sw128(smem_u32(smem + PK_OFF_V + st * PK_KTILE));
+      const uint32_t add = v.j != 0;
       if (leader) {
 #pragma unroll
         for (int kk = 0; kk < PK_BN / 16; ++kk)
-          mma_f16_ta(t_o, t_p + 8 * kk, vdesc + (uint64_t)(kk * (2048 >> 4)), idesc_o, (v.j | kk) != 0);
+          mma_f16_ta(t_o, t_p + 8 * kk, vdesc + (uint64_t)(kk * (2048 >> 4)), idesc_o, kk ? 1u : add);
         tc_commit(&o_full[buf]);
         tc_commit(&v_empty[st]);
       }
@@ -283,11 +298,13 @@ attn_pack_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     // little of the record lives through the key loop: where the rows go is looked up again behind it
     int n_kt, lim, warp_lim;                                     // lim: keys this row sees (-1: no row); warp_lim: the fewest of the warp's rows that exist
     float slope = 0.f, at = 0.f;
+    int start;
     {
       const QTile tile = tile_of(it);
       n_kt = key_tiles(tile);
       lim = row < tile.rows ? tile.limit(row) : -1;
       warp_lim = tile.limit(warp * 32);
+      start = start_of(tile, n_kt);
       if constexpr (BIAS) {
         slope = __ldg(a.slopes + head_of(it)) * 1.4426950408889634f;
         at = (float)(tile.pos + row);
@@ -297,22 +314,31 @@ attn_pack_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     auto logits = [&](uint32_t (&r)[32], int key0) {
       if constexpr (!RAW) {
         const float gap = at - (float)key0;
+        bool flat = false;
+        if constexpr (CAP) {
+          float m4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          float2 x = make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1]));
-          if constexpr (CAP) {
-            const float2 rc = make_float2(rcp_approx(1.f + ex2(x.x * a.cap_in)), rcp_approx(1.f + ex2(x.y * a.cap_in)));
-            x = fma2(rc, splat2(-2.f * a.cap_out), splat2(a.cap_out));
-          } else {
-            x = mul2(x, splat2(a.scale_log2));
-          }
-          if constexpr (BIAS) {
-            x.x = fmaf(-slope, fabsf(gap - (float)i), x.x);
-            x.y = fmaf(-slope, fabsf(gap - (float)(i + 1)), x.y);
-          }
-          r[i] = __float_as_uint(x.x);
-          r[i + 1] = __float_as_uint(x.y);
+          for (int i = 0; i < 16; ++i) m4[i & 3] = max3(m4[i & 3], fabsf(__uint_as_float(r[2 * i])), fabsf(__uint_as_float(r[2 * i + 1])));
+          flat = __all_sync(0xffffffffu, amax_nan(amax_nan(m4[0], m4[1]), amax_nan(m4[2], m4[3])) <= a.cap.flat);
         }
+        auto each = [&](auto kind) {                             // 0: no cap, 1: small scores, 2: any
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            float2 x = make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1]));
+            if constexpr (decltype(kind)::value == 0) x = mul2(x, splat2(a.scale_log2));
+            else if constexpr (decltype(kind)::value == 1) x = cap_flat(a.cap, x);
+            else x = cap_any(a.cap, x);
+            if constexpr (BIAS) {
+              x.x = fmaf(-slope, fabsf(gap - (float)i), x.x);
+              x.y = fmaf(-slope, fabsf(gap - (float)(i + 1)), x.y);
+            }
+            r[i] = __float_as_uint(x.x);
+            r[i + 1] = __float_as_uint(x.y);
+          }
+        };
+        if constexpr (!CAP) each(std::integral_constant<int, 0>{});
+        else if (flat) each(std::integral_constant<int, 1>{});
+        else each(std::integral_constant<int, 2>{});
       }
       if (key0 + 32 > warp_lim) {
 #pragma unroll
@@ -337,7 +363,7 @@ attn_pack_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         sph ^= 1;
       }
       const bool prefetch = j + 1 < n_kt;
-      const int kbase = j * PK_BN;
+      const int kbase = tile_at(j, start, n_kt) * PK_BN;
       tmem_ld_wait();
       tmem_ld_fence(ra);
       tmem_ld_fence(rb);
@@ -347,9 +373,10 @@ attn_pack_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       logits(rc, kbase + 64);
       if (j == 0) {
         m_run = row_max(rb, row_max(ra, -INFINITY));
-        if (m_run == -INFINITY) m_run = 0.f;                     // a row that sees nothing
+        if (!BIAS && m_run == -INFINITY) m_run = 0.f;            // a row that sees nothing
       }
-      const float2 mn2 = splat2(-m_run * sc);
+      const bool unseen = BIAS && m_run == -INFINITY;            // none of its keys so far
+      const float2 mn2 = splat2(unseen ? 0.f : -m_run * sc);
       float2 s0 = make_float2(0.f, 0.f), s1 = s0;
       uint32_t w[48];
       exp_half(ra, w, mn2, s0, s1);
@@ -364,7 +391,7 @@ attn_pack_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       exp_half(rc, w + 32, mn2, s0, s1);
       if (prefetch) tmem_ld32(t_lane + buf * PK_BN + 64, rc);
       float sum = (s0.x + s0.y) + (s1.x + s1.y), alpha = 1.f;
-      const bool need = lim >= 0 && !(sum <= PK_SUM_LIMIT);   // rows that are not stored go on with whatever they have
+      const bool need = lim >= 0 && (!(sum <= PK_SUM_LIMIT) || (unseen && lim > 0));   // rows that are not stored go on with whatever they have
       if (__any_sync(0xffffffffu, need)) {
         uint32_t r[32];
         float mx = m_run;
@@ -376,10 +403,11 @@ attn_pack_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
           logits(r, kbase + 32 * c);
           mx = row_max(r, mx);
         }
-        if (need) {
+        if (need && !(BIAS && mx == -INFINITY)) {
           alpha = ex2((m_run - mx) * sc);
           m_run = mx;
         }
+        const float2 mn = splat2(BIAS && m_run == -INFINITY ? 0.f : -m_run * sc);
         s0 = s1 = make_float2(0.f, 0.f);
 #pragma unroll 1
         for (int c = 0; c < PK_BN / 32; ++c) {
@@ -387,9 +415,9 @@ attn_pack_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
           tmem_ld_wait();
           tmem_ld_fence(r);
           logits(r, kbase + 32 * c);
-          if (c == 0) exp_half(r, w, splat2(-m_run * sc), s0, s1);
-          else if (c == 1) exp_half(r, w + 16, splat2(-m_run * sc), s0, s1);
-          else exp_half(r, w + 32, splat2(-m_run * sc), s0, s1);
+          if (c == 0) exp_half(r, w, mn, s0, s1);
+          else if (c == 1) exp_half(r, w + 16, mn, s0, s1);
+          else exp_half(r, w + 32, mn, s0, s1);
         }
         sum = (s0.x + s0.y) + (s1.x + s1.y);
         if (j > 0) {                                             // rescale O: PV(G - 1) must have landed first
@@ -567,10 +595,7 @@ extern "C" int kf_attn_pack_fwd(const kf_attn_pack_params* p, void* stream) {
   a.O = o.ptr; a.o_st = o.row_stride; a.o_sh = o.head_stride; a.lse = p->lse; a.lse_ld = p->Tq;
   a.tiles = reinterpret_cast<const int4*>(p->q_tiles); a.n_tiles = p->n_q_tiles; a.Hq = p->Hq; a.share = p->Hq / p->Hk;
   a.scale_log2 = p->scale * LOG2E;
-  if (c) {
-    a.cap_in = 2.f * p->scale * LOG2E / p->cap;
-    a.cap_out = p->cap * LOG2E;
-  }
+  if (c) a.cap.set(p->scale, p->cap);
   a.slopes = p->slopes;
   a.wide = ((reinterpret_cast<uintptr_t>(o.ptr) | (uintptr_t)(o.row_stride * 2) | (uintptr_t)(o.head_stride * 2)) & 31) == 0;
   a.err = dev_error_ptr();

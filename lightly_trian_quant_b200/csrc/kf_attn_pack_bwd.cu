@@ -41,12 +41,13 @@ struct BwdMem {
 };
 constexpr int PB_COL_S = 0, PB_COL_D = 2 * PB_W, PB_COL_A1 = 4 * PB_W, PB_COL_A2 = PB_COL_A1 + PB_D, PB_TMEM_COLS = 512;
 static_assert(PB_COL_A2 + PB_D <= PB_TMEM_COLS, "TMEM budget");
-constexpr int PB_POLY = 0x88, PB_POLY_CAP = 0xaa;               // which of eight element pairs take the polynomial exponential
+constexpr int PB_POLY = 0x88, PB_POLY_KEYS = 0x80;              // which of eight element pairs take the polynomial exponential
 
 struct PackBwdArgs {
   const int4* tiles;
   int n_items, heads, share;     // heads of an item: query heads (ROWS = queries) or key heads
-  float scale, scale_log2, cap_in, cap_out;
+  float scale, scale_log2;
+  Cap cap;
   const float* slopes;
   float *lse2, *delta;           // -lse * log2(e) (-inf: no row, or one that sees nothing) and -delta: [Hq][n_q_tiles * 128], a sequence's rows from its first tile's slot on
   int64_t stat_ld;
@@ -427,40 +428,49 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
         const float* stat = reinterpret_cast<const float*>(smem + PB_OFF_STAT + st * 1024) + c0;
         if (KEYS && !mbar_wait_warp(&st_full[st], st_ph, ctx, 71)) { ok = false; break; }
         const float gap = at - (float)index;
+        bool flat = false;
+        if constexpr (CAP) {
+          float m4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < COLS; i += 8) {
-          uint32_t f[8];                                         // with a cap: 1 - tanh^2 = 4 r (1 - r), r = 1 / (1 + e^2y)
-          float v[8];
-          if (KEYS) {
-            *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(stat + i);
-            *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(stat + i + 4);
-          }
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int c = i + 2 * k;
-            float2 l = KEYS ? make_float2(v[2 * k], v[2 * k + 1]) : splat2(nlse2);
-            float2 x = make_float2(__uint_as_float(p[c / 16][c % 16]), __uint_as_float(p[c / 16][c % 16 + 1]));
-            if constexpr (CAP) {
-              const float2 r = make_float2(rcp_approx(1.f + ex2(x.x * a.cap_in)), rcp_approx(1.f + ex2(x.y * a.cap_in)));
-              const float2 r4 = mul2(r, splat2(4.f));
-              const float2 d = fma2(make_float2(-r4.x, -r4.y), r, r4);
-              f[2 * k] = __float_as_uint(d.x);
-              f[2 * k + 1] = __float_as_uint(d.y);
-              x = fma2(r, splat2(-2.f * a.cap_out), splat2(a.cap_out));
-            } else if constexpr (BIAS) {
-              x = mul2(x, splat2(a.scale_log2));
-            }
-            if constexpr (BIAS) {
-              l.x = fmaf(-slope, fabsf(gap - (float)c), l.x);
-              l.y = fmaf(-slope, fabsf(gap - (float)(c + 1)), l.y);
-            }
-            x = CAP || BIAS ? add2(x, l) : fma2(x, splat2(a.scale_log2), l);
-            x = ((CAP ? PB_POLY_CAP : PB_POLY) >> ((i / 2 + k) % 8)) & 1 ? ex2_poly2_neg(x) : make_float2(ex2(x.x), ex2(x.y));
-            p[c / 16][c % 16] = __float_as_uint(x.x);
-            p[c / 16][c % 16 + 1] = __float_as_uint(x.y);
-          }
-          if constexpr (CAP) tmem_st8(t_s + i, f);               // over S, for the other half of the step
+          for (int i = 0; i < COLS; i += 2) m4[(i / 2) & 3] = max3(m4[(i / 2) & 3], fabsf(__uint_as_float(p[i / 16][i % 16])), fabsf(__uint_as_float(p[i / 16][i % 16 + 1])));
+          flat = __all_sync(0xffffffffu, amax_nan(amax_nan(m4[0], m4[1]), amax_nan(m4[2], m4[3])) <= a.cap.flat);
         }
+        auto exponentials = [&](auto small) {                    // with a cap: every score is small
+#pragma unroll
+          for (int i = 0; i < COLS; i += 8) {
+            uint32_t f[8];                                         // with a cap: 1 - tanh^2
+            float v[8];
+            if (KEYS) {
+              *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(stat + i);
+              *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(stat + i + 4);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int c = i + 2 * k;
+              float2 l = KEYS ? make_float2(v[2 * k], v[2 * k + 1]) : splat2(nlse2);
+              float2 x = make_float2(__uint_as_float(p[c / 16][c % 16]), __uint_as_float(p[c / 16][c % 16 + 1]));
+              if constexpr (CAP) {
+                x = decltype(small)::value ? cap_flat(a.cap, x) : cap_any(a.cap, x);
+                const float2 y = mul2(x, splat2(a.cap.inv_out)), d = fma2(make_float2(-y.x, -y.y), y, splat2(1.f));
+                f[2 * k] = __float_as_uint(d.x);
+                f[2 * k + 1] = __float_as_uint(d.y);
+              } else if constexpr (BIAS) {
+                x = mul2(x, splat2(a.scale_log2));
+              }
+              if constexpr (BIAS) {
+                l.x = fmaf(-slope, fabsf(gap - (float)c), l.x);
+                l.y = fmaf(-slope, fabsf(gap - (float)(c + 1)), l.y);
+              }
+              x = CAP || BIAS ? add2(x, l) : fma2(x, splat2(a.scale_log2), l);
+              x = ((KEYS ? PB_POLY_KEYS : PB_POLY) >> ((i / 2 + k) % 8)) & 1 ? ex2_poly2_neg(x) : make_float2(ex2(x.x), ex2(x.y));
+              p[c / 16][c % 16] = __float_as_uint(x.x);
+              p[c / 16][c % 16 + 1] = __float_as_uint(x.y);
+            }
+            if constexpr (CAP) tmem_st8(t_s + i, f);               // over S, for the other half of the step
+          }
+        };
+        if (CAP && flat) exponentials(std::true_type{});
+        else exponentials(std::false_type{});
         if constexpr (CAP) tmem_st_wait();
         // the columns that the row sees (operands behind the end of a sequence are zero, so that P = 0 is enough)
         if (KEYS ? index < warp_edge || end - index < COLS : index + COLS > warp_edge) {
@@ -645,10 +655,7 @@ extern "C" int kf_attn_pack_bwd(const kf_attn_pack_params* p, void* stream) {
   a.share = p->Hq / p->Hk;
   a.scale = p->scale;
   a.scale_log2 = p->scale * LOG2E;
-  if (c) {
-    a.cap_in = 2.f * p->scale * LOG2E / p->cap;
-    a.cap_out = p->cap * LOG2E;
-  }
+  if (c) a.cap.set(p->scale, p->cap);
   a.slopes = p->slopes;
   a.stat_ld = (int64_t)p->n_q_tiles * PB_T;
   a.lse2 = static_cast<float*>(p->ws);
