@@ -338,12 +338,12 @@ typedef struct kf_attn_pack_params {
   float* lse;              /* fp32 [Hq, Tq]: written by the forward, read by the gradient              */
   kf_heads q, k, v, o;     /* o: written by the forward, read by the gradient                          */
   kf_heads dout, dq, dk, dv; /* gradient only                                                          */
-  void* ws;                /* gradient only: kf_attn_pack_ws_bytes bytes                               */
+  void* ws;                /* gradient only: kf_attn_pack_ws_bytes bytes, 32-byte aligned              */
   int64_t ws_bytes;
 } kf_attn_pack_params;
 KF_API int kf_attn_pack_fwd(const kf_attn_pack_params* p, void* stream);
 /* dq, dk, dv from dout and what the forward read and wrote (the same tables, scale, cap and slopes; slopes have no gradient).  No atomics. */
-KF_API int64_t kf_attn_pack_ws_bytes(int Hq, int n_q_tiles);
+KF_API int64_t kf_attn_pack_ws_bytes(int Hq, int Hk, int n_q_tiles, int n_k_tiles); /* for the current device */
 KF_API int kf_attn_pack_bwd(const kf_attn_pack_params* p, void* stream);
 
 #ifdef __cplusplus

@@ -78,7 +78,7 @@ def lib() -> C.CDLL:
         L.kf_sf_bytes.argtypes = [C.c_int64, C.c_int64, C.c_int]
         vp, i32, i64, f32 = C.c_void_p, C.c_int, C.c_int64, C.c_float
         L.kf_attn_pack_ws_bytes.restype = i64
-        L.kf_attn_pack_ws_bytes.argtypes = [i32, i32]
+        L.kf_attn_pack_ws_bytes.argtypes = [i32, i32, i32, i32]
         L.kf_layer_norm_ws_bytes.restype = i64
         L.kf_layer_norm_ws_bytes.argtypes = [i64, i32]
         sigs = {

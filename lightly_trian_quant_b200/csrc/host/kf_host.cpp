@@ -918,7 +918,8 @@ PyObject* attn_packed_bwd(PyObject* const* v) {
   c.p.dq = pack_heads(g[0]);
   c.p.dk = pack_heads(g[1]);
   c.p.dv = pack_heads(g[2]);
-  c.p.ws_bytes = kf_attn_pack_ws_bytes(c.p.Hq, c.p.n_q_tiles);
+  c.p.ws_bytes = kf_attn_pack_ws_bytes(c.p.Hq, c.p.Hk, c.p.n_q_tiles, c.p.n_k_tiles);
+  if (c.p.ws_bytes < 0) check((int)c.p.ws_bytes, "kf_attn_pack_ws_bytes");
   at::Tensor ws = empty({c.p.ws_bytes / 4}, at::kFloat, c.q.device());
   c.p.ws = ws.data_ptr();
   launch(op, kf_attn_pack_bwd, (const kf_attn_pack_params*)&c.p, stream());

@@ -45,7 +45,9 @@ constexpr int PB_POLY = 0x88, PB_POLY_KEYS = 0x80;              // which of eigh
 
 struct PackBwdArgs {
   const int4* tiles;
-  int n_items, heads, share;     // heads of an item: query heads (ROWS = queries) or key heads
+  int n_items, heads, share;     // heads of the items: query heads (ROWS = queries), key heads times `split`
+  int split;                     // ROWS = keys: items per key head: 1, or the query heads that share it; their sums are then joined by bwd_join_kernel
+  float* parts;                  // [n_items][2][128][64] of a split
   float scale, scale_log2;
   Cap cap;
   const float* slopes;
@@ -86,14 +88,16 @@ struct BwdItem<false> {
 template <>
 struct BwdItem<true> {
   KTile t;
-  int head, n, per, first;                                      // per: passing tiles per query head, from tile `first` of the sequence on
+  int head, n, per, first, q_head;                              // per: passing tiles per query head, from tile `first` of the sequence on; q_head: the first one
   __device__ __forceinline__ void load(const PackBwdArgs& a, int item) {
     t = load_tile<KTile>(a.tiles, item / a.heads);
-    head = item % a.heads;
+    const int h = item % a.heads, each = a.share / a.split;     // query heads of an item
+    head = h / a.split;
+    q_head = h * each;
     first = t.lowest(0) / PB_W;
     const int tiles = (t.q_len + PB_W - 1) / PB_W;
     per = tiles > first ? tiles - first : 0;
-    n = per * a.share;
+    n = per * each;
   }
   __device__ __forceinline__ int rows() const { return t.rows; }
   __device__ __forceinline__ int row0() const { return t.row; }
@@ -108,7 +112,7 @@ __device__ __forceinline__ BwdStep step_of(const PackBwdArgs& a, const BwdItem<f
 }
 __device__ __forceinline__ BwdStep step_of(const PackBwdArgs& a, const BwdItem<true>& i, int j) {
   const int hh = j / i.per, qt = i.first + j - hh * i.per;
-  return {i.t.q_row + qt * PB_W, i.head * a.share + hh, qt * PB_W, i.t.q_len - qt * PB_W};
+  return {i.t.q_row + qt * PB_W, i.q_head + hh, qt * PB_W, i.t.q_len - qt * PB_W};
 }
 
 template <int F16, bool KEYS, bool CAP, bool BIAS>
@@ -396,7 +400,7 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
       if constexpr (KEYS) {
         index += I.first * PB_W;
         end = I.t.q_len;
-        head = I.head * a.share;
+        head = I.q_head;
         per_rows = I.per * PB_W;
       }
       const int start = index;
@@ -544,6 +548,11 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
 #pragma unroll
           for (int k = 0; k < 32; ++k) r[k] = 0u;
         }
+        if (KEYS && a.split > 1) {                               // the item's sums as they are
+          float* to = a.parts + (((int64_t)item_of_cta(it) * 2 + half) * PB_T + row) * PB_D + 32 * i;
+#pragma unroll
+          for (int k = 0; k < 32; k += 8) stg8w(to + k, r + k);
+        }
 #pragma unroll
         for (int k = 0; k < 16; ++k) w[i][k] = pack16(__uint_as_float(r[2 * k]) * scale, __uint_as_float(r[2 * k + 1]) * scale, F16);
       }
@@ -551,6 +560,7 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
         tc_fence_before();
         mbar_arrive(acc_free);
       }
+      if (KEYS && a.split > 1) continue;
       if (row < I.rows()) {
         const int64_t r = I.row0() + row;
         uint8_t* dst = KEYS && half ? static_cast<uint8_t*>(a.g2) + 2 * (r * a.g2_st + (int64_t)I.head * a.g2_sh)
@@ -580,6 +590,39 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
     tmem_dealloc(tmem_base, PB_TMEM_COLS);
   }
 }
+
+// dK and dV of a key tile and head: the sums of the query heads that share it, in their order.  A CTA per (tile, key head).
+template <int F16>
+__global__ void __launch_bounds__(256) bwd_join_kernel(const __grid_constant__ PackBwdArgs a) {
+  pdl_wait();
+  const int heads = a.heads / a.split, head = blockIdx.x % heads;
+  const KTile t = load_tile<KTile>(a.tiles, blockIdx.x / heads);
+  const float* from = a.parts + (int64_t)blockIdx.x * a.split * 2 * PB_T * PB_D;
+  for (int i = threadIdx.x; i < 2 * PB_T * (PB_D / 8); i += 256) {
+    const int which = i / (PB_T * (PB_D / 8)), rest = i - which * PB_T * (PB_D / 8), row = rest / (PB_D / 8), c = rest % (PB_D / 8) * 8;
+    if (row >= t.rows) continue;
+    const float* p = from + (which * PB_T + row) * PB_D + c;
+    float s[8] = {};
+    for (int k = 0; k < a.split; ++k, p += 2 * PB_T * PB_D) {
+      const float4 u = __ldg(reinterpret_cast<const float4*>(p)), v = __ldg(reinterpret_cast<const float4*>(p) + 1);
+      s[0] += u.x; s[1] += u.y; s[2] += u.z; s[3] += u.w;
+      s[4] += v.x; s[5] += v.y; s[6] += v.z; s[7] += v.w;
+    }
+    const float f = which ? 1.f : a.scale;
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = pack16(s[2 * k] * f, s[2 * k + 1] * f, F16);
+    const int64_t r = t.row + row;
+    uint8_t* dst = which ? static_cast<uint8_t*>(a.g2) + 2 * (r * a.g2_st + (int64_t)head * a.g2_sh + c) : static_cast<uint8_t*>(a.g1) + 2 * (r * a.g1_st + (int64_t)head * a.g1_sh + c);
+    *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// Items per key head in the second launch.  A key head that several query heads share makes an item of that many times the steps; where there are few
+// items, an item per query head fills the device evenly, at the price of fp32 sums through memory (10 sequences of 1 to 2053 tokens, 12 heads
+// on 4: 240 items, the longest with 66 steps where 37 are the mean).
+static int bwd_split(int Hq, int Hk, int n_k_tiles, int sms) { return (int64_t)n_k_tiles * Hk < 4ll * sms ? Hq / Hk : 1; }
+static int64_t bwd_stat_bytes(int Hq, int n_q_tiles) { return 2 * ((int64_t)Hq * n_q_tiles + 1) * PB_T * 4; }      // the last passing tile may reach behind the last row
 
 using BwdFn = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, PackBwdArgs);
 template <int F16, bool KEYS>
@@ -612,12 +655,16 @@ static int bwd_ready(BwdFn kern, int which, size_t smem) {
 
 using namespace kf;
 
-extern "C" int64_t kf_attn_pack_ws_bytes(int Hq, int n_q_tiles) {
-  if (Hq <= 0 || n_q_tiles < 0) {
-    set_error("kf_attn_pack_ws_bytes: bad argument Hq=%d n_q_tiles=%d", Hq, n_q_tiles);
+extern "C" int64_t kf_attn_pack_ws_bytes(int Hq, int Hk, int n_q_tiles, int n_k_tiles) {
+  if (Hq <= 0 || Hk <= 0 || Hq % Hk || n_q_tiles < 0 || n_k_tiles < 0) {
+    set_error("kf_attn_pack_ws_bytes: bad argument Hq=%d Hk=%d n_q_tiles=%d n_k_tiles=%d", Hq, Hk, n_q_tiles, n_k_tiles);
     return KF_ERR_BAD_ARGUMENT;
   }
-  return 2 * ((int64_t)Hq * n_q_tiles + 1) * PB_T * 4;         // the last passing tile may reach behind the last row
+  int sms = 0;
+  const int rc = device_sm_count(&sms);
+  if (rc != KF_OK) return rc > 0 ? KF_ERR_UNSUPPORTED : rc;
+  const int64_t split = bwd_split(Hq, Hk, n_k_tiles, sms);
+  return bwd_stat_bytes(Hq, n_q_tiles) + (split > 1 ? split * n_k_tiles * Hk * 2 * PB_T * PB_D * 4 : 0);
 }
 
 extern "C" int kf_attn_pack_bwd(const kf_attn_pack_params* p, void* stream) {
@@ -640,8 +687,10 @@ extern "C" int kf_attn_pack_bwd(const kf_attn_pack_params* p, void* stream) {
     if ((rc = check_heads("dk", p->dk, p->Tk, p->Hk, &gk)) != KF_OK) return rc;
     if ((rc = check_heads("dv", p->dv, p->Tk, p->Hk, &gv)) != KF_OK) return rc;
   }
-  KF_REQUIRE(p->ws && (reinterpret_cast<uintptr_t>(p->ws) & 15) == 0 && p->ws_bytes >= kf_attn_pack_ws_bytes(p->Hq, p->n_q_tiles),
-             "kf_attn_pack_bwd: workspace of %lld bytes, needs %lld, 16-byte aligned", (long long)p->ws_bytes, (long long)kf_attn_pack_ws_bytes(p->Hq, p->n_q_tiles));
+  const int64_t need = kf_attn_pack_ws_bytes(p->Hq, p->Hk, p->n_q_tiles, p->n_k_tiles);
+  if (need < 0) return (int)need;
+  KF_REQUIRE(p->ws && (reinterpret_cast<uintptr_t>(p->ws) & 31) == 0 && p->ws_bytes >= need, "kf_attn_pack_bwd: workspace of %lld bytes, needs %lld, 32-byte aligned",
+             (long long)p->ws_bytes, (long long)need);
   CUtensorMap r1, r2, r3, c1, c2;
   // (a side stays in boxes of 128 rows in one launch and passes in boxes of 96 in the other)
   auto maps = [&](const kf_heads& x, const kf_heads& y, int64_t rows, int heads, int box, CUtensorMap* mx, CUtensorMap* my) {
@@ -653,6 +702,7 @@ extern "C" int kf_attn_pack_bwd(const kf_attn_pack_params* p, void* stream) {
   const bool f = p->dtype == KF_F16, c = p->cap > 0.f, b = p->slopes != nullptr;
   PackBwdArgs a{};
   a.share = p->Hq / p->Hk;
+  a.split = 1;
   a.scale = p->scale;
   a.scale_log2 = p->scale * LOG2E;
   if (c) a.cap.set(p->scale, p->cap);
@@ -685,8 +735,10 @@ extern "C" int kf_attn_pack_bwd(const kf_attn_pack_params* p, void* stream) {
   }
   if (any_k) {
     a.tiles = reinterpret_cast<const int4*>(p->k_tiles);
-    a.heads = p->Hk;
-    a.n_items = p->n_k_tiles * p->Hk;
+    a.split = bwd_split(p->Hq, p->Hk, p->n_k_tiles, sms);
+    a.heads = p->Hk * a.split;
+    a.n_items = p->n_k_tiles * a.heads;
+    a.parts = static_cast<float*>(p->ws) + bwd_stat_bytes(p->Hq, p->n_q_tiles) / 4;
     a.g1 = gk.ptr; a.g1_st = gk.row_stride; a.g1_sh = gk.head_stride;
     a.g2 = gv.ptr; a.g2_st = gv.row_stride; a.g2_sh = gv.head_stride;
     a.wide = wide_rows(gk) && wide_rows(gv);
@@ -701,6 +753,10 @@ extern "C" int kf_attn_pack_bwd(const kf_attn_pack_params* p, void* stream) {
     if ((rc = bwd_ready(kern, f * 8 + 4 + c * 2 + b, BwdMem<true>::BYTES)) != KF_OK) return rc;
     const cudaError_t e = launch_maybe_pdl(p->Tk, kern, dim3(a.n_items < sms ? a.n_items : sms), dim3(PB_THREADS), BwdMem<true>::BYTES, st, r1, r2, r1, c1, c2, a);
     if (e != cudaSuccess) return cuda_status(e, "kf_attn_pack_bwd launch (keys)");
+    if (a.split > 1) {
+      const cudaError_t j = launch_maybe_pdl(p->Tk, f ? bwd_join_kernel<1> : bwd_join_kernel<0>, dim3(p->n_k_tiles * p->Hk), dim3(256), 0, st, a);
+      if (j != cudaSuccess) return cuda_status(j, "kf_attn_pack_bwd launch (join)");
+    }
   }
   return KF_OK;
 }

@@ -318,6 +318,33 @@ def test_the_same_bits_from_run_to_run_in_graphs_and_on_other_streams():
 
 
 @gpu
+def test_workspace_is_checked_by_the_call():
+    from lightly_trian_quant_b200 import _lib
+
+    L, p = _lib.lib(), _lib.AttnPackParams()
+    p.dtype, p.Hq, p.Hk, p.n_q_tiles, p.n_k_tiles, p.scale, p.Tq, p.Tk = 1, 4, 2, 1, 1, 0.125, 40, 40
+    p.q_tiles = p.k_tiles = p.lse = p.ws = 4096                     # never dereferenced: the calls end on the host
+    for n in ("q", "k", "v", "o", "dout", "dq", "dk", "dv"):
+        setattr(p, n, _lib.Heads(4096, 256, 64))
+    need = L.kf_attn_pack_ws_bytes(4, 2, 1, 1)
+    assert need >= 2 * 4 * 128 * 4
+    for size, at in ((need - 1, 4096), (need, None), (need, 4112)):
+        p.ws_bytes, p.ws = size, at
+        assert L.kf_attn_pack_bwd(p, None) == -1 and "workspace" in L.kf_last_error_string().decode()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("heads", [(3, 1), (8, 2), (2, 2)])
+def test_shared_key_heads_with_few_and_many_items(heads, dtype):
+    """an item per query head and their sums joined (few tiles), an item per key head (many tiles): both against the same reference"""
+    ops = _ops()
+    for lens in ([200, 37], [130] * 160):
+        q, k, v, do = case(lens, lens, *heads, dtype, 77)
+        close(run(q, k, v, do, ops.AttnPlan(lens, causal=True)), reference(q, k, v, do, lens, lens, True, None, 0.125, 0.0, None, dtype), NAMES)
+
+
+@gpu
 def test_refusals():
     ops = _ops()
     q, k, v, do = case([40], [40], 4, 2, BF, 1)
@@ -408,10 +435,9 @@ def test_host_checks_of_the_packed_attention():
                      (dict(k=H(4096, 252, 64)), "strides of k"), (dict(v=H(4096, 0, 64)), "strides of v"), (dict(o=H(4096, 256, 8)), "strides of o")):
         for call in (L.kf_attn_pack_fwd, L.kf_attn_pack_bwd):
             assert call(params(**kw), None) == -1 and text in msg(), (kw, msg())
-    assert L.kf_attn_pack_bwd(params(ws_bytes=64), None) == -1 and "workspace" in msg()
     assert L.kf_attn_pack_bwd(params(dk=H(4096, 256, 63)), None) == -1 and "strides of dk" in msg()
     assert L.kf_attn_pack_fwd(params(n_q_tiles=0), None) == 0 and L.kf_attn_pack_bwd(params(n_q_tiles=0, n_k_tiles=0), None) == 0
-    assert L.kf_attn_pack_ws_bytes(4, 3) >= 4 * 3 * 1024 and L.kf_attn_pack_ws_bytes(0, 3) == -1
+    assert L.kf_attn_pack_ws_bytes(0, 1, 3, 3) == -1 and L.kf_attn_pack_ws_bytes(4, 3, 3, 3) == -1 and L.kf_attn_pack_ws_bytes(4, 2, -1, 3) == -1
 
 
 def test_mirrors_match_the_header(tmp_path):
