@@ -96,6 +96,7 @@ struct Cap {
     flat = (float)(0.5 / r < 1e18 ? 0.5 / r : 1e18);
     double m = scale * LOG2E;
     for (int i = 0; i < 5; ++i, m *= r * r) c[i] = (float)(a[i] * m);
+    if (!(m < 1e30)) flat = -1.f;                               // a cap so small that the polynomial has no range
   }
 };
 __device__ __forceinline__ float2 cap_flat(const Cap& k, float2 x) {

@@ -175,6 +175,19 @@ def test_cap_and_distance(cap, bias, causal, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("cap", [1e-12, 1e-3, 1e6])
+def test_caps_at_the_ends_of_their_range(cap):
+    """a cap that leaves no score (P is uniform over the keys a query sees, and q, k have next to no gradient), and one that changes none"""
+    ops = _ops()
+    lens = [130, 33]
+    q, k, v, do = case(lens, lens, 2, 1, BF, 3)
+    q[5] = 0
+    out, lse, dq, dk, dv = run(q, k, v, do, ops.AttnPlan(lens), cap=cap)
+    close((out, lse, dv), reference(q, k, v, do, lens, lens, False, None, 0.125, cap, None, BF), ("out", "lse", "dv"))
+    assert torch.isfinite(dq).all() and torch.isfinite(dk).all()
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [BF, F16])
 def test_images_of_several_sizes(dtype):
     """more items than CTAs, of one to many tiles"""
