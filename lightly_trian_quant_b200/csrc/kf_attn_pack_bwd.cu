@@ -18,6 +18,10 @@
 //            S(G + 2) is issued while it works on step G; dP(G + 2) goes behind the gradients' products of step G, which read P and dS from
 //            the same buffer, and is needed when the exponentials of step G + 2 are done.  The groups of an item's last step write the
 //            item's gradients, the others go on with the next item.
+//   delta    dO . O takes the output as it was rounded; with ROWS = queries the sum of P (dP - delta) along a row, which should be 0, tells by how
+//            much delta is off, and dQ is put right by that times the product P K (which dQ's error is), as is the delta that the second
+//            launch takes.  Without it dQ and dK of a few queries with steep slopes were 1.53 times as far off as a single
+//            rounding of the result, now 1.4 times; it costs one product more in the first launch
 //   numerics P and dS are rounded to the 16-bit type of the operands (the products' A operand); everything else fp32; three of every four pairs of
 //            exponentials by the special-function unit, the fourth on the FMA pipe
 #include "kf_attn.cuh"
@@ -30,12 +34,12 @@ constexpr int PB_REGS_WORK = 104, PB_REGS_LEAN = 64;
 constexpr int PB_REGS_LAUNCH = 96;
 static_assert(512 * PB_REGS_WORK + 128 * PB_REGS_LEAN <= PB_THREADS * PB_REGS_LAUNCH, "register split");
 constexpr int PB_RTILE = PB_T * PB_D * 2, PB_CTILE = PB_W * PB_D * 2;     // 16 KB, 12 KB
-// Shared memory: row operands in two buffers (with ROWS = queries also O, for delta), a ring of passing ones, with ROWS = keys the log-sum-exp
-// and delta of the passing rows (1 KB per stage), barriers.
+// Shared memory: row operands in two buffers (with ROWS = queries also O, for delta), a ring of passing ones; with ROWS = keys the log-sum-exp
+// and delta of the passing rows (1 KB per stage), with ROWS = queries the row sums of dS of four items (2 KB each); barriers.
 template <bool KEYS>
 struct BwdMem {
   static constexpr int RING = KEYS ? 6 : 5, RTILES = KEYS ? 2 : 3;
-  static constexpr int OFF_C = 2 * RTILES * PB_RTILE, OFF_STAT = OFF_C + RING * 2 * PB_CTILE, OFF_BAR = OFF_STAT + (KEYS ? RING * 1024 : 0);
+  static constexpr int OFF_C = 2 * RTILES * PB_RTILE, OFF_STAT = OFF_C + RING * 2 * PB_CTILE, OFF_BAR = OFF_STAT + (KEYS ? RING : 8) * 1024;
   static constexpr size_t BYTES = (size_t)OFF_BAR + 512;
   static_assert(BYTES <= 227 * 1024, "shared memory");
 };
@@ -125,8 +129,8 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + PB_OFF_BAR);
   uint64_t *r_full = bars, *r_empty = r_full + 2, *c1_full = r_empty + 2, *c2_full = c1_full + PB_RING, *c_empty = c2_full + PB_RING, *st_full = c_empty + PB_RING,
            *s_full = st_full + PB_RING, *s_free = s_full + 2, *dp_full = s_free + 2, *ds_full = dp_full + 2, *d_free = ds_full + 2, *acc_full = d_free + 2,
-           *acc_free = acc_full + 2;
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(acc_free + 1);
+           *acc_free = acc_full + 2, *rs_full = acc_free + 1;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(rs_full + 4);
   volatile uint32_t* abort_flag = tmem_holder + 1;
 
   pdl_launch_dependents();
@@ -151,6 +155,7 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
       mbar_init(&st_full[i], 1);
     }
     mbar_init(acc_free, 256);
+    for (int i = 0; i < 4; ++i) mbar_init(&rs_full[i], 512);
     *abort_flag = 0u;
     fence_mbar_init();
   }
@@ -325,7 +330,7 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
 #pragma unroll
           for (int kk = 0; kk < PB_W / 16; ++kk) {                            // 16 columns of dP hold 8 words of dS and 8 of P
             const uint32_t d = t_d + kk * 16;
-            if (KEYS) mma_f16_ta(tmem_base + PB_COL_A2, d + 8, c2 + (uint64_t)(kk * (2048 >> 4)), idesc, kk ? 1u : more);
+            mma_f16_ta(tmem_base + PB_COL_A2, d + 8, (KEYS ? c2 : c1) + (uint64_t)(kk * (2048 >> 4)), idesc, kk ? 1u : more);
             mma_f16_ta(tmem_base + PB_COL_A1, d, c1 + (uint64_t)(kk * (2048 >> 4)), idesc, kk ? 1u : more);
           }
           tc_commit(d_done);
@@ -379,9 +384,10 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
         if (warp < 4) {
           const int64_t o = I.head * a.stat_ld + (int64_t)I.slot() * PB_T + row;
           a.lse2[o] = nlse2;
-          a.delta[o] = ndelta;
+          if (n == 0) a.delta[o] = 0.f;
         }
       }
+      float2 vsum = make_float2(0.f, 0.f);                       // ROWS = queries: sum of P (dP - delta) over this thread's columns
       // ROWS = queries: the row sees columns below `edge`; ROWS = keys: from `edge` on
       int edge, warp_edge;
       float at;                                                  // ROWS = queries: position; ROWS = keys: the query that stands at the key
@@ -500,13 +506,17 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
             if (KEYS && i % 4 == 0) *reinterpret_cast<float4*>(u) = *reinterpret_cast<const float4*>(stat + 128 + 16 * q + i);
             const float2 m = KEYS ? make_float2(u[i % 4], u[i % 4 + 1]) : splat2(ndelta);
             const float2 pp = make_float2(__uint_as_float(p[q][i]), __uint_as_float(p[q][i + 1]));
-            float2 v = mul2(add2(make_float2(__uint_as_float(d[i]), __uint_as_float(d[i + 1])), m), pp);
-            if constexpr (CAP) v = mul2(v, make_float2(__uint_as_float(f[i]), __uint_as_float(f[i + 1])));
+            float2 v = mul2(add2(make_float2(__uint_as_float(d[i]), __uint_as_float(d[i + 1])), m), pp), g = pp;
+            if constexpr (!KEYS) vsum = add2(vsum, v);
+            if constexpr (CAP) {
+              const float2 b = make_float2(__uint_as_float(f[i]), __uint_as_float(f[i + 1]));
+              v = mul2(v, b);
+              if constexpr (!KEYS) g = mul2(g, b);
+            }
             w[i >> 1] = pack16(v.x, v.y, F16);
-            if (KEYS) w[8 + (i >> 1)] = pack16(pp.x, pp.y, F16);
+            w[8 + (i >> 1)] = pack16(g.x, g.y, F16);
           }
-          if (KEYS) tmem_st16(t_d + 16 * q, w);
-          else tmem_st8(t_d + 16 * q, *reinterpret_cast<const uint32_t(*)[8]>(w));
+          tmem_st16(t_d + 16 * q, w);
         }
         tmem_st_wait();
         tc_fence_before();
@@ -524,7 +534,16 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
       }
       if (!ok) break;
       G0 += n;
-      if (n > 0) ++ri;
+      float* const rs = reinterpret_cast<float*>(smem + PB_OFF_STAT) + (ri & 3) * 4 * PB_T + row;      // [part][row]
+      const uint32_t rs_ph = (ri >> 2) & 1;
+      uint64_t* const rs_bar = &rs_full[ri & 3];
+      if (n > 0) {
+        if (!KEYS) {
+          rs[(par * 2 + half) * PB_T] = vsum.x + vsum.y;
+          mbar_arrive(rs_bar);
+        }
+        ++ri;
+      }
       // the groups of the last step write the item's gradients, those of an item without steps (zeros) groups 0
       if (par != (n > 0 ? (G0 - 1) & 1 : 0u)) continue;
       if (n > 0) {
@@ -537,6 +556,12 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
       uint32_t w[PIECES][16];
       const uint32_t t_a = t_lane + PB_COL_A1 + half * (32 * PIECES);
       const float scale = KEYS && half ? 1.f : a.scale;
+      float gap_d = 0.f;                                         // delta as it was used less what it should have been
+      if (!KEYS && n > 0) {
+        if (!mbar_wait_warp(rs_bar, rs_ph, ctx, 74)) { ok = false; break; }
+        gap_d = -((rs[0] + rs[PB_T]) + (rs[2 * PB_T] + rs[3 * PB_T]));
+        if (half == 0) a.delta[I.head * a.stat_ld + (int64_t)I.slot() * PB_T + row] = row < I.rows() ? ndelta + gap_d : 0.f;
+      }
 #pragma unroll
       for (int i = 0; i < PIECES; ++i) {
         uint32_t r[32];
@@ -544,6 +569,17 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
           tmem_ld32(t_a + 32 * i, r);
           tmem_ld_wait();
           tmem_ld_fence(r);
+          if (!KEYS) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              uint32_t u[16];
+              tmem_ld16(t_a + PB_D + 16 * q, u);
+              tmem_ld_wait();
+              tmem_ld_fence(u);
+#pragma unroll
+              for (int k = 0; k < 16; ++k) r[16 * q + k] = __float_as_uint(fmaf(gap_d, __uint_as_float(u[k]), __uint_as_float(r[16 * q + k])));
+            }
+          }
         } else {
 #pragma unroll
           for (int k = 0; k < 32; ++k) r[k] = 0u;
