@@ -22,8 +22,7 @@
 //            much delta is off, and dQ is put right by that times the product P K (which dQ's error is), as is the delta that the second
 //            launch takes.  Without it dQ and dK of a few queries with steep slopes were 1.53 times as far off as a single
 //            rounding of the result, now 1.4 times; it costs one product more in the first launch
-//   numerics P and dS are rounded to the 16-bit type of the operands (the products' A operand); everything else fp32; three of every four pairs of
-//            exponentials by the special-function unit, the fourth on the FMA pipe
+//   numerics P and dS are rounded to the 16-bit type of the operands (the products' A operand); everything else fp32
 #include "kf_attn.cuh"
 
 namespace kf {
@@ -45,7 +44,9 @@ struct BwdMem {
 };
 constexpr int PB_COL_S = 0, PB_COL_D = 2 * PB_W, PB_COL_A1 = 4 * PB_W, PB_COL_A2 = PB_COL_A1 + PB_D, PB_TMEM_COLS = 512;
 static_assert(PB_COL_A2 + PB_D <= PB_TMEM_COLS, "TMEM budget");
-constexpr int PB_POLY = 0x88, PB_POLY_KEYS = 0x80;              // which of eight element pairs take the polynomial exponential
+// Which of eight element pairs take the polynomial exponential: where instructions are shorter than the special-function unit's time.  8 x 1605 tokens:
+// first launch none / one / two of eight 166.8 / 164.4 / 165.3 us, with a cap (fewer tokens) 69.1 / 72.9 / 74.8, second launch none / one / two 191 / 194 / 201
+__host__ __device__ constexpr int bwd_poly(bool keys, bool cap) { return keys || cap ? 0 : 0x80; }
 
 struct PackBwdArgs {
   const int4* tiles;
@@ -472,7 +473,7 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
                 l.y = fmaf(-slope, fabsf(gap - (float)(c + 1)), l.y);
               }
               x = CAP || BIAS ? add2(x, l) : fma2(x, splat2(a.scale_log2), l);
-              x = ((KEYS ? PB_POLY_KEYS : PB_POLY) >> ((i / 2 + k) % 8)) & 1 ? ex2_poly2_neg(x) : make_float2(ex2(x.x), ex2(x.y));
+              x = (bwd_poly(KEYS, CAP) >> ((i / 2 + k) % 8)) & 1 ? ex2_poly2_neg(x) : make_float2(ex2(x.x), ex2(x.y));
               p[c / 16][c % 16] = __float_as_uint(x.x);
               p[c / 16][c % 16 + 1] = __float_as_uint(x.y);
             }
