@@ -16,7 +16,9 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cstdarg>
+#include <vector>
 
 #include "../../../include/kf_b200.h"
 
@@ -859,6 +861,78 @@ at::Tensor pack_new(const at::Tensor& like, int64_t used) {
   return t;
 }
 
+// The lengths of a plan: any sequence of integers.
+std::vector<int64_t> lengths(PyObject* o, const char* what) {
+  PyObject* seq = PySequence_Fast(o, what);
+  if (!seq) throw Failed{};
+  std::vector<int64_t> v((size_t)PySequence_Fast_GET_SIZE(seq));
+  for (size_t i = 0; i < v.size(); ++i) {
+    PyObject* n = PyNumber_Index(PySequence_Fast_GET_ITEM(seq, (Py_ssize_t)i));
+    v[i] = n ? PyLong_AsLongLong(n) : -1;
+    Py_XDECREF(n);
+    if (!n || (v[i] == -1 && PyErr_Occurred())) {
+      Py_DECREF(seq);
+      throw Failed{};
+    }
+  }
+  Py_DECREF(seq);
+  return v;
+}
+
+// q lengths, k lengths | None, causal, prefixes | None -> (table int32 [query tiles + key tiles, 8] on the CPU, query tiles, query rows, key rows):
+// the records of kf_attn_pack_params, of queries and then of keys, each with the longest work first
+PyObject* attn_plan(PyObject* const* v) {
+  constexpr int64_t T = 128, MOST = INT32_MAX - 256;
+  const std::vector<int64_t> lq = lengths(v[0], "AttnPlan: q_lens must be a sequence of integers"),
+                             lk = v[1] == Py_None ? lq : lengths(v[1], "AttnPlan: k_lens must be a sequence of integers");
+  const bool causal = truth(v[2]);
+  if (lq.size() != lk.size()) fail("AttnPlan: %zd sequences of queries, %zd of keys", (Py_ssize_t)lq.size(), (Py_ssize_t)lk.size());
+  if (v[3] != Py_None && !causal) fail("AttnPlan: a prefix goes with causal=True (without it every key is seen)");
+  const std::vector<int64_t> pre = v[3] == Py_None ? std::vector<int64_t>(lk.size(), 0) : lengths(v[3], "AttnPlan: prefix must be a sequence of integers");
+  if (pre.size() != lk.size()) fail("AttnPlan: %zd sequences, %zd prefixes", (Py_ssize_t)lk.size(), (Py_ssize_t)pre.size());
+  int64_t rows_q = 0, rows_k = 0, nq = 0, nk = 0;
+  for (size_t d = 0; d < lq.size(); ++d) {
+    if (lq[d] < 0 || lk[d] < 0 || pre[d] < 0 || pre[d] > lk[d]) fail("AttnPlan: lengths must not be negative, a prefix not longer than its sequence of keys");
+    if (lq[d] >= MOST || lk[d] >= MOST || (rows_q += lq[d]) >= MOST || (rows_k += lk[d]) >= MOST) fail("AttnPlan: more rows than a call takes");
+    nq += (lq[d] + T - 1) / T;
+    nk += (lk[d] + T - 1) / T;
+  }
+  struct Tile {
+    int64_t work;
+    int32_t w[8];
+  };
+  std::vector<Tile> q, k;
+  q.reserve((size_t)nq);
+  k.reserve((size_t)nk);
+  int64_t q0 = 0, k0 = 0;
+  for (size_t d = 0; d < lq.size(); ++d) {
+    const int64_t p = causal ? pre[d] : lk[d], off = lk[d] - lq[d], slot0 = (int64_t)q.size();
+    for (int64_t i = 0; i < lq[d]; i += T) {
+      const int64_t rows = std::min(T, lq[d] - i), seen = std::clamp(std::max(i + off + rows, p), (int64_t)0, lk[d]);
+      q.push_back({seen, {(int32_t)(q0 + i), (int32_t)rows, (int32_t)k0, (int32_t)lk[d], (int32_t)(i + off), (int32_t)p, (int32_t)q.size(), 0}});
+    }
+    for (int64_t i = 0; i < lk[d]; i += T) {
+      const int64_t low = i < p ? 0 : std::max(i - off, (int64_t)0);
+      k.push_back({lq[d] - low, {(int32_t)(k0 + i), (int32_t)std::min(T, lk[d] - i), (int32_t)q0, (int32_t)lq[d], (int32_t)i, (int32_t)off, (int32_t)p, (int32_t)slot0}});
+    }
+    q0 += lq[d];
+    k0 += lk[d];
+  }
+  const auto longer = [](const Tile& a, const Tile& b) { return a.work > b.work; };
+  std::stable_sort(q.begin(), q.end(), longer);
+  std::stable_sort(k.begin(), k.end(), longer);
+  at::Tensor table = at::empty({nq + nk, 8}, at::TensorOptions().dtype(at::kInt));
+  int32_t* to = table.data_ptr<int32_t>();
+  for (const std::vector<Tile>* tiles : {&q, &k})
+    for (const Tile& t : *tiles) to = std::copy(t.w, t.w + 8, to);
+  PyObject* r = PyTuple_New(4);
+  PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(std::move(table)));
+  PyTuple_SET_ITEM(r, 1, PyLong_FromLongLong(nq));
+  PyTuple_SET_ITEM(r, 2, PyLong_FromLongLong(rows_q));
+  PyTuple_SET_ITEM(r, 3, PyLong_FromLongLong(rows_k));
+  return r;
+}
+
 // ..., out | None
 PyObject* attn_packed(PyObject* const* v) {
   const char* const op = "attn_packed";
@@ -964,7 +1038,7 @@ PyMethodDef g_methods[] = {KF_ENTRY(quant_rows, 4),     KF_ENTRY(ln_quant, 7),  
                            KF_ENTRY(ln_tail, 8),        KF_ENTRY(attn_fwd, 3),   KF_ENTRY(attn_fwd_quant, 4), KF_ENTRY(im2col_patch16, 1), KF_ENTRY(dw_ln, 10),
                            KF_ENTRY(semantic, 3),       KF_ENTRY(amax_scale, 5), KF_ENTRY(ln_amax_scale, 7),
                            KF_ENTRY(layer_norm_fwd, 5), KF_ENTRY(layer_norm_bwd, 7), KF_ENTRY(rope_axes, 9),
-                           KF_ENTRY(attn_packed, 11),   KF_ENTRY(attn_packed_bwd, 16),
+                           KF_ENTRY(attn_plan, 4),      KF_ENTRY(attn_packed, 11),   KF_ENTRY(attn_packed_bwd, 16),
                            KF_ENTRY(reads_weight_early, 1), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_kf_host", "native operator layer over libkf_b200.so", -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

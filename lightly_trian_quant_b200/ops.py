@@ -420,45 +420,10 @@ class AttnPlan:
     __slots__ = ("q_rows", "k_rows", "causal", "q_tiles", "k_tiles")
 
     def __init__(self, q_lens, k_lens=None, *, causal: bool = False, prefix=None, device="cuda"):
-        import numpy as np
-
-        lens = [np.asarray([int(n) for n in (q_lens if ls is None else ls)], dtype=np.int64) for ls in (q_lens, k_lens)]
-        lq, lk = lens
-        if len(lq) != len(lk):
-            raise KfError(f"AttnPlan: {len(lq)} sequences of queries, {len(lk)} of keys")
-        if prefix is not None and not causal:
-            raise KfError("AttnPlan: a prefix goes with causal=True (without it every key is seen)")
-        pre = np.asarray([int(n) for n in prefix], dtype=np.int64) if prefix is not None else np.zeros_like(lk)
-        if len(pre) != len(lk):
-            raise KfError(f"AttnPlan: {len(lk)} sequences, {len(pre)} prefixes")
-        if (lq < 0).any() or (lk < 0).any() or (pre < 0).any() or (pre > lk).any():
-            raise KfError("AttnPlan: lengths must not be negative, a prefix not longer than its sequence of keys")
-        if lq.sum() >= 2**31 - 256 or lk.sum() >= 2**31 - 256:
-            raise KfError("AttnPlan: more rows than a call takes")
-        if not causal:
-            pre = lk
-        T = 128
-        q0, k0 = np.cumsum(lq) - lq, np.cumsum(lk) - lk
-        nq, nk = -(-lq // T), -(-lk // T)
-        slot0 = np.cumsum(nq) - nq
-        self.q_rows, self.k_rows, self.causal = int(lq.sum()), int(lk.sum()), bool(causal)
-
-        def tiles(n, first):                               # (sequence, tile of it) of every tile
-            d = np.repeat(np.arange(len(n)), n)
-            return d, np.arange(len(d)) - first[d]
-
-        d, i = tiles(nq, slot0)
-        rows = np.minimum(T, lq[d] - T * i)
-        pos = T * i + lk[d] - lq[d]
-        q = np.stack([q0[d] + T * i, rows, k0[d], lk[d], pos, pre[d], slot0[d] + i, 0 * d], 1)
-        seen = np.clip(np.maximum(pos + rows, pre[d]), 0, lk[d])
-        q = q[np.argsort(-seen, kind="stable")]
-        d, i = tiles(nk, np.cumsum(nk) - nk)
-        off = lk[d] - lq[d]
-        k = np.stack([k0[d] + T * i, np.minimum(T, lk[d] - T * i), q0[d], lq[d], T * i, off, pre[d], slot0[d]], 1)
-        low = np.where(T * i < pre[d], 0, np.maximum(T * i - off, 0))
-        k = k[np.argsort(low - lq[d], kind="stable")]
-        self.q_tiles, self.k_tiles = (torch.from_numpy(np.ascontiguousarray(t, dtype=np.int32)).reshape(-1, 8).to(device) for t in (q, k))
+        table, n, self.q_rows, self.k_rows = _h.attn_plan(q_lens, k_lens, causal, prefix)
+        self.causal = bool(causal)
+        table = table.to(device)
+        self.q_tiles, self.k_tiles = table[:n], table[n:]
 
 
 def _pack_args(q, k, v, plan: AttnPlan, scale, cap, slopes) -> tuple:
