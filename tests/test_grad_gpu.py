@@ -13,6 +13,12 @@ gpu = pytest.mark.gpu
 BF = torch.bfloat16
 
 
+@pytest.fixture(autouse=True)
+def _with_grad():
+    with torch.enable_grad():                     # modules of the inference path turn it off for the whole process
+        yield
+
+
 def _block(x, w1, b1, wqkv, wout, lens, prefix, pos, table, slopes, cap, low):
     """a pre-norm attention block: low precision through grad, or float64 through the oracle"""
     H = 4
@@ -49,9 +55,8 @@ def test_a_block_and_its_gradients():
     y.backward(dy.cuda())
     ops.check_device_error()
     ref = {n: t.double().requires_grad_() for n, t in data.items()}
-    with torch.enable_grad():
-        want = _block(*ref.values(), lens, prefix, pos, freqs, slopes, 20.0, False)
-        want.backward(dy.double())
+    want = _block(*ref.values(), lens, prefix, pos, freqs, slopes, 20.0, False)
+    want.backward(dy.double())
     rel = lambda a, b: ((a.double().cpu() - b).norm() / b.norm()).item()  # noqa: E731
     errors = {"y": rel(y.detach() - leaves["x"].detach(), (want - ref["x"]).detach()), **{n: rel(t.grad, ref[n].grad) for n, t in leaves.items()}}
     assert max(errors.values()) < 6 * 2 ** -8, errors
