@@ -746,6 +746,87 @@ Heads heads_of(const at::Tensor& x, const char* op, const char* what) {
   return {o ? x.size(0) : 1, x.size(o), x.size(o + 1), x.size(o + 2), o ? x.stride(0) : 0, x.stride(o), x.stride(o + 1)};
 }
 
+// The bytes of a tensor of up to four dimensions: blocks of `len` (its last dimension where that is contiguous) at steps of the others.
+struct Blocks {
+  int64_t at, len, end;
+  int n = 0;
+  int64_t count[4], step[4];
+  explicit Blocks(const at::Tensor& t) {
+    const int64_t size = (int64_t)t.element_size(), dim = t.dim(), row = dim && (t.stride(-1) == 1 || t.size(-1) == 1);
+    at = (int64_t)reinterpret_cast<uintptr_t>(t.data_ptr());
+    len = t.numel() ? (row ? t.size(-1) : 1) * size : 0;
+    end = at + len;
+    for (int64_t i = 0; t.numel() && i < dim - row; ++i)
+      if (t.size(i) > 1) {
+        count[n] = t.size(i);
+        step[n++] = t.stride(i) * size;
+        end += (t.size(i) - 1) * t.stride(i) * size;
+      }
+  }
+  bool operator==(const Blocks& o) const {
+    return at == o.at && len == o.len && n == o.n && std::equal(count, count + n, o.count) && std::equal(step, step + n, o.step);
+  }
+};
+
+// Whether two tensors share a byte; of a tensor with itself: whether two of its places do.  Looks for steps that bring a block of one to a block of
+// the other, the longest first, each bounded by what the shorter ones can still make up: few to look at where dimensions lie inside one another, as
+// parts of a projection do.  Where there are more than it looks at, the tensors count as overlapping.
+class Overlap {
+ public:
+  static bool of(const Blocks& a, const Blocks& b) { return a.len && b.len && a.at < b.end && b.at < a.end && Overlap(a, b, false).found_; }
+  static bool inside(const Blocks& a) { return a.len && Overlap(a, a, true).found_; }
+
+ private:
+  struct Dim {
+    int64_t step, lo, hi;
+  };
+  Overlap(const Blocks& a, const Blocks& b, bool self) : low_(-b.len), high_(a.len), self_(self) {
+    for (int i = 0; i < a.n; ++i) add(a.step[i], -(a.count[i] - 1), 0);
+    for (int i = 0; i < b.n; ++i) add(b.step[i], 0, b.count[i] - 1);
+    for (int i = 1; self && i < a.n; ++i) found_ |= std::find(a.step, a.step + i, a.step[i]) != a.step + i;      // (1, 0) and (0, 1) are one place
+    if (found_) return;
+    std::sort(dims_, dims_ + n_, [](const Dim& x, const Dim& y) { return x.step > y.step; });
+    found_ = reaches(0, b.at - a.at, false);
+  }
+  void add(int64_t step, int64_t lo, int64_t hi) {
+    if (step == 0) {                                               // the same place again
+      found_ |= self_;
+      return;
+    }
+    for (int i = 0; i < n_; ++i)
+      if (dims_[i].step == step) {
+        dims_[i].lo += lo;
+        dims_[i].hi += hi;
+        return;
+      }
+    dims_[n_++] = {step, lo, hi};
+  }
+  bool reaches(int i, int64_t apart, bool moved) {
+    if (i == n_) return low_ < apart && apart < high_ && (moved || !self_);
+    int64_t least = 0, most = 0;
+    for (int k = i + 1; k < n_; ++k) {
+      least += dims_[k].lo * dims_[k].step;
+      most += dims_[k].hi * dims_[k].step;
+    }
+    const Dim& d = dims_[i];
+    const auto floor_div = [](int64_t x, int64_t y) { return x / y - (x % y < 0); };
+    const int64_t first = std::max(d.lo, floor_div(low_ - most - apart, d.step) + 1), last = std::min(d.hi, -floor_div(apart + least - high_, d.step) - 1);
+    for (int64_t x = first; x <= last; ++x) {
+      if (--budget_ < 0 || reaches(i + 1, apart + x * d.step, moved || x != 0)) return true;
+    }
+    return false;
+  }
+  Dim dims_[8];
+  int n_ = 0, budget_ = 4096;
+  int64_t low_, high_;
+  bool self_, found_ = false;
+};
+
+// `out` is about to be written by an operator that reads (or writes) `other` as well
+void apart(const at::Tensor& out, const at::Tensor& other, const char* op, const char* what, const char* from) {
+  if (Overlap::of(Blocks(out), Blocks(other))) fail("%s: %s overlaps %s", op, what, from);
+}
+
 // x, pos, freq (fp64 [P]), axis (int32 [P]), axes, head channels, interleaved, inverse, out | None
 PyObject* rope_axes(PyObject* const* v) {
   const char* const op = "rope_axes";
@@ -773,6 +854,10 @@ PyObject* rope_axes(PyObject* const* v) {
   const Heads o = heads_of(out, op, "out");
   if (v[8] != Py_None) {
     need((o.sg != 0 || o.g < 2) && (o.st != 0 || o.t < 2) && (o.sh != 0 || o.h < 2), "rope_axes: out must not be an expanded tensor");
+    const Blocks to(out);
+    need(!Overlap::inside(to), "rope_axes: out overlaps itself");
+    need(Blocks(x) == to || !Overlap::of(to, Blocks(x)), "rope_axes: out must be x or not overlap it");
+    apart(out, pos, op, "out", "pos");
     writable(out);
   }
   kf_rope_params p = {};
@@ -810,6 +895,7 @@ void same_shape(const at::Tensor& a, const at::Tensor& b, const char* op, const 
 void same_place(const at::Tensor& t, const char* op, const char* what) {          // written row by row from many threads
   for (int i = 0; i < 2; ++i)
     if (t.size(i) > 1 && t.stride(i) == 0) fail("%s: %s must not be an expanded tensor", op, what);
+  if (Overlap::inside(Blocks(t))) fail("%s: %s overlaps itself", op, what);
 }
 
 // What both directions share.  v: q, k, v, q_tiles, k_tiles, query rows, key rows, scale, cap, slopes | None
@@ -945,6 +1031,9 @@ PyObject* attn_packed(PyObject* const* v) {
     out = pack_tensor(v[10], &c.q, op, "out");
     same_shape(c.q, out, op, "out");
     same_place(out, op, "out");
+    apart(out, c.q, op, "out", "q");
+    apart(out, c.k, op, "out", "k");
+    apart(out, c.v, op, "out", "v");
     writable(out);
   }
   at::Tensor lse = empty({c.q.size(1), c.q.size(0)}, at::kFloat, c.q.device());
@@ -981,6 +1070,11 @@ PyObject* attn_packed_bwd(PyObject* const* v) {
     g[i] = pack_tensor(v[13 + i], &c.q, op, names[i]);
     same_shape(*of[i], g[i], op, names[i]);
     same_place(g[i], op, names[i]);
+    const at::Tensor* const others[] = {&c.q, &c.k, &c.v, &dout, &out, &lse};
+    const char* const from[] = {"q", "k", "v", "dout", "out", "lse"};
+    for (int j = 0; j < 6; ++j) apart(g[i], *others[j], op, names[i], from[j]);
+    for (int j = 0; j < i; ++j)
+      if (g[j].defined()) apart(g[i], g[j], op, names[i], names[j]);
   }
   for (int i = 0; i < 3; ++i) {
     if (g[i].defined()) writable(g[i]);

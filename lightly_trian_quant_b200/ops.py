@@ -398,9 +398,9 @@ class RopeTable:
 
 
 def rope_axes(x: torch.Tensor, pos: torch.Tensor, table: RopeTable, *, inverse: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """x [T, H, D] or [G, T, H, D] (f32 | bf16 | f16, channels contiguous, any other strides) with every head turned by its token's positions
-    pos [T, axes] (int32 | int64 | fp32).  inverse=True turns back, which is also the gradient.  out may be x.  Tokens that are not to be turned
-    (cls, registers, queries) have position 0.  Angles are exact to fp32 however far the position."""
+    """x [T, H, D] or [G, T, H, D] (f32 | bf16 | f16, channels contiguous, any other strides; interleaved pairs at even ones) with every head turned by
+    its token's positions pos [T, axes] (int32 | int64 | fp32).  inverse=True turns back, which is also the gradient.  out may be x, but not overlap it
+    otherwise.  Tokens that are not to be turned (cls, registers, queries) have position 0.  Angles are exact to fp32 however far the position."""
     global LAUNCHES
     LAUNCHES += 1
     args = (x, pos, table.freq, table.axis, table.axes, table.head_dim, table.interleaved, inverse, out)
@@ -437,7 +437,7 @@ def attn_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: AttnPla
 
     score = scale * q . k (scale 1/8 by default), then cap * tanh(score / cap) with cap > 0, then minus slopes[head] * |distance| (fp32 [Hq]);
     plan says which keys a query sees.  A query that sees nothing gets 0 and -inf.  Rows behind the last sequence: zero in new tensors, left as they
-    were in a given out.  Keys and values inside a sequence have to be finite; rows outside the sequences may hold anything."""
+    were in a given out, which may not overlap q, k or v.  Keys and values inside a sequence have to be finite; rows outside the sequences may hold anything."""
     global LAUNCHES
     LAUNCHES += 1
     args = (*_pack_args(q, k, v, plan, scale, cap, slopes), out)
@@ -447,8 +447,9 @@ def attn_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: AttnPla
 def attn_packed_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, lse: torch.Tensor, plan: AttnPlan, *,
                     scale: Optional[float] = None, cap: float = 0.0, slopes: Optional[torch.Tensor] = None, grads=(None, None, None)):
     """Gradients of attn_packed -> (dq, dk, dv) in the operands' type; the other arguments as the forward took and gave them (slopes have no
-    gradient).  grads: tensors to write instead of new ones, e.g. the parts of one projection's gradient.  f16 gradients have the range of f16: scale
-    the loss as for any f16 product.  No atomics: the same bits from run to run."""
+    gradient).  q and dout inside a sequence have to be finite as k and v.  grads: tensors to write instead of new ones, e.g. the parts of one
+    projection's gradient; they may not overlap one another or what the call reads.  f16 gradients have the range of f16: scale the loss as for any
+    f16 product.  No atomics: the same bits from run to run."""
     global LAUNCHES
     LAUNCHES += 2
     args = (*_pack_args(q, k, v, plan, scale, cap, slopes), dout, out, lse, *grads)

@@ -380,6 +380,38 @@ def test_refusals():
     assert torch.equal(ops.attn_packed(q, k, v, plan)[0], out)
 
 
+@gpu
+def test_outputs_that_overlap_what_is_read():
+    """refused, while parts of one buffer that lie between one another without a common byte are taken"""
+    ops = _ops()
+    q, k, v, do = case([40], [40], 4, 2, BF, 1)
+    plan = ops.AttnPlan([40])
+    out, lse = ops.attn_packed(q, k, v, plan)
+    want = ops.attn_packed_bwd(do, q, k, v, out, lse, plan)
+    flat, both = torch.zeros(45 * 8 * 64, dtype=BF, device="cuda"), torch.zeros(40, 8, 64, dtype=BF, device="cuda")
+    both[:, :4], both[:, 4:6], both[:, 6:] = q, k, v
+    bq, bk, bv = both[:, :4], both[:, 4:6], both[:, 6:]
+    overlapping = flat.as_strided((40, 4, 64), (64, 64, 1))
+    shifted = flat[32 * 64:].as_strided((40, 4, 64), (512, 64, 1))
+    f = lambda o, q=q, k=k, v=v: (lambda: ops.attn_packed(q, k, v, plan, out=o))  # noqa: E731
+    b = lambda *g: (lambda: ops.attn_packed_bwd(do, q, k, v, out, lse, plan, grads=g))  # noqa: E731
+    for bad in (f(q), f(both[:, 3:7], bq, bk, bv), f(both[:, 4:], bq, bk, bv), f(overlapping), b(q, None, None), b(do, None, None), b(out, None, None),
+                b(None, k, None), b(None, None, v), b(None, want[1], want[1]), b(flat.as_strided((40, 4, 64), (512, 64, 1)), both[:, :2], both[:, 1:3]),
+                b(shifted, flat[33 * 64:].as_strided((40, 2, 64), (512, 64, 1)), None)):
+        with pytest.raises(ops.KfError):
+            bad()
+    # heads of q, k and v in turn, gradients side by side, an output in the columns that the call does not read
+    turn = torch.zeros(40, 4, 2, 64, dtype=BF, device="cuda")
+    turn[:, :, 0] = q
+    assert torch.equal(ops.attn_packed(turn[:, :, 0], k, v, plan, out=turn[:, :, 1])[0], out)
+    side = torch.zeros(40, 8, 64, dtype=BF, device="cuda")
+    got = ops.attn_packed_bwd(do, bq, bk, bv, out, lse, plan, grads=(side[:, :4], side[:, 4:6], side[:, 6:]))
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+    # key rows of one tensor behind the query rows of another: extents side by side
+    assert torch.equal(ops.attn_packed(q, k, v, plan, out=flat[:40 * 256].view(40, 4, 64))[0], out)
+    ops.check_device_error()
+
+
 def test_plan_says_who_sees_whom():
     """the tables of random batches, expanded to (query, key) pairs, are the masks; slots number the query tiles along the rows"""
     import random

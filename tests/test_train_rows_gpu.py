@@ -244,6 +244,22 @@ def test_rope_refusals():
     assert ops.rope_axes(x[:0], pos[:0], table).shape == (0, 2, 64)
 
 
+@gpu
+def test_rope_outputs_that_overlap_the_input():
+    ops = _ops()
+    pos, table = torch.arange(8, device="cuda").view(4, 2).int(), ops.RopeTable(FREQS[64], 64)
+    buf = torch.randn(2, 4, 6, 64, device="cuda")
+    x = buf[:, :, :3]
+    want = ops.rope_axes(x, pos, table)
+    for bad in (buf[:, :, 2:5], buf[:, :, 1:4], buf.flatten()[32:32 + 2 * 4 * 192].view(2, 4, 3, 64), buf.as_strided((2, 4, 3, 64), (64, 64, 64, 1)),
+                torch.zeros(1024, device="cuda").as_strided((2, 4, 3, 64), (192, 64, 64, 1))):
+        with pytest.raises(ops.KfError, match="overlap"):
+            ops.rope_axes(x, pos, table, out=bad)
+    assert torch.equal(ops.rope_axes(x, pos, table, out=buf[:, :, 3:]), want)        # the columns between
+    assert torch.equal(ops.rope_axes(x, pos, table, out=x), want)
+    ops.check_device_error()
+
+
 def test_rope_table_refusals():
     ops = _ops()
     for bad in (lambda: ops.RopeTable([[1.0] * 33], 64, device="cpu"), lambda: ops.RopeTable([[1.0]], 258, device="cpu"), lambda: ops.RopeTable([[float("inf")]], 64, device="cpu"),
