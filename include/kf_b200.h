@@ -331,6 +331,7 @@ typedef struct kf_heads {
 } kf_heads;
 typedef struct kf_attn_pack_params {
   int dtype, Hq, Hk, n_q_tiles, n_k_tiles;
+  int longest;             /* the most keys that a record of q_tiles sees, 0 if not known: then few records are not split along their keys */
   float scale, cap;        /* scale > 0; cap 0 = none                                                  */
   int64_t Tq, Tk;
   const int32_t *q_tiles, *k_tiles;

@@ -47,7 +47,7 @@ class Heads(C.Structure):
 
 class AttnPackParams(C.Structure):
     """mirror of kf_attn_pack_params."""
-    _fields_ = [("dtype", C.c_int), ("Hq", C.c_int), ("Hk", C.c_int), ("n_q_tiles", C.c_int), ("n_k_tiles", C.c_int), ("scale", C.c_float), ("cap", C.c_float),
+    _fields_ = [("dtype", C.c_int), ("Hq", C.c_int), ("Hk", C.c_int), ("n_q_tiles", C.c_int), ("n_k_tiles", C.c_int), ("longest", C.c_int), ("scale", C.c_float), ("cap", C.c_float),
                 ("Tq", C.c_int64), ("Tk", C.c_int64), ("q_tiles", C.c_void_p), ("k_tiles", C.c_void_p), ("slopes", C.c_void_p), ("lse", C.c_void_p),
                 ("q", Heads), ("k", Heads), ("v", Heads), ("o", Heads), ("dout", Heads), ("dq", Heads), ("dk", Heads), ("dv", Heads), ("ws", C.c_void_p),
                 ("ws_bytes", C.c_int64)]

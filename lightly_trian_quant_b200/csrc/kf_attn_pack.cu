@@ -16,9 +16,12 @@
 //     fall with the distance, and a maximum that rises from tile to tile sends every tile down the slow path (200 queries behind 1605
 //     keys, slope 1/16: 49 us in the keys' order)
 //   - the polynomial exponential is a degree finer, for the log-sum-exp
+//   - few items over long keys (SPLIT): a cluster of up to eight CTAs takes an item, each a share of the key tiles, and joins its parts through the
+//     shared memory of its CTAs: accumulators, maxima and sums in fp32, in the order of the parts
 #include <type_traits>
 
 #include "kf_attn.cuh"
+#include "kf_sm100_pair.cuh"
 
 namespace kf {
 
@@ -34,6 +37,11 @@ constexpr int PK_POLY_K = 3;                           // element pairs PK_POLY_
 constexpr int PK_SBUF = 2;
 constexpr int PK_TMEM_COLS = 256, PK_COL_O = PK_SBUF * PK_BN;
 static_assert(PK_COL_O + PK_D <= PK_TMEM_COLS, "TMEM budget");
+// A split item: the CTAs of a cluster take a share of its key tiles each, leave their accumulators, maxima and sums in shared memory (where K and V
+// were) and put a share of the rows together each.
+constexpr int PK_PARTS = 8, PK_LD = PK_D + 4;             // rows of 68 floats: no two of eight neighbours in the same banks
+constexpr int PK_OFF_PART = PK_OFF_K, PK_OFF_ML = PK_OFF_PART + PK_BM * PK_LD * 4;
+static_assert(PK_OFF_ML + PK_BM * 8 <= PK_OFF_BAR, "a part's results take the place of K and V");
 
 struct PackFwdArgs {
   void* O;
@@ -46,10 +54,22 @@ struct PackFwdArgs {
   Cap cap;
   const float* slopes;      // [Hq]
   int wide;                 // rows of O are 32-byte aligned
+  int parts;                // CTAs per item (SPLIT)
   unsigned int* err;
 };
 
-template <int F16, bool CAP, bool BIAS>
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 ld_cluster2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+
+template <int F16, bool CAP, bool BIAS, bool SPLIT>
 __global__ void __launch_bounds__(PK_THREADS, 2)
 attn_pack_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                      const __grid_constant__ PackFwdArgs a) {
@@ -63,7 +83,7 @@ attn_pack_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   pdl_launch_dependents();
   const int warp = warp_index(), lane = threadIdx.x & 31;
   const int items = a.n_tiles * a.Hq;
-  const int n_my = items_of_cta(items);
+  const int n_my = SPLIT ? 1 : items_of_cta(items);
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -99,12 +119,30 @@ attn_pack_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     a.err[1] = 110;
     a.err[2] = blockIdx.x;
   }
-  auto tile_of = [&](int it) { return load_tile<QTile>(a.tiles, item_of_cta(it) / a.Hq); };
-  auto head_of = [&](int it) { return item_of_cta(it) % a.Hq; };
-  auto key_tiles = [](const QTile& t) { return (t.limit(t.rows - 1) + PK_BN - 1) / PK_BN; };
+  const int rank = SPLIT ? (int)cluster_ctarank() : 0;
+  auto item_at = [&](int it) { return SPLIT ? (int)blockIdx.x / a.parts : item_of_cta(it); };
+  auto tile_of = [&](int it) { return load_tile<QTile>(a.tiles, item_at(it) / a.Hq); };
+  auto head_of = [&](int it) { return item_at(it) % a.Hq; };
+  auto all_tiles = [](const QTile& t) { return (t.limit(t.rows - 1) + PK_BN - 1) / PK_BN; };
+  int all = 0, first = 0, mine = 0;                        // SPLIT: the item's key tiles and this CTA's of them, in the order of tile_at
+  if constexpr (SPLIT) {
+    all = all_tiles(tile_of(0));
+    first = all * rank / a.parts;
+    mine = all * (rank + 1) / a.parts - first;
+  }
+  auto key_tiles = [&](const QTile& t) { return SPLIT ? mine : all_tiles(t); };
   // the order of an item's n key tiles: from tile `start` up, then from the one in front of it down
-  auto start_of = [](const QTile& t, int n) { return !BIAS || t.pos < 0 ? 0 : t.pos / PK_BN < n ? t.pos / PK_BN : n - 1; };
-  auto tile_at = [](int i, int start, int n) { return !BIAS ? i : start + i < n ? start + i : n - 1 - i; };
+  auto start_of = [&](const QTile& t, int n) {
+    if (SPLIT) n = all;
+    return !BIAS || t.pos < 0 ? 0 : t.pos / PK_BN < n ? t.pos / PK_BN : n - 1;
+  };
+  auto tile_at = [&](int i, int start, int n) {
+    if (SPLIT) {
+      i += first;
+      n = all;
+    }
+    return !BIAS ? i : start + i < n ? start + i : n - 1 - i;
+  };
 
   if (warp >= 4) {
   setmaxnreg_dec<PK_REGS_LEAN>();
@@ -444,7 +482,28 @@ attn_pack_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     }
     // the item's last PV product
     if (ok && n_kt > 0) ok = mbar_wait_warp(&o_full[buf == 0 ? PK_SBUF - 1 : buf - 1], buf == 0 ? sph ^ 1 : sph, ctx, 49);
-    if (ok) {
+    if (SPLIT && ok) {
+      float* part = reinterpret_cast<float*>(smem + PK_OFF_PART) + row * PK_LD;
+      if (n_kt > 0) tc_fence_after();
+#pragma unroll 1
+      for (int c = 0; c < 2; ++c) {
+        uint32_t r[32];
+        if (n_kt > 0) {
+          tmem_ld32(t_lane + PK_COL_O + 32 * c, r);
+          tmem_ld_wait();
+          tmem_ld_fence(r);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) r[i] = 0u;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) reinterpret_cast<uint4*>(part)[8 * c + i] = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
+      }
+      // a part of which the row sees nothing has no maximum (what its sum holds comes from masked keys)
+      const bool nothing = n_kt == 0 || (BIAS ? m_run == -INFINITY : lim <= first * PK_BN);
+      reinterpret_cast<float2*>(smem + PK_OFF_ML)[row] = nothing ? make_float2(-INFINITY, 0.f) : make_float2(m_run * sc, l_run);
+    }
+    if (!SPLIT && ok) {
       uint32_t r0[32], r1[32];
       if (n_kt > 0) {
         tc_fence_after();
@@ -479,7 +538,53 @@ attn_pack_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       }
     }
     }   // items
+    if constexpr (SPLIT) {
+      __syncwarp();
+      cluster_sync_all();                                        // every part of the item lies in its CTA's shared memory
+      const QTile tile = tile_of(0);
+      const int h = head_of(0), r1 = PK_BM * (rank + 1) / a.parts;
+      const uint32_t part0 = smem_u32(smem + PK_OFF_PART), ml0 = smem_u32(smem + PK_OFF_ML);
+      for (int r = PK_BM * rank / a.parts + (int)(threadIdx.x >> 3); r < r1 && r < tile.rows; r += 16) {      // eight threads a row, eight channels each
+        const int c = threadIdx.x & 7;
+        float2 ml[PK_PARTS];
+        float4 x[PK_PARTS], y[PK_PARTS];
+#pragma unroll
+        for (int p = 0; p < PK_PARTS; ++p) {
+          ml[p] = make_float2(-INFINITY, 0.f);
+          if (p < a.parts) {                                     // all on their way before the first is used
+            const uint32_t at = map_addr(part0 + (r * PK_LD + c * 8) * 4, p);
+            ml[p] = ld_cluster2(map_addr(ml0 + r * 8, p));
+            x[p] = ld_cluster4(at);
+            y[p] = ld_cluster4(at + 16);
+          }
+        }
+        float m = -INFINITY, l = 0.f, o[8] = {};
+#pragma unroll
+        for (int p = 0; p < PK_PARTS; ++p) m = amax_nan(m, ml[p].x);
+#pragma unroll
+        for (int p = 0; p < PK_PARTS; ++p) {
+          if (p < a.parts) {
+            const float w = ml[p].x == -INFINITY ? 0.f : ex2(ml[p].x - m);
+            l = fmaf(w, ml[p].y, l);
+            o[0] = fmaf(w, x[p].x, o[0]); o[1] = fmaf(w, x[p].y, o[1]); o[2] = fmaf(w, x[p].z, o[2]); o[3] = fmaf(w, x[p].w, o[3]);
+            o[4] = fmaf(w, y[p].x, o[4]); o[5] = fmaf(w, y[p].y, o[5]); o[6] = fmaf(w, y[p].z, o[6]); o[7] = fmaf(w, y[p].w, o[7]);
+          }
+        }
+        const bool none = tile.limit(r) == 0;
+        const float inv = 1.0f / l;
+        const uint4 w = none ? make_uint4(0u, 0u, 0u, 0u)
+                             : make_uint4(pack16(o[0] * inv, o[1] * inv, F16), pack16(o[2] * inv, o[3] * inv, F16), pack16(o[4] * inv, o[5] * inv, F16), pack16(o[6] * inv, o[7] * inv, F16));
+        uint8_t* dst = static_cast<uint8_t*>(a.O) + 2 * ((int64_t)(tile.row + r) * a.o_st + (int64_t)h * a.o_sh);
+        reinterpret_cast<uint4*>(dst)[c] = w;
+        if (c == 0) a.lse[(int64_t)h * a.lse_ld + tile.row + r] = none ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+      }
     }
+    }
+  }
+  if constexpr (SPLIT) {
+    __syncwarp();
+    if (warp >= 4 || bad_align) cluster_sync_all();              // the softmax warps have been there
+    cluster_sync_all();                                          // nobody reads this CTA's shared memory any more
   }
 
   tc_fence_before();
@@ -556,6 +661,15 @@ int check_pack(const kf_attn_pack_params* p) {
 
 using namespace kf;
 
+// CTAs per item: more than one where the items leave room for them and the longest has three tiles or more for each.  The join costs about 3 us (32 KB per
+// part and item pass between SMs), a tile 0.8 us: 4 items of 128 queries on 1029 keys (11 tiles) 12.4 us unsplit, 11.9 / 10.1 / 9.2 / 9.6 / 9.3 in 2 / 3 / 4 / 5 / 6
+// parts; 8 items on 517 keys (6 tiles) 8.6 unsplit, 9.8 / 8.7 in 2 / 3; 24 items on 8197 keys 74 unsplit, 23 in 8
+static int fwd_parts(int64_t items, int longest, int slots) {
+  const int64_t tiles = (longest + PK_BN - 1) / PK_BN, room = slots / items;
+  const int64_t most = tiles < 9 ? 1 : tiles / 3 < room ? tiles / 3 : room;
+  return most < 2 ? 1 : most < PK_PARTS ? (int)most : PK_PARTS;
+}
+
 extern "C" int kf_attn_pack_fwd(const kf_attn_pack_params* p, void* stream) {
   int rc = check_pack(p);
   if (rc != KF_OK) return rc;
@@ -578,17 +692,24 @@ extern "C" int kf_attn_pack_fwd(const kf_attn_pack_params* p, void* stream) {
   if ((rc = make_tmap_heads(&tk, k.ptr, k_rows, k_heads, k.row_stride, k.head_stride, PK_BN)) != KF_OK) return rc;
   if ((rc = make_tmap_heads(&tv, v.ptr, k_rows, k_heads, v.row_stride, v.head_stride, PK_BN)) != KF_OK) return rc;
   using KernelFn = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, PackFwdArgs);
-  static const KernelFn table[2][2][2] = {{{attn_pack_fwd_kernel<0, false, false>, attn_pack_fwd_kernel<0, false, true>}, {attn_pack_fwd_kernel<0, true, false>, attn_pack_fwd_kernel<0, true, true>}},
-                                          {{attn_pack_fwd_kernel<1, false, false>, attn_pack_fwd_kernel<1, false, true>}, {attn_pack_fwd_kernel<1, true, false>, attn_pack_fwd_kernel<1, true, true>}}};
-  const int f = p->dtype == KF_F16, c = p->cap > 0.f, b = p->slopes != nullptr;
-  const KernelFn kern = table[f][c][b];
-  static PerDevice<bool> attr_set[2][2][2];
+  int sms = 0;
+  if ((rc = device_sm_count(&sms)) != KF_OK) return rc;
+  const int64_t items = (int64_t)p->n_q_tiles * p->Hq;
+  const int parts = fwd_parts(items, p->longest, 2 * sms);    // two CTAs are resident per SM
+  static const KernelFn table[2][2][2][2] = {
+      {{{attn_pack_fwd_kernel<0, false, false, false>, attn_pack_fwd_kernel<0, false, false, true>}, {attn_pack_fwd_kernel<0, false, true, false>, attn_pack_fwd_kernel<0, false, true, true>}},
+       {{attn_pack_fwd_kernel<0, true, false, false>, attn_pack_fwd_kernel<0, true, false, true>}, {attn_pack_fwd_kernel<0, true, true, false>, attn_pack_fwd_kernel<0, true, true, true>}}},
+      {{{attn_pack_fwd_kernel<1, false, false, false>, attn_pack_fwd_kernel<1, false, false, true>}, {attn_pack_fwd_kernel<1, false, true, false>, attn_pack_fwd_kernel<1, false, true, true>}},
+       {{attn_pack_fwd_kernel<1, true, false, false>, attn_pack_fwd_kernel<1, true, false, true>}, {attn_pack_fwd_kernel<1, true, true, false>, attn_pack_fwd_kernel<1, true, true, true>}}}};
+  const int f = p->dtype == KF_F16, c = p->cap > 0.f, b = p->slopes != nullptr, s = parts > 1;
+  const KernelFn kern = table[f][c][b][s];
+  static PerDevice<bool> attr_set[2][2][2][2];
   int dev = 0;
   cudaGetDevice(&dev);
-  if (!attr_set[f][c][b].get(dev)) {
+  if (!attr_set[f][c][b][s].get(dev)) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PK_SMEM);
     if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(attn_pack_fwd_kernel)");
-    attr_set[f][c][b].put(dev, true);
+    attr_set[f][c][b][s].put(dev, true);
   }
   constexpr float LOG2E = 1.4426950408889634f;
   PackFwdArgs a{};
@@ -600,9 +721,8 @@ extern "C" int kf_attn_pack_fwd(const kf_attn_pack_params* p, void* stream) {
   a.wide = ((reinterpret_cast<uintptr_t>(o.ptr) | (uintptr_t)(o.row_stride * 2) | (uintptr_t)(o.head_stride * 2)) & 31) == 0;
   a.err = dev_error_ptr();
   KF_REQUIRE(a.err != nullptr, "kf_attn_pack_fwd: device error word unavailable");
-  int sms = 0;
-  if ((rc = device_sm_count(&sms)) != KF_OK) return rc;
-  const int64_t items = (int64_t)p->n_q_tiles * p->Hq;
-  const int grid = items < 2 * sms ? (int)items : 2 * sms;    // two CTAs are resident per SM
-  return cuda_status(launch_maybe_pdl(p->Tq, kern, dim3(grid), dim3(PK_THREADS), PK_SMEM, static_cast<cudaStream_t>(stream), tq, tk, tv, a), "kf_attn_pack_fwd launch");
+  a.parts = parts;
+  const int grid = parts > 1 ? (int)items * parts : items < 2 * sms ? (int)items : 2 * sms;
+  return cuda_status(launch_maybe_pdl_cluster(p->Tq, parts, kern, dim3(grid), dim3(PK_THREADS), PK_SMEM, static_cast<cudaStream_t>(stream), tq, tk, tv, a),
+                     "kf_attn_pack_fwd launch");
 }

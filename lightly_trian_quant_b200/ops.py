@@ -417,17 +417,17 @@ class AttnPlan:
 
     A record per 128 rows of queries and of keys, the longest work first: the kernels' CTAs take them in turn."""
 
-    __slots__ = ("q_rows", "k_rows", "causal", "q_tiles", "k_tiles")
+    __slots__ = ("q_rows", "k_rows", "longest", "causal", "q_tiles", "k_tiles")
 
     def __init__(self, q_lens, k_lens=None, *, causal: bool = False, prefix=None, device="cuda"):
-        table, n, self.q_rows, self.k_rows = _h.attn_plan(q_lens, k_lens, causal, prefix)
+        table, n, self.q_rows, self.k_rows, self.longest = _h.attn_plan(q_lens, k_lens, causal, prefix)
         self.causal = bool(causal)
         table = table.to(device)
         self.q_tiles, self.k_tiles = table[:n], table[n:]
 
 
 def _pack_args(q, k, v, plan: AttnPlan, scale, cap, slopes) -> tuple:
-    return q, k, v, plan.q_tiles, plan.k_tiles, plan.q_rows, plan.k_rows, 0.125 if scale is None else scale, cap, slopes
+    return q, k, v, plan.q_tiles, plan.k_tiles, plan.q_rows, plan.k_rows, plan.longest, 0.125 if scale is None else scale, cap, slopes
 
 
 def attn_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: AttnPlan, *, scale: Optional[float] = None, cap: float = 0.0,

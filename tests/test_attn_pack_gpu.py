@@ -5,7 +5,10 @@ A rounding is off by at most u |x|, with a standard deviation of at most u |x| /
 6 standard deviations of sum_j r_j x_j v_j are 6 / sqrt(3) u sqrt(sum x_j^2 v_j^2) < 3.5 u sqrt(...).  The fp32 part is bounded outright: the exponent of
 a score is off by E = 2^-24 (72 sum_c |q_c k_c| scale + 8 |s| + 4 cap) + 4e-6 (accumulation, scaling, exponentials' 2.7e-6), and so P by the factor E.
 delta = rowsum(dO * O) takes the rounded output: off by 3.5 u sqrt(sum (dO O)^2) for the whole row.  Numbers below the 16-bit type's normal range are
-off by half its smallest step."""
+off by half its smallest step.  Below 2^-126 the exponential gives 0 (ex2.ftz) or stops falling (the polynomial's clamp), and products of fp32 numbers may
+be flushed: P and dS are off by up to 2^-126 besides, which for a key 97 steps of slope 0.9 away from any query (P = e^-87.3 = 2^-126) is more than half a
+step of bf16 below its normal range, 2^-134: with |dP - delta| about 15, |Q| 3 and 1/8 for the scale 2^-126 * 6 = 7e-38 where 3.5 * 2^-134 * sqrt(201) =
+2.3e-39 was allowed."""
 import math
 
 import pytest
@@ -58,7 +61,7 @@ def reference(q, k, v, do, q_lens, k_lens, causal, prefix, scale, cap, slopes, d
             E = 2.0 ** -24 * (72 * (Q.abs() @ K.abs().t()) * scale + 8 * s.masked_fill(~sees, 0).abs() + 4 * cap) + 4e-6
             o = p @ V
             val["out"][rq, h], val["lse"][h, rq] = o, z[:, 0]
-            pe = p * (E + (p * E).sum(-1, keepdim=True))
+            pe = p * (E + (p * E).sum(-1, keepdim=True)) + 2.0 ** -126 * sees
             var["out"][rq, h] = u * u * ((p * p) @ (V * V) + o * o) + tiny ** 2 * (1 + (V * V).sum(0))
             hard["out"][rq, h] = pe @ V.abs()
             hard["lse"][h, rq] = (p * E).sum(-1) + 2.0 ** -22 * (1 + z[:, 0].abs().nan_to_num(posinf=0))
@@ -71,7 +74,7 @@ def reference(q, k, v, do, q_lens, k_lens, causal, prefix, scale, cap, slopes, d
             val["dk"][rk, g] += dk
             d_delta = u * _rms(dO * o, -1)[:, None]
             # fp32: P off by E, dp and delta by 64 steps of their sums of sizes, the cap's factor by 2^-20
-            dse = pe * (dp - delta).abs() + p * 2.0 ** -24 * 72 * (dO.abs() @ V.abs().t() + (dO * o).abs().sum(-1, keepdim=True)) + ds.abs() * 2.0 ** -20 + pe * (dO.abs() * (pe @ V.abs())).sum(-1, keepdim=True)
+            dse = pe * (dp - delta).abs() + p * 2.0 ** -24 * 72 * (dO.abs() @ V.abs().t() + (dO * o).abs().sum(-1, keepdim=True)) + (ds.abs() * 2.0 ** -20 + 2.0 ** -126) + pe * (dO.abs() * (pe @ V.abs())).sum(-1, keepdim=True)
             one = p * slope * d_delta                                  # the same error for the whole row: adds up along it
             var["dv"][rk, g] += u * u * (p * p).t() @ (dO * dO) + tiny ** 2 * (dO * dO).sum(0)
             hard["dv"][rk, g] += pe.t() @ dO.abs()
@@ -355,6 +358,25 @@ def test_shared_key_heads_with_few_and_many_items(heads, dtype):
     for lens in ([200, 37], [130] * 160):
         q, k, v, do = case(lens, lens, *heads, dtype, 77)
         close(run(q, k, v, do, ops.AttnPlan(lens, causal=True)), reference(q, k, v, do, lens, lens, True, None, 0.125, 0.0, None, dtype), NAMES)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("cap,bias", [(0.0, False), (20.0, False), (0.0, True), (50.0, True)])
+@pytest.mark.parametrize("q_lens,k_lens,causal,prefix", [([200], [1605], False, None), ([1], [4101], False, None), ([1], [97], True, None), ([261], [261], True, None), ([700], [700], True, [5]),
+                                                         ([130, 1, 40], [96, 300, 0], False, None), ([500, 3], [200, 97], True, None), ([300], [193], True, [193]),
+                                                         ([130, 1, 40], [960, 1300, 0], False, None), ([500, 3], [1200, 97], True, None), ([1300], [900], True, [7]), ([900], [901], True, None)], ids=str)
+def test_few_queries_share_their_keys_among_ctas(q_lens, k_lens, causal, prefix, cap, bias, dtype):
+    """items so few that each is split along its keys, and the same ones unsplit: parts of several tiles and of none, rows that see nothing of a part or at all"""
+    ops = _ops()
+    q, k, v, do = case(q_lens, k_lens, 4, 2, dtype, 31)
+    slopes = torch.tensor([0.0, 0.01, 0.1, 0.9], device="cuda") if bias else None
+    ref = reference(q, k, v, do, q_lens, k_lens, causal, prefix, 0.125, cap, slopes, dtype)
+    plan = ops.AttnPlan(q_lens, k_lens, causal=causal, prefix=prefix)
+    assert plan.longest == max(k_lens)
+    close(run(q, k, v, do, plan, cap=cap, slopes=slopes), ref, NAMES)
+    plan.longest = 0                                              # not known: no split
+    close(run(q, k, v, do, plan, cap=cap, slopes=slopes), ref, NAMES)
 
 
 @gpu

@@ -7,7 +7,7 @@ import torch
 gpu = pytest.mark.gpu
 
 
-@pytest.mark.parametrize("stem,kernels,registers", [("kf_attn_pack", 8, 128), ("kf_attn_pack_bwd", 16, 96)])
+@pytest.mark.parametrize("stem,kernels,registers", [("kf_attn_pack", 16, 128), ("kf_attn_pack_bwd", 16, 96)])
 def test_register_splits_have_what_they_draw_on(stem, kernels, registers):
     """the packed attention's kernels hand registers from one role to another; the sum comes from what a block is launched with, and a build that
     allocates less would wait for the rest without end."""
