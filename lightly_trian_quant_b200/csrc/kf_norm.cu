@@ -426,7 +426,9 @@ static int ln_launch(const char* what, int64_t rows, size_t smem, cudaStream_t s
   const int rc = ln_grid(rows, a.W, smem, regs, grid);
   if (rc != KF_OK) return rc;
   KF_REQUIRE(ws_bytes < 0 || ws_bytes >= (int64_t)*grid * 2 * a.d * 4, "kf_layer_norm_bwd: workspace of %lld bytes, needs %lld", (long long)ws_bytes, (long long)*grid * 2 * a.d * 4);
-  return cuda_status(launch_maybe_pdl(rows, kern, dim3(*grid), dim3(LN_THREADS), smem, st, a), what);
+  // a dependent launch at any number of rows (the 1): it starts none early itself, so that only the gap between kernels closes (22 470 x 1024 both directions
+  // 84.0 -> 79.4 us, 40 009 x 333 51.4 -> 48.1)
+  return cuda_status(launch_maybe_pdl(1, kern, dim3(*grid), dim3(LN_THREADS), smem, st, a), what);
 }
 
 // f(TI, TO, CH, NC) for the types, the access width and the values per thread of a call

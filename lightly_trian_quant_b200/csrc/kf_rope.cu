@@ -133,6 +133,8 @@ using namespace kf;
 
 template <typename T, typename TP, int V>
 static int rope_launch(const RopeArgs& a, int interleaved, dim3 grid, cudaStream_t st) {
+  // dependent launches at any number of rows (the 1): the kernel starts none early itself, so that only the gap between kernels closes (51 205 x 32 x 64 bf16 both
+  // directions 147.4 -> 142.9 us)
   cudaError_t e;
   const size_t smem = (size_t)a.tokens * a.P * sizeof(float2);
   if (interleaved) {
@@ -140,10 +142,10 @@ static int rope_launch(const RopeArgs& a, int interleaved, dim3 grid, cudaStream
       set_error("kf_rope_axes: interleaved pairs need an even alignment");
       return KF_ERR_BAD_ARGUMENT;
     } else {
-      e = launch_maybe_pdl((int64_t)a.T * a.G, rope_axes_kernel<T, TP, V, true>, grid, dim3(ROPE_THREADS), smem, st, a);
+      e = launch_maybe_pdl(1, rope_axes_kernel<T, TP, V, true>, grid, dim3(ROPE_THREADS), smem, st, a);
     }
   } else {
-    e = launch_maybe_pdl((int64_t)a.T * a.G, rope_axes_kernel<T, TP, V, false>, grid, dim3(ROPE_THREADS), smem, st, a);
+    e = launch_maybe_pdl(1, rope_axes_kernel<T, TP, V, false>, grid, dim3(ROPE_THREADS), smem, st, a);
   }
   return cuda_status(e, "kf_rope_axes launch");
 }
