@@ -251,7 +251,8 @@ KF_API int kf_attn_fwd_quant(int dtype, const void* qkv, int B, int N, int H, fl
                              const float* tso, int flags, void* stream);
 
 /* Programmatic dependent launch, process-wide: KF_PDL_OFF = plain stream order, KF_PDL_ALL (and any other non-zero value) = every
- * launch, KF_PDL_AUTO (the state before the first call) = launches over few rows, where it is the faster form (kf_api.cu).
+ * launch, KF_PDL_AUTO (the state before the first call) = launches over few rows, where it is the faster form (kf_api.cu), and those of
+ * kf_layer_norm_* and kf_rope_axes over any number.
  * Results are the same in all three.
  * Counterpart: set_pdl(bool) (infer-opt/round13_mxfp8_full/impl/mx13.cu:282). */
 #define KF_PDL_OFF 0
