@@ -23,6 +23,7 @@
 //            launch takes.  Without it dQ and dK of a few queries with steep slopes were 1.53 times as far off as a single
 //            rounding of the result, now 1.4 times; it costs one product more in the first launch
 //   numerics P and dS are rounded to the 16-bit type of the operands (the products' A operand); everything else fp32
+//   measured 8 x 1605 tokens, 16 heads, bf16: first launch 165 us, second 178; issue slots 57 and 53 % busy, tensor cores 43 %, special-function unit 50 and 38 %
 #include "kf_attn.cuh"
 
 namespace kf {

