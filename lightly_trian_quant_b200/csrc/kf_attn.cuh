@@ -45,21 +45,23 @@ __device__ __forceinline__ uint32_t pack16(float a, float b, int f16) {
   return *reinterpret_cast<uint32_t*>(&h);
 }
 
-// The same with a quartic (2.7e-6): where the sums of the exponentials are an output of their own (the log-sum-exp), one more FMA per pair.
+// The same with a quartic: where the sums of the exponentials are an output of their own (the log-sum-exp), one more FMA per pair.  Its constant is 1 (minimax
+// for the others: 2.9e-6, 2.7e-6 with a free one) and t is clamped at -127: there f = 0, the polynomial is 1 and the add makes an exact 0 of it, so that a masked
+// key, -inf, weighs nothing, not 2^-126, which a value of 10^38 would show in a bf16 output.  Between -127 and -126 the add leaves a denormal number.
 __device__ __forceinline__ float2 ex2_poly2_fine(float2 t) {
-  t.x = clamp_ex2(t.x);
-  t.y = clamp_ex2(t.y);
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;\n\tmin.NaN.f32 %0, %0, 0f42FE0000;" : "+f"(t.x));   // [-127, 127]
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;\n\tmin.NaN.f32 %0, %0, 0f42FE0000;" : "+f"(t.y));
   const float2 r = add2(t, splat2(12582912.f));
   const float2 n = add2(r, splat2(-12582912.f));
   const float2 f = fma2(n, splat2(-1.f), t);
-  float2 p = fma2(f, splat2(0x1.3997d4p-7f), splat2(0x1.ca1440p-5f));
-  p = fma2(p, f, splat2(0x1.ec06dap-3f));
-  p = fma2(p, f, splat2(0x1.62e0dcp-1f));
-  p = fma2(p, f, splat2(0x1.ffffe8p-1f));
+  float2 p = fma2(f, splat2(0x1.3a02b6p-7f), splat2(0x1.c9fc74p-5f));
+  p = fma2(p, f, splat2(0x1.ec0378p-3f));
+  p = fma2(p, f, splat2(0x1.62e12cp-1f));
+  p = fma2(p, f, splat2(1.f));
   return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(r.x) << 23)), __int_as_float(__float_as_int(p.y) + (__float_as_int(r.y) << 23)));
 }
 
-// The quartic for t that is not above 0 (but for rounding): one clamp, and the power of two goes in by a multiplication, which keeps what is no number.
+// A quartic (2.7e-6) for t that is not above 0 (but for rounding): one clamp at -126, and the power of two goes in by a multiplication, which keeps what is no number.
 __device__ __forceinline__ float2 ex2_poly2_neg(float2 t) {
   asm("max.NaN.f32 %0, %0, 0fC2FC0000;\n\tmax.NaN.f32 %1, %1, 0fC2FC0000;" : "+f"(t.x), "+f"(t.y));
   const float2 r = add2(t, splat2(12582912.f));

@@ -15,7 +15,7 @@
 //   - with slopes the key tiles start at the one where the first query stands, go up to the last and then down to the first: scores mostly
 //     fall with the distance, and a maximum that rises from tile to tile sends every tile down the slow path (200 queries behind 1605
 //     keys, slope 1/16: 49 us in the keys' order)
-//   - the polynomial exponential is a degree finer, for the log-sum-exp
+//   - the polynomial exponential is a degree finer, for the log-sum-exp, and 0 for masked keys
 //   - few items over long keys (SPLIT): a cluster of up to eight CTAs takes an item, each a share of the key tiles, and joins its parts through the
 //     shared memory of its CTAs: accumulators, maxima and sums in fp32, in the order of the parts
 // Measured (16 heads, bf16 unless noted): 8 x 1605 tokens 127 us (0.66 PFLOP/s), sizes of 1 to 4101 tokens 147, a causal clip of 8197 tokens in f16 191; bound by
@@ -501,7 +501,7 @@ attn_pack_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 #pragma unroll
         for (int i = 0; i < 8; ++i) reinterpret_cast<uint4*>(part)[8 * c + i] = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
       }
-      // a part of which the row sees nothing has no maximum (what its sum holds comes from masked keys)
+      // a part of which the row sees nothing has no maximum
       const bool nothing = n_kt == 0 || (BIAS ? m_run == -INFINITY : lim <= first * PK_BN);
       reinterpret_cast<float2*>(smem + PK_OFF_ML)[row] = nothing ? make_float2(-INFINITY, 0.f) : make_float2(m_run * sc, l_run);
     }
@@ -521,7 +521,7 @@ attn_pack_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       if (lim >= 0) {
         const QTile tile = tile_of(it);
         const int h = head_of(it);
-        const bool none = lim == 0;                              // (its sum is not quite 0: the polynomial gives 2^-126 for masked keys)
+        const bool none = lim == 0;
         const float inv = 1.0f / l_run;
         uint32_t w[32];
 #pragma unroll
