@@ -337,8 +337,8 @@ attn_pack_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     for (int it = 0; it < n_my && ok; ++it) {
     // little of the record lives through the key loop: where the rows go is looked up again behind it
     int n_kt, lim, warp_lim;                                     // lim: keys this row sees (-1: no row); warp_lim: the fewest of the warp's rows that exist
-    float slope = 0.f, at = 0.f;
-    int start;
+    float slope = 0.f;
+    int start, at = 0;                                           // at: the row's position
     {
       const QTile tile = tile_of(it);
       n_kt = key_tiles(tile);
@@ -347,13 +347,13 @@ attn_pack_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       start = start_of(tile, n_kt);
       if constexpr (BIAS) {
         slope = __ldg(a.slopes + head_of(it)) * 1.4426950408889634f;
-        at = (float)(tile.pos + row);
+        at = tile.pos + row;
       }
     }
     // raw products -> logits in units of the exponent, then the keys that the row does not see
     auto logits = [&](uint32_t (&r)[32], int key0) {
       if constexpr (!RAW) {
-        const float gap = at - (float)key0;
+        const float gap = (float)(at - key0);                    // behind 2^24 only the difference is a number that fp32 holds
         bool flat = false;
         if constexpr (CAP) {
           float m4[4] = {0.f, 0.f, 0.f, 0.f};

@@ -392,15 +392,15 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
       float2 vsum = make_float2(0.f, 0.f);                       // ROWS = queries: sum of P (dP - delta) over this thread's columns
       // ROWS = queries: the row sees columns below `edge`; ROWS = keys: from `edge` on
       int edge, warp_edge;
-      float at;                                                  // ROWS = queries: position; ROWS = keys: the query that stands at the key
+      int at;                                                    // ROWS = queries: position; ROWS = keys: the query that stands at the key
       if constexpr (KEYS) {
         edge = row < I.rows() ? I.t.lowest(row) : 0;
         warp_edge = I.t.lowest((warp & 3) * 32 + 31);            // the largest of the warp's
-        at = (float)(I.t.first + row - I.t.off);
+        at = I.t.first + row - I.t.off;
       } else {
         edge = row < I.rows() ? I.t.limit(row) : 0x7fffffff;
         warp_edge = I.t.limit((warp & 3) * 32);
-        at = (float)(I.t.pos + row);
+        at = I.t.pos + row;
       }
       float slope = 0.f;
       if (BIAS && !KEYS) slope = __ldg(a.slopes + I.head) * 1.4426950408889634f;
@@ -439,7 +439,7 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
         }
         const float* stat = reinterpret_cast<const float*>(smem + PB_OFF_STAT + st * 1024) + c0;
         if (KEYS && !mbar_wait_warp(&st_full[st], st_ph, ctx, 71)) { ok = false; break; }
-        const float gap = at - (float)index;
+        const float gap = (float)(at - index);                   // (only the difference fits fp32 behind 2^24)
         bool flat = false;
         if constexpr (CAP) {
           float m4[4] = {0.f, 0.f, 0.f, 0.f};

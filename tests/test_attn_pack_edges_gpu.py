@@ -1,5 +1,7 @@
 """Packed attention at the edges of its range: saturated caps, masked keys of any size, positions behind 2^24, probabilities below f16's normal range,
 gradients that nobody asks for."""
+import math
+
 import pytest
 import torch
 
@@ -42,3 +44,49 @@ def test_masked_keys_have_no_part_in_a_row(q_lens, k_lens, huge, cap, bias, dtyp
                     assert torch.equal(got[q0 + i], want[q0 + i]), (q0 + i, (got[q0 + i].float() - want[q0 + i].float()).abs().max())
             q0, k0 = q0 + lq, k0 + lk
         assert rows
+
+
+# ------------------------------------------------------------------------------------------------ far positions
+@gpu
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("split", [True, False])
+def test_distances_behind_position_two_to_the_24(split, causal):
+    """a sequence of more than 2^24 keys: the distance of neighbours is a small number there too.  Keys but the last 200 are zero, the slope is steep, so that a float64 sum
+    over the last 2048 keys is all of it (e^-900 is left out).  Tolerance: scores up to 8 and slopes times distances in fp32, 1e-5 of a probability; u = 2^-8 of each
+    term for P or dS and of the result, 3.5 standard deviations as everywhere in these tests."""
+    ops = _ops()
+    Lq, Lk, near, slope, u = 3, 2 ** 24 + 5, 2048, 0.5, 2.0 ** -8
+    g = torch.Generator(device="cuda").manual_seed(6)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda").to(BF)  # noqa: E731
+    q, do = r(Lq, 1, 64), r(Lq, 1, 64)
+    k, v = torch.zeros(Lk, 1, 64, dtype=BF, device="cuda"), torch.zeros(Lk, 1, 64, dtype=BF, device="cuda")
+    k[-200:], v[-200:] = r(200, 1, 64), r(200, 1, 64)
+    slopes = torch.tensor([slope], device="cuda")
+    plan = ops.AttnPlan([Lq], [Lk], causal=causal)
+    if not split:
+        plan.longest = 0
+    out, lse = ops.attn_packed(q, k, v, plan, slopes=slopes)
+    dq, dk, dv = ops.attn_packed_bwd(do, q, k, v, out, lse, plan, slopes=slopes)
+    ops.check_device_error()
+    assert not dk[:-near].any() and not dv[:-near].any()
+    Q, K, V, dO = q[:, 0].double(), k[-near:, 0].double(), v[-near:, 0].double(), do[:, 0].double()
+    at, key = torch.arange(Lk - Lq, Lk, device="cuda")[:, None], torch.arange(Lk - near, Lk, device="cuda")[None]
+    s = Q @ K.t() * 0.125 - slope * (at - key).abs()
+    if causal:
+        s = s.masked_fill(key > at, -math.inf)
+    z = torch.logsumexp(s, -1, keepdim=True)
+    p = torch.exp(s - z)
+    o = p @ V
+    dp, delta = dO @ V.t(), (dO * o).sum(-1, keepdim=True)
+    ds = p * (dp - delta)
+    size = p * (dp.abs() + (dO * o).abs().sum(-1, keepdim=True))
+    row = p * (u * (dO * o).square().sum(-1, keepdim=True).sqrt())
+    assert (lse[0].double() - z[:, 0]).abs().max() <= 1e-5
+    checks = {"out": (out, o, (u * p) ** 2 @ V ** 2, 1e-5 * p @ V.abs()),
+              "dq": (dq, ds @ K / 8, (u / 8) ** 2 * (ds ** 2 @ K ** 2) + (row @ K / 8) ** 2, 2e-5 * (size @ K.abs()) / 8),
+              "dk": (dk[-near:], ds.t() @ Q / 8, (u / 8) ** 2 * ((ds ** 2).t() @ Q ** 2) + (row ** 2).t() @ Q ** 2 / 64, 2e-5 * (size.t() @ Q.abs()) / 8),
+              "dv": (dv[-near:], p.t() @ dO, (u * p.t()) ** 2 @ dO ** 2, 1e-5 * p.t() @ dO.abs())}
+    for name, (got, want, var, hard) in checks.items():
+        bound = 3.5 * (var + u * u * want ** 2).sqrt() + hard + 2.0 ** -118
+        worst = ((got[:, 0].double() - want).abs() / bound).max().item()
+        assert worst <= 1, (name, worst)
