@@ -61,7 +61,7 @@ __device__ __forceinline__ float2 ex2_poly2_fine(float2 t) {
   return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(r.x) << 23)), __int_as_float(__float_as_int(p.y) + (__float_as_int(r.y) << 23)));
 }
 
-// A quartic (2.7e-6) for t that is not above 0 (but for rounding): one clamp at -126, and the power of two goes in by a multiplication, which keeps what is no number.
+// A quartic (2.7e-6) for t that stays below 127: one clamp at -126, and the power of two goes in by a multiplication, which keeps what is no number.
 __device__ __forceinline__ float2 ex2_poly2_neg(float2 t) {
   asm("max.NaN.f32 %0, %0, 0fC2FC0000;\n\tmax.NaN.f32 %1, %1, 0fC2FC0000;" : "+f"(t.x), "+f"(t.y));
   const float2 r = add2(t, splat2(12582912.f));

@@ -22,7 +22,9 @@
 //            much delta is off, and dQ is put right by that times the product P K (which dQ's error is), as is the delta that the second
 //            launch takes.  Without it dQ and dK of a few queries with steep slopes were 1.53 times as far off as a single
 //            rounding of the result, now 1.4 times; it costs one product more in the first launch
-//   numerics P and dS are rounded to the 16-bit type of the operands (the products' A operand); everything else fp32
+//   numerics P and dS are rounded to the 16-bit type of the operands (the products' A operand); everything else fp32.  With f16 P is 2^14 times what it is, by the
+//            exponent's offset: probabilities of long rows lie below f16's normal range (at 818 401 keys dV was 2.4 % off, the same way in every row).  Delta and dP take
+//            the power of two back in front of dS, by the multiplication that was an addition; dV and the product P K at the end.
 //   measured 8 x 1605 tokens, 16 heads, bf16: first launch 165 us, second 178; issue slots 57 and 53 % busy, tensor cores 43 %, special-function unit 50 and 38 %
 #include "kf_attn.cuh"
 
@@ -49,6 +51,10 @@ static_assert(PB_COL_A2 + PB_D <= PB_TMEM_COLS, "TMEM budget");
 // first launch none / one / two of eight 166.8 / 164.4 / 165.3 us, with a cap (fewer tokens) 69.1 / 72.9 / 74.8, second launch none / one / two 191 / 194 / 201
 __host__ __device__ constexpr int bwd_poly(bool keys, bool cap) { return keys || cap ? 0 : 0x80; }
 
+// P is computed 2^shift times as large
+__host__ __device__ constexpr int bwd_shift(int f16) { return f16 ? 14 : 0; }
+__host__ __device__ constexpr float bwd_unshift(int f16) { return f16 ? 0x1p-14f : 1.f; }
+
 struct PackBwdArgs {
   const int4* tiles;
   int n_items, heads, share;     // heads of the items: query heads (ROWS = queries), key heads times `split`
@@ -57,7 +63,7 @@ struct PackBwdArgs {
   float scale, scale_log2;
   Cap cap;
   const float* slopes;
-  float *lse2, *delta;           // -lse * log2(e) (-inf: no row, or one that sees nothing) and -delta: [Hq][n_q_tiles * 128], a sequence's rows from its first tile's slot on
+  float *lse2, *delta;           // shift - lse * log2(e) (-inf: no row, or one that sees nothing) and -delta / 2^shift: [Hq][n_q_tiles * 128], a sequence's rows from its first tile's slot on
   int64_t stat_ld;
   // ROWS = queries
   const float* lse;
@@ -126,6 +132,7 @@ __global__ void __launch_bounds__(PB_THREADS, 1)
 attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constant__ CUtensorMap tmR2, const __grid_constant__ CUtensorMap tmR3,
                      const __grid_constant__ CUtensorMap tmC1, const __grid_constant__ CUtensorMap tmC2, const __grid_constant__ PackBwdArgs a) {
   using Mem = BwdMem<KEYS>;
+  constexpr float UNSHIFT = bwd_unshift(F16);
   constexpr int PB_RING = Mem::RING, RTILES = Mem::RTILES, PB_OFF_C = Mem::OFF_C, PB_OFF_STAT = Mem::OFF_STAT, PB_OFF_BAR = Mem::OFF_BAR;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + PB_OFF_BAR);
@@ -380,9 +387,9 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
           }
           __syncwarp();
           if (lane == 0) mbar_arrive(&r_empty[ri & 1]);
-          if (row < I.rows()) ndelta = -(s.x + s.y);
+          if (row < I.rows()) ndelta = -(s.x + s.y) * UNSHIFT;
         }
-        nlse2 = nlse2 == -INFINITY ? -INFINITY : nlse2 * -1.4426950408889634f;
+        nlse2 = nlse2 == -INFINITY ? -INFINITY : fmaf(nlse2, -1.4426950408889634f, (float)bwd_shift(F16));
         if (warp < 4) {
           const int64_t o = I.head * a.stat_ld + (int64_t)I.slot() * PB_T + row;
           a.lse2[o] = nlse2;
@@ -508,7 +515,8 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
             if (KEYS && i % 4 == 0) *reinterpret_cast<float4*>(u) = *reinterpret_cast<const float4*>(stat + 128 + 16 * q + i);
             const float2 m = KEYS ? make_float2(u[i % 4], u[i % 4 + 1]) : splat2(ndelta);
             const float2 pp = make_float2(__uint_as_float(p[q][i]), __uint_as_float(p[q][i + 1]));
-            float2 v = mul2(add2(make_float2(__uint_as_float(d[i]), __uint_as_float(d[i + 1])), m), pp), g = pp;
+            const float2 dp = make_float2(__uint_as_float(d[i]), __uint_as_float(d[i + 1]));
+            float2 v = mul2(F16 ? fma2(dp, splat2(UNSHIFT), m) : add2(dp, m), pp), g = pp;
             if constexpr (!KEYS) vsum = add2(vsum, v);
             if constexpr (CAP) {
               const float2 b = make_float2(__uint_as_float(f[i]), __uint_as_float(f[i + 1]));
@@ -557,12 +565,13 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
       constexpr int PIECES = KEYS ? 2 : 1;
       uint32_t w[PIECES][16];
       const uint32_t t_a = t_lane + PB_COL_A1 + half * (32 * PIECES);
-      const float scale = KEYS && half ? 1.f : a.scale;
+      const float scale = KEYS && half ? UNSHIFT : a.scale;
       float gap_d = 0.f;                                         // delta as it was used less what it should have been
       if (!KEYS && n > 0) {
         if (!mbar_wait_warp(rs_bar, rs_ph, ctx, 74)) { ok = false; break; }
         gap_d = -((rs[0] + rs[PB_T]) + (rs[2 * PB_T] + rs[3 * PB_T]));
-        if (half == 0) a.delta[I.head * a.stat_ld + (int64_t)I.slot() * PB_T + row] = row < I.rows() ? ndelta + gap_d : 0.f;
+        if (half == 0) a.delta[I.head * a.stat_ld + (int64_t)I.slot() * PB_T + row] = row < I.rows() ? fmaf(gap_d, UNSHIFT, ndelta) : 0.f;
+        gap_d *= UNSHIFT;                                        // for the product P K
       }
 #pragma unroll
       for (int i = 0; i < PIECES; ++i) {
@@ -657,7 +666,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) bwd_join_kernel(const __grid_con
         s[4] += v[k].x; s[5] += v[k].y; s[6] += v[k].z; s[7] += v[k].w;
       }
   }
-  const float f = which ? 1.f : a.scale;
+  const float f = which ? bwd_unshift(F16) : a.scale;
   uint32_t w[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) w[k] = pack16(s[2 * k] * f, s[2 * k + 1] * f, F16);

@@ -90,3 +90,27 @@ def test_distances_behind_position_two_to_the_24(split, causal):
         bound = 3.5 * (var + u * u * want ** 2).sqrt() + hard + 2.0 ** -118
         worst = ((got[:, 0].double() - want).abs() / bound).max().item()
         assert worst <= 1, (name, worst)
+
+
+# ------------------------------------------------------------------------------------------------ small probabilities in f16
+@gpu
+@pytest.mark.parametrize("heads", [(1, 1), (2, 1)])
+@pytest.mark.parametrize("Lk", [818401, 65537])
+def test_f16_gradients_of_values_over_many_keys(Lk, heads):
+    """q = 0: every probability is 1 / Lk, and dv the sum of dout over it.  Below 2^-14 an f16 probability would lose its digits (at 818 401 keys it is 20.5 steps of
+    2^-24), the same ones in every row, so that they do not cancel.  Tolerance: P rounded once by u = 2^-11 in every row alike, the result once; 1e-5 for the exponent
+    (log-sum-exp 13.6 in fp32 and its product with log2(e), 2^-21 each, and the exponentials' 4e-6)."""
+    ops = _ops()
+    Hq, Hk = heads
+    Lq, u = 100, 2.0 ** -11
+    q = torch.zeros(Lq, Hq, 64, dtype=F16, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(8)
+    k = torch.randn(Lk, Hk, 64, generator=g, device="cuda").to(F16)
+    do = (1 + torch.rand(Lq, Hq, 64, generator=g, device="cuda")).to(F16)
+    plan = ops.AttnPlan([Lq], [Lk])
+    out, lse = ops.attn_packed(q, k, k, plan)
+    dq, dk, dv = ops.attn_packed_bwd(do, q, k, k, out, lse, plan)
+    ops.check_device_error()
+    want = do.double().view(Lq, Hk, Hq // Hk, 64).sum((0, 2)) / Lk
+    assert ((dv.double() - want).abs() <= (2 * u + 1e-5) * want + 2.0 ** -25).all(), ((dv.double() / want - 1).abs().max().item())
+    assert not dk.any() and torch.isfinite(dq).all()
