@@ -333,7 +333,7 @@ typedef struct kf_heads {
 typedef struct kf_attn_pack_params {
   int dtype, Hq, Hk, n_q_tiles, n_k_tiles;
   int longest;             /* the most keys that a record of q_tiles sees, 0 if not known: then few records are not split along their keys */
-  float scale, cap;        /* scale > 0; cap 0 = none                                                  */
+  float scale, cap;        /* scale > 0; cap 0 = none, else a normal number with 2 * scale * log2(e) / cap finite */
   int64_t Tq, Tk;
   const int32_t *q_tiles, *k_tiles;
   const float* slopes;     /* fp32 [Hq] or NULL                                                        */

@@ -936,7 +936,9 @@ Pack pack_operands(PyObject* const* v, const char* op) {
   p.n_k_tiles = (int)kt.size(0);
   p.longest = (int)to_int(v[7]);
   p.scale = (float)to_float(v[8]);
-  p.cap = (float)to_float(v[9]);
+  const double cap = to_float(v[9]);
+  p.cap = (float)cap;
+  if (cap > 0 && p.cap == 0.f) fail("%s: the cap is 0 in fp32", op);
   p.Tq = q.size(0);
   p.Tk = c.k.size(0);
   p.q_tiles = qt.data_ptr<int>();

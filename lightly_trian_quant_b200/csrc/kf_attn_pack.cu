@@ -20,6 +20,7 @@
 //     shared memory of its CTAs: accumulators, maxima and sums in fp32, in the order of the parts
 // Measured (16 heads, bf16 unless noted): 8 x 1605 tokens 127 us (0.66 PFLOP/s), sizes of 1 to 4101 tokens 147, a causal clip of 8197 tokens in f16 191; bound by
 // the softmax' instructions, two warps per scheduler
+#include <cfloat>
 #include <type_traits>
 
 #include "kf_attn.cuh"
@@ -656,6 +657,8 @@ int check_pack(const kf_attn_pack_params* p) {
   KF_REQUIRE(p->n_q_tiles >= 0 && p->n_k_tiles >= 0 && (int64_t)p->n_q_tiles * p->Hq < (1ll << 30) && (int64_t)p->n_k_tiles * p->Hk < (1ll << 30),
              "kf_attn_pack: too many (tile, head) items");
   KF_REQUIRE(p->scale > 0.f && p->scale < 1e30f && p->cap >= 0.f && p->cap < 1e30f, "kf_attn_pack: scale must be positive and cap not negative, both finite");
+  // what Cap::set makes of them: fp32 numbers with all their digits (an infinity would meet scores of 0)
+  KF_REQUIRE(p->cap == 0.f || (p->cap >= FLT_MIN && 2.9 * p->scale / p->cap < FLT_MAX), "kf_attn_pack: cap %g with scale %g leaves fp32's range", p->cap, p->scale);
   return KF_OK;
 }
 

@@ -114,3 +114,35 @@ def test_f16_gradients_of_values_over_many_keys(Lk, heads):
     want = do.double().view(Lq, Hk, Hq // Hk, 64).sum((0, 2)) / Lk
     assert ((dv.double() - want).abs() <= (2 * u + 1e-5) * want + 2.0 ** -25).all(), ((dv.double() / want - 1).abs().max().item())
     assert not dk.any() and torch.isfinite(dq).all()
+
+
+# ------------------------------------------------------------------------------------------------ caps that fp32 cannot hold
+def test_caps_out_of_fp32s_range_are_refused_by_the_library():
+    """a cap below fp32's normal range, or one whose scale leaves it, makes infinities of factors that meet zeros"""
+    from lightly_trian_quant_b200 import _lib
+
+    L, H = _lib.lib(), _lib.Heads
+    for cap, scale in ((1e-40, 0.125), (1e-38, 0.125), (1e-20, 1e25), (1e-36, 1e3)):
+        p = _lib.AttnPackParams()
+        p.dtype, p.Hq, p.Hk, p.n_q_tiles, p.n_k_tiles, p.scale, p.cap, p.Tq, p.Tk = 1, 4, 2, 1, 1, scale, cap, 40, 40
+        p.q_tiles = p.k_tiles = p.lse = p.ws = 4096                     # never dereferenced: the calls end on the host
+        p.ws_bytes = 1 << 20
+        for n in ("q", "k", "v", "o", "dout", "dq", "dk", "dv"):
+            setattr(p, n, H(4096, 256, 64))
+        for call in (L.kf_attn_pack_fwd, L.kf_attn_pack_bwd):
+            assert call(p, None) == -1 and "cap" in L.kf_last_error_string().decode(), (cap, scale, L.kf_last_error_string())
+
+
+@gpu
+def test_caps_that_vanish_in_fp32_are_refused():
+    """1e-50 is 0 in fp32, which means no cap: the opposite of what was asked for"""
+    ops = _ops()
+    q = torch.randn(8, 1, 64, device="cuda").to(BF)
+    plan = ops.AttnPlan([8])
+    out, lse = ops.attn_packed(q, q, q, plan)
+    for cap in (1e-50, 1e-300, 1e-40):
+        with pytest.raises(ops.KfError, match="cap"):
+            ops.attn_packed(q, q, q, plan, cap=cap)
+        with pytest.raises(ops.KfError, match="cap"):
+            ops.attn_packed_bwd(q, q, q, q, out, lse, plan, cap=cap)
+    ops.check_device_error()
