@@ -469,8 +469,14 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
               float2 l = KEYS ? make_float2(v[2 * k], v[2 * k + 1]) : splat2(nlse2);
               float2 x = make_float2(__uint_as_float(p[c / 16][c % 16]), __uint_as_float(p[c / 16][c % 16 + 1]));
               if constexpr (CAP) {
-                x = decltype(small)::value ? cap_flat(a.cap, x) : cap_any(a.cap, x);
-                const float2 y = mul2(x, splat2(a.cap.inv_out)), d = fma2(make_float2(-y.x, -y.y), y, splat2(1.f));
+                float2 d;
+                if constexpr (decltype(small)::value) {            // |y| <= 1/2
+                  x = cap_flat(a.cap, x);
+                  const float2 y = mul2(x, splat2(a.cap.inv_out));
+                  d = fma2(make_float2(-y.x, -y.y), y, splat2(1.f));
+                } else {
+                  x = cap_any(a.cap, x, d);
+                }
                 f[2 * k] = __float_as_uint(d.x);
                 f[2 * k + 1] = __float_as_uint(d.y);
               } else if constexpr (BIAS) {

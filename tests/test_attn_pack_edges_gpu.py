@@ -146,3 +146,60 @@ def test_caps_that_vanish_in_fp32_are_refused():
         with pytest.raises(ops.KfError, match="cap"):
             ops.attn_packed_bwd(q, q, q, q, out, lse, plan, cap=cap)
     ops.check_device_error()
+
+
+# ------------------------------------------------------------------------------------------------ saturated caps
+@gpu
+@pytest.mark.parametrize("heads", [(1, 1), (2, 1)])
+@pytest.mark.parametrize("cap", [1.5, 30.0])
+@pytest.mark.parametrize("lo,hi", [(7.0, 9.0), (0.4, 9.0)])
+def test_gradients_at_saturated_scores(lo, hi, cap, heads):
+    """queries and keys whose capped scores lie at lo to hi times the cap: their gradients are the small 1 - tanh^2 = 4 e / (1 + e)^2, e = exp(-2y), which has to
+    come out with its own digits, not with those of 1.
+
+    Scores are products of one channel with few digits each, so that they are exact; the other channels of q meet zeros of k and the other way round, and carry the
+    gradients.  Tolerance in bf16, u = 2^-8: dS and the result are rounded once (standard deviation u / sqrt(3), six of them: 3.5 u sqrt(sum of squares)), delta
+    takes the rounded output, for a whole row.  fp32: t = 2 y log2(e) <= 26 is off by two roundings, so e by 26 * 2^-23 * ln 2 = 2.2e-6 of itself; exponential 2^-22, reciprocal
+    2^-23 twice, three products 2^-24; P from a capped score off by 2^-22 cap and its log-sum-exp the same, so 2 * 2^-22 * 30 = 1.4e-5 of itself at cap 30: 2e-5 of every term
+    in all, with the sizes of dP and delta in place of their difference."""
+    ops = _ops()
+    Hq, Hk = heads
+    n, scale, u = 96, 0.125, 2.0 ** -8
+    g = torch.Generator().manual_seed(int(hi + 100 * lo))
+    q, k = torch.zeros(n, Hq, 64), torch.zeros(n, Hk, 64)
+    k[..., 0] = torch.where(torch.rand(n, Hk, generator=g) < 0.5, -1.0, 1.0)
+    q[..., 0] = torch.empty(n, Hq).uniform_(lo, hi, generator=g) * cap / scale
+    q[..., 1:32] = torch.randn(n, Hq, 31, generator=g)
+    k[..., 32:] = torch.randn(n, Hk, 32, generator=g)
+    q, k = q.to(BF), k.to(BF)
+    v, do = torch.randn(n, Hk, 64, generator=g).to(BF), torch.randn(n, Hq, 64, generator=g).to(BF)
+    plan = ops.AttnPlan([n])
+    qc, kc, vc, dc = (t.cuda() for t in (q, k, v, do))
+    out, lse = ops.attn_packed(qc, kc, vc, plan, scale=scale, cap=cap)
+    dq, dk, dv = ops.attn_packed_bwd(dc, qc, kc, vc, out, lse, plan, scale=scale, cap=cap)
+    ops.check_device_error()
+    q, k, v, do = (t.double() for t in (q, k, v, do))
+    dk_want, dk_var, dk_hard = torch.zeros_like(k), torch.zeros_like(k), torch.zeros_like(k)
+    for h in range(Hq):
+        gk = h * Hk // Hq
+        Q, K, V, dO = q[:, h], k[:, gk], v[:, gk], do[:, h]
+        y = Q @ K.t() * scale / cap
+        e = torch.exp(-2 * y.abs())
+        factor = 4 * e / (1 + e) ** 2
+        p = torch.softmax(cap * torch.tanh(y), -1)
+        o = p @ V
+        dp, delta = dO @ V.t(), (dO * o).sum(-1, keepdim=True)
+        ds = p * (dp - delta) * factor
+        size = p * factor * (dp.abs() + (dO * o).abs().sum(-1, keepdim=True))
+        row = p * factor * (u * (dO * o).square().sum(-1, keepdim=True).sqrt())
+        value = ds @ K * scale
+        bound = 3.5 * ((u * scale) ** 2 * (ds ** 2 @ K ** 2) + (scale * row @ K) ** 2 + u * u * value ** 2).sqrt() + 2e-5 * scale * (size @ K.abs()) + 2.0 ** -120
+        worst = ((dq[:, h].cpu().double() - value).abs() / bound).max().item()
+        assert worst <= 1, ("dq", h, worst)
+        dk_want[:, gk] += ds.t() @ Q * scale
+        dk_var[:, gk] += scale ** 2 * (u * u * (ds ** 2).t() @ Q ** 2 + (row ** 2).t() @ Q ** 2)
+        dk_hard[:, gk] += 2e-5 * scale * (size.t() @ Q.abs())
+    bound = 3.5 * (dk_var + u * u * dk_want ** 2).sqrt() + dk_hard + 2.0 ** -120
+    worst = ((dk.cpu().double() - dk_want).abs() / bound).max().item()
+    assert worst <= 1, ("dk", worst)
+    assert torch.isfinite(dv).all()
