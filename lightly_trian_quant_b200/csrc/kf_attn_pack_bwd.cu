@@ -371,7 +371,7 @@ attn_pack_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_cons
       // ROWS = queries: the row's log-sum-exp and delta (negated: they are added), also for the second launch
       float nlse2 = 0.f, ndelta = 0.f;
       if constexpr (!KEYS) {
-        nlse2 = row < I.rows() ? __ldg(a.lse + (int64_t)I.head * a.lse_ld + I.row0() + row) : -INFINITY;
+        nlse2 = row < I.rows() ? a.lse[(int64_t)I.head * a.lse_ld + I.row0() + row] : -INFINITY;
         if (n > 0) {
           if (!mbar_wait_warp(&r_full[ri & 1], (ri >> 1) & 1, ctx, 65)) break;
           const uint8_t* d = smem + ((ri & 1) * RTILES + 1) * PB_RTILE + row * 128;
@@ -662,8 +662,8 @@ __global__ void __launch_bounds__(JOIN_THREADS) bwd_join_kernel(const __grid_con
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k)
       if (k0 + k < a.split) {
-        u[k] = __ldg(p + (int64_t)(k0 + k) * PART);
-        v[k] = __ldg(p + (int64_t)(k0 + k) * PART + 1);
+        u[k] = p[(int64_t)(k0 + k) * PART];
+        v[k] = p[(int64_t)(k0 + k) * PART + 1];
       }
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k)

@@ -277,12 +277,12 @@ __global__ void __launch_bounds__(LN_THREADS) layer_norm_bwd_kernel(const __grid
     for (int j = 0; j < CH; ++j) aw[i][j] = ab[i][j] = 0.f;
   }
   int k = 0;
-  float mean = first < a.rows ? __ldg(a.mean + first) : 0.f, rstd = first < a.rows ? __ldg(a.rstd + first) : 0.f;
+  float mean = first < a.rows ? a.mean[first] : 0.f, rstd = first < a.rows ? a.rstd[first] : 0.f;
   for (int64_t row = first; row < a.rows; row += stride, ++k) {
     const int slot = k % LN_RING;
     if (a.W == 1) request(row + stride, (k + 1) % LN_RING);
     const bool more = row + stride < a.rows;
-    const float next_mean = more ? __ldg(a.mean + row + stride) : 0.f, next_rstd = more ? __ldg(a.rstd + row + stride) : 0.f;
+    const float next_mean = more ? a.mean[row + stride] : 0.f, next_rstd = more ? a.rstd[row + stride] : 0.f;
     ok = mbar_wait_warp(&bars[group][slot], (k / LN_RING) & 1, ctx, 81) && ok;
     const uint8_t* from = ring + slot * slot_bytes;
     const TI* x = ln_row_at(from, x0 + row * a.ldx) + at.first;
@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(LN_THREADS) layer_norm_bwd_kernel(const __grid
 }
 
 // dw, db = the sum of `n` lines [2][d]: 32 columns per CTA, 32 threads per column
-__global__ void __launch_bounds__(1024) layer_norm_cols_kernel(const float* __restrict__ part, int n, int d, float* __restrict__ dw, float* __restrict__ db) {
+__global__ void __launch_bounds__(1024) layer_norm_cols_kernel(const float* part, int n, int d, float* dw, float* db) {
   __shared__ float sm[32][33];
   pdl_wait();
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;

@@ -1,0 +1,19 @@
+"""Rules of the kernels for training that a run cannot show without failing on the GPU, read from their sources."""
+import re
+from pathlib import Path
+
+CSRC = Path(__file__).resolve().parent.parent / "lightly_trian_quant_b200" / "csrc"
+SOURCES = ("kf_norm.cu", "kf_rope.cu", "kf_attn_pack.cu", "kf_attn_pack_bwd.cu", "kf_attn.cuh")
+
+
+def _code(name):
+    return re.sub(r"//[^\n]*", "", (CSRC / name).read_text())
+
+
+def test_read_only_loads_are_of_what_no_kernel_writes():
+    """dependent launches may be resident while the kernel before them still writes its results, which the read-only path (__ldg, const __restrict__) does not allow for: it
+    is for the plan's tables and the slopes, which the host makes."""
+    for name in SOURCES:
+        loads = re.findall(r"__ldg\(\s*([\w.]+)", _code(name))
+        assert set(loads) <= {"a.slopes", "tiles"}, (name, loads)
+        assert "__restrict__" not in _code(name), name
