@@ -203,3 +203,36 @@ def test_gradients_at_saturated_scores(lo, hi, cap, heads):
     worst = ((dk.cpu().double() - dk_want).abs() / bound).max().item()
     assert worst <= 1, ("dk", worst)
     assert torch.isfinite(dv).all()
+
+
+# ------------------------------------------------------------------------------------------------ dependent launches
+@gpu
+@pytest.mark.parametrize("mode", [True, False, None])
+def test_a_chain_of_the_operators_in_every_launch_mode(mode):
+    """both directions of all operators behind one another, short ones, so that each is there while the one before it still runs: the same bits in every mode"""
+    ops = _ops()
+    g = torch.Generator(device="cuda").manual_seed(12)
+    lens, H, Hk = [70, 1, 130], 6, 2
+    T, d = sum(lens), (H + 2 * Hk) * 64
+    x, w = torch.randn(T, d, generator=g, device="cuda"), 1 + 0.1 * torch.randn(d, generator=g, device="cuda")
+    do = torch.randn(T, H, 64, generator=g, device="cuda").to(BF)
+    pos, table = torch.arange(2 * T, device="cuda").view(T, 2).int(), ops.RopeTable([[1.0, 0.1], [0.5]], 64)
+    plan = ops.AttnPlan(lens, causal=True)
+
+    def step():
+        y, mean, rstd = ops.layer_norm_fwd(x, w, w, 1e-5, BF)
+        qkv = y.view(T, H + 2 * Hk, 64)
+        turned = ops.rope_axes(qkv, pos, table)
+        q, k, v = turned[:, :H], turned[:, H:H + Hk], qkv[:, H + Hk:]
+        out, lse = ops.attn_packed(q, k, v, plan, cap=20.0)
+        gq = torch.empty_like(qkv)
+        ops.attn_packed_bwd(do, q, k, v, out, lse, plan, cap=20.0, grads=(gq[:, :H], gq[:, H:H + Hk], gq[:, H + Hk:]))
+        ops.rope_axes(gq[:, :H + Hk], pos, table, inverse=True, out=gq[:, :H + Hk])
+        return (out, lse, gq, *ops.layer_norm_bwd(gq.view(T, d), x, w, mean, rstd, dres=x))
+
+    ops.set_pdl(False)
+    want = step()
+    ops.set_pdl(mode)
+    for _ in range(20):
+        assert all(torch.equal(a, b) for a, b in zip(step(), want))
+    ops.check_device_error()
