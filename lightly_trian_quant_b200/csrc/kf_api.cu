@@ -42,6 +42,22 @@ bool pdl_for(int64_t rows, cudaStream_t st) {
   return cudaStreamIsCapturing(st, &cap) == cudaSuccess && cap == cudaStreamCaptureStatusNone;
 }
 
+int split_ready(const void* kernel, PerDevice<bool>& ready, int regs_per_thread, size_t smem, const char* what) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (ready.get(dev)) return KF_OK;
+  cudaFuncAttributes attr;
+  cudaError_t e = cudaFuncGetAttributes(&attr, kernel);
+  if (e == cudaSuccess && attr.numRegs < regs_per_thread) {
+    set_error("%s: the kernel was built with %d registers per thread, its roles need %d", what, attr.numRegs, regs_per_thread);
+    return KF_ERR_UNSUPPORTED;
+  }
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return cuda_status(e, what);
+  ready.put(dev, true);
+  return KF_OK;
+}
+
 __device__ unsigned int g_dev_error[4];
 
 unsigned int* dev_error_ptr() {

@@ -601,15 +601,9 @@ static int attn_launch(int dtype, const void* qkv, void* O, int B, int N, int H,
       {attn_fwd_kernel<1, -1>, attn_fwd_kernel<1, KF_FMT_MX8>, attn_fwd_kernel<1, KF_FMT_NV4>, attn_fwd_kernel<1, KF_FMT_MX4>}};
   const int oi = out_fmt < 0 ? 0 : out_fmt == KF_FMT_MX8 ? 1 : out_fmt == KF_FMT_NV4 ? 2 : 3;
   const KernelFn kern = table[dtype == KF_F16 ? 1 : 0][oi];
-  static PerDevice<bool> attr_set[2][4];
-  int dev = 0;
-  cudaGetDevice(&dev);
-  PerDevice<bool>& ready = attr_set[dtype == KF_F16 ? 1 : 0][oi];
-  if (!ready.get(dev)) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)AT_SMEM);
-    if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(attn_fwd_kernel)");
-    ready.put(dev, true);
-  }
+  static PerDevice<bool> ready[2][4];
+  const int rst = split_ready(reinterpret_cast<const void*>(kern), ready[dtype == KF_F16 ? 1 : 0][oi], split_regs(128, AT_REGS_SOFTMAX, 128, AT_REGS_LEAN), AT_SMEM, "kf_attn_fwd");
+  if (rst != KF_OK) return rst;
   AttnArgs a{};
   a.O = O; a.B = B; a.N = N; a.H = H; a.f16 = dtype == KF_F16;
   a.scale_log2 = 0.125f * 1.4426950408889634f;

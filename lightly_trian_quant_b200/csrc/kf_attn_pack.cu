@@ -30,7 +30,8 @@ namespace kf {
 
 constexpr int PK_BM = 128, PK_BN = 96, PK_D = 64;
 constexpr int PK_THREADS = 256;                        // warps 0..3 softmax, 4 TMA, 5 MMA issuer, 6 and 7 idle
-constexpr int PK_REGS_SOFTMAX = 208, PK_REGS_LEAN = 48; // 128 * 208 + 128 * 48 <= 256 * 128, the allocation at launch
+constexpr int PK_REGS_SOFTMAX = 208, PK_REGS_LEAN = 48, PK_REGS = split_regs(128, PK_REGS_SOFTMAX, 128, PK_REGS_LEAN);
+static_assert(2 * PK_THREADS * PK_REGS <= 65536, "two CTAs per SM");
 constexpr int PK_KV = 3;
 constexpr int PK_QTILE = PK_BM * PK_D * 2, PK_KTILE = PK_BN * PK_D * 2;
 constexpr int PK_OFF_K = 2 * PK_QTILE, PK_OFF_V = PK_OFF_K + PK_KV * PK_KTILE, PK_OFF_BAR = PK_OFF_V + PK_KV * PK_KTILE;
@@ -708,14 +709,8 @@ extern "C" int kf_attn_pack_fwd(const kf_attn_pack_params* p, void* stream) {
        {{attn_pack_fwd_kernel<1, true, false, false>, attn_pack_fwd_kernel<1, true, false, true>}, {attn_pack_fwd_kernel<1, true, true, false>, attn_pack_fwd_kernel<1, true, true, true>}}}};
   const int f = p->dtype == KF_F16, c = p->cap > 0.f, b = p->slopes != nullptr, s = parts > 1;
   const KernelFn kern = table[f][c][b][s];
-  static PerDevice<bool> attr_set[2][2][2][2];
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (!attr_set[f][c][b][s].get(dev)) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PK_SMEM);
-    if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(attn_pack_fwd_kernel)");
-    attr_set[f][c][b][s].put(dev, true);
-  }
+  static PerDevice<bool> ready[2][2][2][2];
+  if ((rc = split_ready(reinterpret_cast<const void*>(kern), ready[f][c][b][s], PK_REGS, PK_SMEM, "kf_attn_pack_fwd")) != KF_OK) return rc;
   constexpr float LOG2E = 1.4426950408889634f;
   PackFwdArgs a{};
   a.O = o.ptr; a.o_st = o.row_stride; a.o_sh = o.head_stride; a.lse = p->lse; a.lse_ld = p->Tq;

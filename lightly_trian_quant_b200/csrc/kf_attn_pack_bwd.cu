@@ -32,9 +32,8 @@ namespace kf {
 
 constexpr int PB_T = 128, PB_W = 96, PB_D = 64;                // rows of a tile that stays, rows of a passing one
 constexpr int PB_THREADS = 640;
-constexpr int PB_REGS_WORK = 104, PB_REGS_LEAN = 64;
-constexpr int PB_REGS_LAUNCH = 96;
-static_assert(512 * PB_REGS_WORK + 128 * PB_REGS_LEAN <= PB_THREADS * PB_REGS_LAUNCH, "register split");
+constexpr int PB_REGS_WORK = 104, PB_REGS_LEAN = 64, PB_REGS = split_regs(512, PB_REGS_WORK, 128, PB_REGS_LEAN);
+static_assert(PB_THREADS * PB_REGS <= 65536, "registers of an SM");
 constexpr int PB_RTILE = PB_T * PB_D * 2, PB_CTILE = PB_W * PB_D * 2;     // 16 KB, 12 KB
 // Shared memory: row operands in two buffers (with ROWS = queries also O, for delta), a ring of passing ones; with ROWS = keys the log-sum-exp
 // and delta of the passing rows (1 KB per stage), with ROWS = queries the row sums of dS of four items (2 KB each); barriers.
@@ -698,20 +697,9 @@ static int wide_rows(const kf_heads& t) {
   return ((reinterpret_cast<uintptr_t>(t.ptr) | (uintptr_t)(t.row_stride * 2) | (uintptr_t)(t.head_stride * 2)) & 31) == 0;
 }
 
-// The register split draws on what the block was launched with: a build that allocates less is refused here, it would wait forever.
 static int bwd_ready(BwdFn kern, int which, size_t smem) {
   static PerDevice<bool> ready[16];
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (ready[which].get(dev)) return KF_OK;
-  cudaFuncAttributes attr;
-  cudaError_t e = cudaFuncGetAttributes(&attr, kern);
-  if (e != cudaSuccess) return cuda_status(e, "cudaFuncGetAttributes(attn_pack_bwd_kernel)");
-  KF_REQUIRE(attr.numRegs >= PB_REGS_LAUNCH, "kf_attn_pack_bwd: the kernel was built with %d registers per thread, its split needs %d", attr.numRegs, PB_REGS_LAUNCH);
-  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(attn_pack_bwd_kernel)");
-  ready[which].put(dev, true);
-  return KF_OK;
+  return split_ready(reinterpret_cast<const void*>(kern), ready[which], PB_REGS, smem, "kf_attn_pack_bwd");
 }
 
 }  // namespace kf

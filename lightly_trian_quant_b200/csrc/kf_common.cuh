@@ -34,6 +34,12 @@ class PerDevice {
   }
 };
 
+// In front of the first launch of a kernel that hands registers from one role to another: the sum of its roles comes from what the block was launched with, and where a
+// build allocates less the role that asks for more waits without a limit.  Refuses such a build, sets the limit of dynamic shared memory; `ready` keeps that it was done.
+int split_ready(const void* kernel, PerDevice<bool>& ready, int regs_per_thread, size_t smem, const char* what);
+// registers per thread that two roles take together, rounded up
+constexpr int split_regs(int threads_a, int regs_a, int threads_b, int regs_b) { return (threads_a * regs_a + threads_b * regs_b + threads_a + threads_b - 1) / (threads_a + threads_b); }
+
 // Programmatic dependent launch: a kernel lets its successor's CTAs start on SMs it no longer occupies (its partial last
 // wave, its teardown) and the successor runs its prologue (barrier set-up, TMEM allocation, descriptor prefetch) there; the
 // successor must not touch global memory before pdl_wait(), which returns when every predecessor grid has completed

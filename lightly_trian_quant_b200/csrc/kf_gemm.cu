@@ -351,14 +351,9 @@ struct GemmMaps {
 
 template <int KIND, int EPI, int BN, int FORM>
 static int launch_gemm(const GemmMaps& tm, const GemmArgs& g, int grid, cudaStream_t st) {
-  static PerDevice<bool> attr_set;
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (!attr_set.get(dev)) {
-    cudaError_t e = cudaFuncSetAttribute(gemm_kernel<KIND, EPI, BN, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)GEMM_SMEM_MAX);
-    if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(gemm_kernel)");
-    attr_set.put(dev, true);
-  }
+  static PerDevice<bool> ready;
+  const int rc = split_ready(reinterpret_cast<const void*>(gemm_kernel<KIND, EPI, BN, FORM>), ready, gemm_regs(EPI), GEMM_SMEM_MAX, "kf_gemm_bs");
+  if (rc != KF_OK) return rc;
   return cuda_status(launch_maybe_pdl(g.M, gemm_kernel<KIND, EPI, BN, FORM>, dim3(grid), dim3(GEMM_THREADS), gemm_smem<EPI, BN>(g.stages, g.vec_floats, g.res_tma != 0), st, tm.A, tm.W, tm.R, tm.C, g), "kf_gemm_bs launch");
 }
 

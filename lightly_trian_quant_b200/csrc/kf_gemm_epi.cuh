@@ -687,5 +687,9 @@ __device__ __forceinline__ void epilogue_warps(const GemmArgs& g, uint32_t tmem_
 
 constexpr int REGS_LEAN = 40, REGS_EPI = 104;          // 128 * 40 + 512 * 104 <= 640 * 96, the allocation at launch
 constexpr int REGS_LEAN_ROPE = 32, REGS_EPI_ROPE = 112; // the ROPE epilogue spills at 104 registers (64 accumulators + packed outputs + table values)
+constexpr int gemm_regs(int epi) {                     // what the roles take together, per thread
+  return epi == KF_EPI_ROPE ? split_regs(32 * EPI_WARP0, REGS_LEAN_ROPE, 32 * EPI_WARPS, REGS_EPI_ROPE) : split_regs(32 * EPI_WARP0, REGS_LEAN, 32 * EPI_WARPS, REGS_EPI);
+}
+static_assert(GEMM_THREADS * gemm_regs(KF_EPI_ROPE) <= 65536 && GEMM_THREADS * gemm_regs(KF_EPI_RES) <= 65536, "registers of an SM");
 
 }  // namespace kf

@@ -220,14 +220,9 @@ gemm_pair_kernel(const __grid_constant__ PairMaps tm, const GemmArgs g) {
 // ------------------------------------------------------------------------------------------------ host side
 template <int KIND, int EPI, int FORM>
 static int launch_pair(const PairMaps& tm, GemmArgs& g, int pairs, bool want_vec, cudaStream_t st) {
-  static PerDevice<bool> attr_set;
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (!attr_set.get(dev)) {
-    cudaError_t e = cudaFuncSetAttribute(gemm_pair_kernel<KIND, EPI, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PAIR_SMEM_MAX);
-    if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(gemm_pair_kernel)");
-    attr_set.put(dev, true);
-  }
+  static PerDevice<bool> ready;
+  const int rc = split_ready(reinterpret_cast<const void*>(gemm_pair_kernel<KIND, EPI, FORM>), ready, gemm_regs(EPI), PAIR_SMEM_MAX, "kf_gemm_bs (pair)");
+  if (rc != KF_OK) return rc;
   const int vec = want_vec ? g.N * (EPI == KF_EPI_RES ? 2 : 1) : 0;
   g.vec_floats = pair_smem<KIND, EPI>(3, vec, g.res_tma != 0) <= PAIR_SMEM_MAX ? vec : 0;
   g.stages = 2;

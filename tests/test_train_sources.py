@@ -17,3 +17,13 @@ def test_read_only_loads_are_of_what_no_kernel_writes():
         loads = re.findall(r"__ldg\(\s*([\w.]+)", _code(name))
         assert set(loads) <= {"a.slopes", "tiles"}, (name, loads)
         assert "__restrict__" not in _code(name), name
+
+
+def test_register_splits_are_checked_against_the_build():
+    """a kernel that hands registers from one role to another draws on those it was launched with; where a build gives it fewer, the role that asks for more waits without a limit:
+    every such kernel's launch looks at what the build allocated first."""
+    for path in sorted(CSRC.glob("*.cu")):
+        code = _code(path.name)
+        if "setmaxnreg_inc<" in code:
+            assert "split_ready(" in code, path.name
+            assert "cudaFuncAttributeMaxDynamicSharedMemorySize" not in code, path.name      # the look and this go together
