@@ -148,6 +148,24 @@ attn_pack_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     return !BIAS ? i : start + i < n ? start + i : n - 1 - i;
   };
 
+  // every warp: the CTA's tensor memory goes back, behind the last access to it.  A part of an item says that it is done and gives it back before it waits for the others: a CTA
+  // that held it meanwhile could stand against a cluster of another stream that holds the partner's SM.
+  auto release = [&]() {
+    tc_fence_before();
+    __syncthreads();
+    if (*abort_flag && !bad_align) {
+      for (int i = 0; i < 64; ++i) __nanosleep(2000);
+    }
+    if constexpr (SPLIT) {
+      __syncwarp();
+      cluster_arrive();
+    }
+    if (warp == 5) {
+      tc_fence_after();
+      tmem_dealloc(tmem_base, PK_TMEM_COLS);
+    }
+  };
+
   if (warp >= 4) {
   setmaxnreg_dec<PK_REGS_LEAN>();
   if (bad_align) {
@@ -544,7 +562,8 @@ attn_pack_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     }   // items
     if constexpr (SPLIT) {
       __syncwarp();
-      cluster_sync_all();                                        // every part of the item lies in its CTA's shared memory
+      release();
+      cluster_wait();                                            // every part of the item lies in its CTA's shared memory
       const QTile tile = tile_of(0);
       const int h = head_of(0), r1 = PK_BM * (rank + 1) / a.parts;
       const uint32_t part0 = smem_u32(smem + PK_OFF_PART), ml0 = smem_u32(smem + PK_OFF_ML);
@@ -587,18 +606,14 @@ attn_pack_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   }
   if constexpr (SPLIT) {
     __syncwarp();
-    if (warp >= 4 || bad_align) cluster_sync_all();              // the softmax warps have been there
+    if (warp >= 4 || bad_align) {                                // the softmax warps have been there
+      release();
+      __syncwarp();
+      cluster_wait();
+    }
     cluster_sync_all();                                          // nobody reads this CTA's shared memory any more
-  }
-
-  tc_fence_before();
-  __syncthreads();
-  if (*abort_flag && !bad_align) {
-    for (int i = 0; i < 64; ++i) __nanosleep(2000);
-  }
-  if (warp == 5) {
-    tc_fence_after();
-    tmem_dealloc(tmem_base, PK_TMEM_COLS);
+  } else {
+    release();
   }
 }
 

@@ -27,3 +27,14 @@ def test_register_splits_are_checked_against_the_build():
         if "setmaxnreg_inc<" in code:
             assert "split_ready(" in code, path.name
             assert "cudaFuncAttributeMaxDynamicSharedMemorySize" not in code, path.name      # the look and this go together
+
+
+def test_tensor_memory_is_given_back_before_a_cluster_waits():
+    """a CTA that held tensor memory while it waits for the others of its cluster could stand against a cluster of another stream that does the same the other way round: the
+    forward's parts give it back before they meet."""
+    code = _code("kf_attn_pack.cu")
+    assert code.count("tmem_dealloc(") == 1
+    release = code[code.index("auto release = [&]()"):]
+    assert "tmem_dealloc(" in release[:release.index("  };")] and "cluster_wait" not in release[:release.index("  };")]
+    for at in (m.start() for m in re.finditer(r"cluster_wait\(\)|cluster_sync_all\(\)", code)):
+        assert "release();" in code[:at][code[:at].rindex("if constexpr (SPLIT)"):], code[at - 200:at]
