@@ -13,7 +13,7 @@
 namespace kf {
 
 constexpr int ROPE_THREADS = 256, ROPE_MAX_PAIRS = 128, ROPE_MAX_TOKENS = 16;
-// Chunks (or pairs of chunks) per thread in flight: 32 KB of loads per CTA, four CTAs per SM (with twice as many, which leave room for two CTAs, a batch of
+// Chunks (or pairs of chunks) per thread in flight: 16 KB of loads per CTA, four CTAs per SM (with twice as many, which leave room for two CTAs, a batch of
 // clips took 120 us instead of 89; with half as many interleaved ones 5003 x 9 x 80 fp32 10.6 instead of 8.2)
 __host__ __device__ constexpr int rope_items(bool interleaved) { return interleaved ? 4 : 2; }
 
@@ -151,7 +151,9 @@ static int rope_launch(const RopeArgs& a, int interleaved, dim3 grid, cudaStream
 }
 template <typename T, typename TP>
 static int rope_by_width(const RopeArgs& a, int interleaved, int V, dim3 grid, cudaStream_t st) {
-  if (V == 8) return rope_launch<T, TP, 8>(a, interleaved, grid, st);
+  if constexpr (sizeof(T) == 2) {
+    if (V == 8) return rope_launch<T, TP, 8>(a, interleaved, grid, st);
+  }
   if (V == 4) return rope_launch<T, TP, 4>(a, interleaved, grid, st);
   if (V == 2) return rope_launch<T, TP, 2>(a, interleaved, grid, st);
   return rope_launch<T, TP, 1>(a, interleaved, grid, st);

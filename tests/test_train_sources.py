@@ -38,3 +38,15 @@ def test_tensor_memory_is_given_back_before_a_cluster_waits():
     assert "tmem_dealloc(" in release[:release.index("  };")] and "cluster_wait" not in release[:release.index("  };")]
     for at in (m.start() for m in re.finditer(r"cluster_wait\(\)|cluster_sync_all\(\)", code)):
         assert "release();" in code[:at][code[:at].rindex("if constexpr (SPLIT)"):], code[at - 200:at]
+
+
+def test_rotary_positions_have_no_kernel_that_nothing_reaches():
+    """the widest access is 16 bytes: eight 16-bit values, four of fp32"""
+    from lightly_trian_quant_b200 import build
+
+    build.build()
+    (path,) = (build.CSRC / "build").glob("kf_rope.*.ptxas")
+    kernels = set(re.findall(r"rope_axes_kernelI(\w+?)Li(\d)ELb(\d)E", path.read_text()))
+    assert {v for t, v, _ in kernels if t.startswith("f")} == {"1", "2", "4"}
+    assert {v for t, v, _ in kernels if not t.startswith("f")} == {"1", "2", "4", "8"}
+    assert ("ff", "1", "1") not in kernels                       # pairs side by side need two values at once
