@@ -267,6 +267,9 @@ KF_API int kf_set_pdl(int mode);
  * No counterpart in the reference (its mbarrier waits spin without a bound: infer-opt/round12_lowp_stack/impl/attn16o.cu:77-79). */
 KF_API int kf_check_device_error(void);
 
+/* Kernels that the calling thread has launched through the operators since it started (probes and self-tests aside). */
+KF_API int64_t kf_launch_count(void);
+
 /* ---- Operators for training on packed images and clips ------------------------------------------------------------- */
 
 /* LayerNorm that keeps each row's statistics: x [rows, d] (row stride ldx elements; f32 | bf16 | f16) -> y [rows, d] contiguous

@@ -79,6 +79,8 @@ def lib() -> C.CDLL:
         vp, i32, i64, f32 = C.c_void_p, C.c_int, C.c_int64, C.c_float
         L.kf_attn_pack_ws_bytes.restype = i64
         L.kf_attn_pack_ws_bytes.argtypes = [i32, i32, i32, i32]
+        L.kf_launch_count.restype = i64
+        L.kf_launch_count.argtypes = []
         L.kf_layer_norm_ws_bytes.restype = i64
         L.kf_layer_norm_ws_bytes.argtypes = [i64, i32]
         sigs = {

@@ -1109,6 +1109,9 @@ PyObject* attn_packed_bwd(PyObject* const* v) {
   return t;
 }
 
+// kernels that this thread has launched through the library
+PyObject* launch_count(PyObject* const*) { return PyLong_FromLongLong(kf_launch_count()); }
+
 // a weight: does the next GEMM with it read it ahead of its predecessor's end?
 PyObject* reads_weight_early(PyObject* const* v) {
   const Ref q = attr(v[0], s_q), sf = attr(v[0], s_sf);
@@ -1146,7 +1149,7 @@ PyMethodDef g_methods[] = {KF_ENTRY(quant_rows, 4),     KF_ENTRY(ln_quant, 7),  
                            KF_ENTRY(semantic, 3),       KF_ENTRY(amax_scale, 5), KF_ENTRY(ln_amax_scale, 7),
                            KF_ENTRY(layer_norm_fwd, 5), KF_ENTRY(layer_norm_bwd, 7), KF_ENTRY(rope_axes, 9),
                            KF_ENTRY(attn_plan, 4),      KF_ENTRY(attn_packed, 12),   KF_ENTRY(attn_packed_bwd, 17),
-                           KF_ENTRY(reads_weight_early, 1), {nullptr, nullptr, 0, nullptr}};
+                           KF_ENTRY(reads_weight_early, 1), KF_ENTRY(launch_count, 0), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_kf_host", "native operator layer over libkf_b200.so", -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -17,6 +17,12 @@ void set_error(const char* fmt, ...) {
   va_end(ap);
 }
 
+static thread_local int64_t g_launches = 0;
+cudaError_t counted(cudaError_t launched) {
+  g_launches += launched == cudaSuccess;
+  return launched;
+}
+
 int cuda_status(cudaError_t e, const char* what) {
   if (e == cudaSuccess) return KF_OK;
   set_error("%s: %s (%s)", what, cudaGetErrorName(e), cudaGetErrorString(e));
@@ -107,6 +113,8 @@ extern "C" int kf_set_pdl(int mode) {
 }
 
 extern "C" int kf_pdl_choice(int64_t rows, void* stream) { return kf::pdl_for(rows, static_cast<cudaStream_t>(stream)) ? 1 : 0; }
+
+extern "C" int64_t kf_launch_count(void) { return kf::g_launches; }
 
 extern "C" const char* kf_version(void) { return "kf_b200 0.1 sm_100a"; }
 

@@ -18,6 +18,7 @@ namespace kf {
 void set_error(const char* fmt, ...);
 int cuda_status(cudaError_t e, const char* what);
 int device_sm_count(int* sms);   // multiprocessor count of the current device (cached)
+cudaError_t counted(cudaError_t launched);     // a launch of an operator's kernel, for kf_launch_count
 bool pdl_for(int64_t rows, cudaStream_t st);   // programmatic dependent launch for a launch over this many rows?
 
 // A value that is worked out once per device and kept; T{} while it has not been.  Callers hold no lock (the Python layer releases the
@@ -64,7 +65,7 @@ inline cudaError_t launch_maybe_pdl(int64_t rows, void (*kernel)(KArgs...), dim3
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl_for(rows, st) ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+  return counted(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...));
 }
 
 // The same in clusters of `cluster` CTAs (1: none; at most 8)
@@ -89,7 +90,7 @@ inline cudaError_t launch_maybe_pdl_cluster(int64_t rows, int cluster, void (*ke
   }
   cfg.attrs = attr;
   cfg.numAttrs = n;
-  return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+  return counted(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...));
 }
 
 #define KF_REQUIRE(cond, ...)            \

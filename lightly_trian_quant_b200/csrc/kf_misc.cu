@@ -573,7 +573,7 @@ extern "C" int kf_semantic(const void* mask_logits, const void* class_logits, in
     case 7: semantic_kernel<7><<<grid, 256, smem, cs>>>(mlp, clp, Q, HW, scores, labels); break;
     default: semantic_kernel<8><<<grid, 256, smem, cs>>>(mlp, clp, Q, HW, scores, labels); break;
   }
-  return cuda_status(cudaGetLastError(), "kf_semantic launch");
+  return cuda_status(counted(cudaGetLastError()), "kf_semantic launch");
 }
 
 extern "C" int kf_resize_norm(const uint8_t* frames, void* out, int B, int Hi, int Wi, int So, const float* mean3, const float* std3, void* stream) {
@@ -584,7 +584,7 @@ extern "C" int kf_resize_norm(const uint8_t* frames, void* out, int B, int Hi, i
   dim3 grid((So + 255) / 256, So, B);
   resize_norm_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(frames, static_cast<__nv_bfloat16*>(out), Hi, Wi, So, mean3[0], mean3[1], mean3[2],
                                                                           std3[0], std3[1], std3[2]);
-  return cuda_status(cudaGetLastError(), "kf_resize_norm launch");
+  return cuda_status(counted(cudaGetLastError()), "kf_resize_norm launch");
 }
 
 // ------------------------------------------------------------------------------------------------ patch embed without a caller-provided scratch buffer

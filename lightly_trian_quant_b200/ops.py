@@ -23,7 +23,8 @@ from ._lib import KF_DT, KF_FMT, KF_G_GELU, KF_Q_GELU, KF_Q_RECIP_DIV, KF_Q_ROUN
 
 VEC = {"mx8": 32, "nv4": 16, "mx4": 32}
 
-# Launch accounting used by the benchmark: LAUNCHES counts every kernel launched through this module; when TIMING is
+# Launch accounting used by the benchmark: LAUNCHES counts every kernel launched through this module (an operator of one kernel that finds
+# nothing to do, no rows for instance, counts as one all the same); when TIMING is
 # a dict every launch is bracketed by CUDA events on the launching stream under its kernel-class name and BYTES
 # accumulates the algorithmic bytes of the memory-bound classes.
 LAUNCHES = 0
@@ -52,6 +53,15 @@ def _timed(name: str, fn, args: tuple, nbytes: int = 0):
     TIMING.setdefault(name, []).append((e0, e1))
     if nbytes:
         BYTES[name] = BYTES.get(name, 0) + nbytes
+    return r
+
+
+def _counted(name: str, fn, args: tuple):
+    """fn(*args) of an operator whose number of kernels depends on the call."""
+    global LAUNCHES
+    before = _h.launch_count()
+    r = fn(*args) if TIMING is None else _timed(name, fn, args)
+    LAUNCHES += _h.launch_count() - before
     return r
 
 
@@ -363,10 +373,7 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, mean: tor
                    bias: bool = True):
     """Gradients of layer_norm_fwd -> (dx in x's type, dw fp32 [d], db fp32 [d] or None with bias=False).  dres (shape and type of x) is added to
     dx: the gradient that goes past the norm in a residual block.  No atomics: the same bits from run to run."""
-    global LAUNCHES
-    LAUNCHES += 2
-    args = (dy, x, w, mean, rstd, dres, bias)
-    return _h.layer_norm_bwd(*args) if TIMING is None else _timed("layer_norm_bwd", _h.layer_norm_bwd, args)
+    return _counted("layer_norm_bwd", _h.layer_norm_bwd, (dy, x, w, mean, rstd, dres, bias))
 
 
 class RopeTable:
@@ -450,10 +457,7 @@ def attn_packed_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
     gradient).  q and dout inside a sequence have to be finite as k and v.  grads: tensors to write instead of new ones, e.g. the parts of one
     projection's gradient; they may not overlap one another or what the call reads.  f16 gradients have the range of f16: scale the loss as for any
     f16 product.  No atomics: the same bits from run to run."""
-    global LAUNCHES
-    LAUNCHES += 2
-    args = (*_pack_args(q, k, v, plan, scale, cap, slopes), dout, out, lse, *grads)
-    return _h.attn_packed_bwd(*args) if TIMING is None else _timed("attn_packed_bwd", _h.attn_packed_bwd, args)
+    return _counted("attn_packed_bwd", _h.attn_packed_bwd, (*_pack_args(q, k, v, plan, scale, cap, slopes), dout, out, lse, *grads))
 
 
 # ------------------------------------------------------------------------------------------------ patch embed / head / pre / post
