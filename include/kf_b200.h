@@ -282,8 +282,8 @@ KF_API int kf_layer_norm_fwd(int in_dtype, const void* x, int64_t ldx, const flo
 /* Its gradient: dy [rows, d] (row stride lddy, 0 for one row repeated; the type of y), x, w, mean and rstd as in the forward ->
  * dx [rows, d] contiguous in x's type, dw and db fp32 [d] (db may be NULL).  dres (NULL or [rows, d] in x's type, row stride ldres) is
  * added to dx: the gradient that reaches the rows past the norm, as in a pre-norm residual block.
- * ws: kf_layer_norm_ws_bytes(rows, d) bytes of device memory for the partial column sums (current device).  No atomics: the same bits
- * on every run of one device type. */
+ * ws: kf_layer_norm_ws_bytes(rows, d) bytes of device memory for the partial column sums (current device).  dw, db and ws NULL: dx alone, in one launch.
+ * No atomics: the same bits on every run of one device type. */
 KF_API int64_t kf_layer_norm_ws_bytes(int64_t rows, int d);
 KF_API int kf_layer_norm_bwd(int in_dtype, const void* x, int64_t ldx, int dy_dtype, const void* dy, int64_t lddy, const float* w, const float* mean,
                              const float* rstd, const void* dres, int64_t ldres, int rows, int d, void* dx, float* dw, float* db, void* ws,
@@ -347,7 +347,8 @@ typedef struct kf_attn_pack_params {
   int64_t ws_bytes;
 } kf_attn_pack_params;
 KF_API int kf_attn_pack_fwd(const kf_attn_pack_params* p, void* stream);
-/* dq, dk, dv from dout and what the forward read and wrote (the same tables, scale, cap and slopes; slopes have no gradient).  No atomics. */
+/* dq, dk, dv from dout and what the forward read and wrote (the same tables, scale, cap and slopes; slopes have no gradient).  dk.ptr and dv.ptr both NULL:
+ * dq alone, in one launch, with the workspace of n_k_tiles = 0.  No atomics. */
 KF_API int64_t kf_attn_pack_ws_bytes(int Hq, int Hk, int n_q_tiles, int n_k_tiles); /* for the current device */
 KF_API int kf_attn_pack_bwd(const kf_attn_pack_params* p, void* stream);
 

@@ -714,7 +714,7 @@ PyObject* layer_norm_fwd(PyObject* const* v) {
   return tuple3(std::move(y), piece(stats, 0, rows), THPVariable_Wrap(piece(stats, rows, rows)));
 }
 
-// dy, x, w, mean, rstd, dres | None, want db
+// dy, x, w, mean, rstd, dres | None, want db, want dw
 PyObject* layer_norm_bwd(PyObject* const* v) {
   const char* const op = "layer_norm_bwd";
   const at::Tensor &dy = cuda_tensor(v[0], "dy"), &x = cuda_tensor(v[1], "x");
@@ -734,14 +734,24 @@ PyObject* layer_norm_bwd(PyObject* const* v) {
     ldres = row_stride(r, op, "dres");
     dres = r.data_ptr();
   }
-  const bool want_db = truth(v[6]);
+  const bool want_dw = truth(v[7]), want_db = want_dw && truth(v[6]);
   const c10::cuda::CUDAGuard guard(x.device());
-  const int64_t bytes = kf_layer_norm_ws_bytes(rows, (int)d);
+  const int64_t bytes = want_dw ? kf_layer_norm_ws_bytes(rows, (int)d) : 0;
   if (bytes < 0) check((int)bytes, "kf_layer_norm_ws_bytes");
-  at::Tensor dx = empty(x.sizes(), x.scalar_type(), x.device()), dw = empty({d}, at::kFloat, x.device()), db, ws = empty({bytes / 4}, at::kFloat, x.device());
+  at::Tensor dx = empty(x.sizes(), x.scalar_type(), x.device()), dw, db, ws;
+  if (want_dw) {
+    dw = empty({d}, at::kFloat, x.device());
+    ws = empty({bytes / 4}, at::kFloat, x.device());
+  }
   if (want_db) db = empty({d}, at::kFloat, x.device());
   launch(op, kf_layer_norm_bwd, dtype_code(x.scalar_type()), (const void*)x.data_ptr(), ldx, dtype_code(dy.scalar_type()), (const void*)dy.data_ptr(), lddy, w, mean, rstd, dres, ldres,
-         (int)rows, (int)d, dx.data_ptr(), dw.data_ptr<float>(), want_db ? db.data_ptr<float>() : nullptr, ws.data_ptr(), bytes, stream());
+         (int)rows, (int)d, dx.data_ptr(), want_dw ? dw.data_ptr<float>() : nullptr, want_db ? db.data_ptr<float>() : nullptr, want_dw ? ws.data_ptr() : nullptr, bytes, stream());
+  if (!want_dw) {
+    PyObject* t = PyTuple_New(3);
+    PyTuple_SET_ITEM(t, 0, THPVariable_Wrap(std::move(dx)));
+    for (int i = 1; i < 3; ++i) PyTuple_SET_ITEM(t, i, new_ref(Py_None));
+    return t;
+  }
   return tuple3(std::move(dx), std::move(dw), want_db ? THPVariable_Wrap(std::move(db)) : new_ref(Py_None));
 }
 
@@ -1064,7 +1074,7 @@ PyObject* attn_packed(PyObject* const* v) {
   return t;
 }
 
-// ..., dout, out, lse, dq | None, dk | None, dv | None
+// ..., dout, out, lse, dq | None, dk | None, dv | None, want dk and dv
 PyObject* attn_packed_bwd(PyObject* const* v) {
   const char* const op = "attn_packed_bwd";
   Pack c = pack_operands(v, op);
@@ -1075,6 +1085,8 @@ PyObject* attn_packed_bwd(PyObject* const* v) {
     fail("%s: lse must be contiguous fp32 [query heads, query rows]", op);
   same_device(c.q, lse, op, "lse");
   const c10::cuda::CUDAGuard guard(c.q.device());
+  const bool keys = truth(v[17]);
+  need(keys || (v[15] == Py_None && v[16] == Py_None), "attn_packed_bwd: keys=False makes no dk and dv");
   const at::Tensor* const of[3] = {&c.q, &c.k, &c.v};
   const char* const names[3] = {"dq", "dk", "dv"};
   at::Tensor g[3];
@@ -1091,21 +1103,23 @@ PyObject* attn_packed_bwd(PyObject* const* v) {
   }
   for (int i = 0; i < 3; ++i) {
     if (g[i].defined()) writable(g[i]);
-    else g[i] = pack_new(*of[i], i ? c.k_rows : c.q_rows);
+    else if (keys || i == 0) g[i] = pack_new(*of[i], i ? c.k_rows : c.q_rows);
   }
   c.p.dout = pack_heads(dout);
   c.p.o = pack_heads(out);
   c.p.lse = lse.data_ptr<float>();
   c.p.dq = pack_heads(g[0]);
-  c.p.dk = pack_heads(g[1]);
-  c.p.dv = pack_heads(g[2]);
-  c.p.ws_bytes = kf_attn_pack_ws_bytes(c.p.Hq, c.p.Hk, c.p.n_q_tiles, c.p.n_k_tiles);
+  if (keys) {
+    c.p.dk = pack_heads(g[1]);
+    c.p.dv = pack_heads(g[2]);
+  }
+  c.p.ws_bytes = kf_attn_pack_ws_bytes(c.p.Hq, c.p.Hk, c.p.n_q_tiles, keys ? c.p.n_k_tiles : 0);
   if (c.p.ws_bytes < 0) check((int)c.p.ws_bytes, "kf_attn_pack_ws_bytes");
   at::Tensor ws = empty({c.p.ws_bytes / 4}, at::kFloat, c.q.device());
   c.p.ws = ws.data_ptr();
   launch(op, kf_attn_pack_bwd, (const kf_attn_pack_params*)&c.p, stream());
   PyObject* t = PyTuple_New(3);
-  for (int i = 0; i < 3; ++i) PyTuple_SET_ITEM(t, i, v[14 + i] == Py_None ? THPVariable_Wrap(std::move(g[i])) : new_ref(v[14 + i]));
+  for (int i = 0; i < 3; ++i) PyTuple_SET_ITEM(t, i, v[14 + i] == Py_None && g[i].defined() ? THPVariable_Wrap(std::move(g[i])) : new_ref(v[14 + i]));
   return t;
 }
 
@@ -1147,8 +1161,8 @@ PyMethodDef g_methods[] = {KF_ENTRY(quant_rows, 4),     KF_ENTRY(ln_quant, 7),  
                            KF_ENTRY(qkv_rope, 10),      KF_ENTRY(gemm_gelu_q, 6), KF_ENTRY(bmm_nt, 3),   KF_ENTRY(gemm_tokens, 8),    KF_ENTRY(broadcast_rows, 3),
                            KF_ENTRY(ln_tail, 8),        KF_ENTRY(attn_fwd, 3),   KF_ENTRY(attn_fwd_quant, 4), KF_ENTRY(im2col_patch16, 1), KF_ENTRY(dw_ln, 10),
                            KF_ENTRY(semantic, 3),       KF_ENTRY(amax_scale, 5), KF_ENTRY(ln_amax_scale, 7),
-                           KF_ENTRY(layer_norm_fwd, 5), KF_ENTRY(layer_norm_bwd, 7), KF_ENTRY(rope_axes, 9),
-                           KF_ENTRY(attn_plan, 4),      KF_ENTRY(attn_packed, 12),   KF_ENTRY(attn_packed_bwd, 17),
+                           KF_ENTRY(layer_norm_fwd, 5), KF_ENTRY(layer_norm_bwd, 8), KF_ENTRY(rope_axes, 9),
+                           KF_ENTRY(attn_plan, 4),      KF_ENTRY(attn_packed, 12),   KF_ENTRY(attn_packed_bwd, 18),
                            KF_ENTRY(reads_weight_early, 1), KF_ENTRY(launch_count, 0), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_kf_host", "native operator layer over libkf_b200.so", -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -722,9 +722,10 @@ extern "C" int kf_attn_pack_bwd(const kf_attn_pack_params* p, void* stream) {
   int rc = check_pack(p);
   if (rc != KF_OK) return rc;
   if (p->n_q_tiles == 0 && p->n_k_tiles == 0) return KF_OK;
+  // (dq alone: the first launch)
   constexpr float LOG2E = 1.4426950408889634f;
   kf_heads q{}, k{}, v{}, o{}, go{}, gq{}, gk{}, gv{};
-  const bool any_q = p->n_q_tiles > 0, any_k = p->n_k_tiles > 0;
+  const bool any_q = p->n_q_tiles > 0, any_k = p->n_k_tiles > 0 && (p->dk.ptr || p->dv.ptr);
   KF_REQUIRE((!any_q || (p->Tq > 0 && p->q_tiles && p->lse)) && (!any_k || (p->Tk > 0 && p->k_tiles)), "kf_attn_pack_bwd: null pointer");
   if (p->Tq > 0) {
     if ((rc = check_heads("q", p->q, p->Tq, p->Hq, &q)) != KF_OK) return rc;
@@ -735,10 +736,10 @@ extern "C" int kf_attn_pack_bwd(const kf_attn_pack_params* p, void* stream) {
   if (p->Tk > 0) {
     if ((rc = check_heads("k", p->k, p->Tk, p->Hk, &k)) != KF_OK) return rc;
     if ((rc = check_heads("v", p->v, p->Tk, p->Hk, &v)) != KF_OK) return rc;
-    if ((rc = check_heads("dk", p->dk, p->Tk, p->Hk, &gk)) != KF_OK) return rc;
-    if ((rc = check_heads("dv", p->dv, p->Tk, p->Hk, &gv)) != KF_OK) return rc;
+    if (any_k && (rc = check_heads("dk", p->dk, p->Tk, p->Hk, &gk)) != KF_OK) return rc;
+    if (any_k && (rc = check_heads("dv", p->dv, p->Tk, p->Hk, &gv)) != KF_OK) return rc;
   }
-  const int64_t need = kf_attn_pack_ws_bytes(p->Hq, p->Hk, p->n_q_tiles, p->n_k_tiles);
+  const int64_t need = kf_attn_pack_ws_bytes(p->Hq, p->Hk, p->n_q_tiles, any_k ? p->n_k_tiles : 0);
   if (need < 0) return (int)need;
   KF_REQUIRE(p->ws && (reinterpret_cast<uintptr_t>(p->ws) & 31) == 0 && p->ws_bytes >= need, "kf_attn_pack_bwd: workspace of %lld bytes, needs %lld, 32-byte aligned",
              (long long)p->ws_bytes, (long long)need);

@@ -94,7 +94,7 @@ struct LnArgs {
   const float *w, *b;
   float *mean, *rstd;
   void *y, *dx;
-  float* part;                       // backward: [gridDim.x][2][d]
+  float* part;                       // backward: [gridDim.x][2][d], or null: the rows' gradient alone
   int64_t ldx, lddy, ldres;
   int rows, d, W;
   int slot_x, slot_y, slot_r;        // bytes of a row's place in shared memory, per tensor (multiples of 16; 0: not there)
@@ -337,7 +337,7 @@ __global__ void __launch_bounds__(LN_THREADS) layer_norm_bwd_kernel(const __grid
   // the groups of this CTA, in their order, where the ring was; then the CTA's line of the partial sums
   ln_drain(ok);
   __syncthreads();
-  if (abort_flag) return;
+  if (abort_flag || !a.part) return;
   float* colsum = reinterpret_cast<float*>(ln_smem);             // [2][d], where a CTA has more than one group
   float* part = a.part + (size_t)blockIdx.x * 2 * a.d;
   for (int g = 0; g < groups; ++g) {
@@ -506,17 +506,17 @@ extern "C" int kf_layer_norm_bwd(int in_dtype, const void* x, int64_t ldx, int d
   KF_REQUIRE(ln_float_type(in_dtype) && ln_float_type(dy_dtype), "kf_layer_norm_bwd: types must be f32, bf16 or f16");
   KF_REQUIRE(rows >= 0 && d > 0 && d <= LN_MAX_WIDTH && ldx >= 0 && lddy >= 0 && ldres >= 0, "kf_layer_norm_bwd: bad shape rows=%d d=%d (at most %d wide)", rows, d,
              LN_MAX_WIDTH);
-  KF_REQUIRE(w && dw, "kf_layer_norm_bwd: null pointer");
+  KF_REQUIRE(w && (dw || !db), "kf_layer_norm_bwd: null pointer");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (rows == 0) {
-    cudaError_t e = cudaMemsetAsync(dw, 0, (size_t)d * 4, st);
+    cudaError_t e = dw ? cudaMemsetAsync(dw, 0, (size_t)d * 4, st) : cudaSuccess;
     if (e == cudaSuccess && db) e = cudaMemsetAsync(db, 0, (size_t)d * 4, st);
     return cuda_status(e, "kf_layer_norm_bwd memset");
   }
-  KF_REQUIRE(x && dy && mean && rstd && dx && ws, "kf_layer_norm_bwd: null pointer");
+  KF_REQUIRE(x && dy && mean && rstd && dx && (ws || !dw), "kf_layer_norm_bwd: null pointer");
   LnArgs a{};
   a.x = x; a.ldx = ldx; a.dy = dy; a.lddy = lddy; a.dres = dres; a.ldres = ldres; a.w = w; a.mean = const_cast<float*>(mean); a.rstd = const_cast<float*>(rstd);
-  a.dx = dx; a.part = static_cast<float*>(ws); a.rows = rows; a.d = d; a.W = ln_warps(d, true); a.inv_d = 1.0f / (float)d;
+  a.dx = dx; a.part = dw ? static_cast<float*>(ws) : nullptr; a.rows = rows; a.d = d; a.W = ln_warps(d, true); a.inv_d = 1.0f / (float)d;
   a.slot_x = ln_slot(d, ln_size(in_dtype));
   a.slot_y = ln_slot(d, ln_size(dy_dtype));
   a.slot_r = dres ? a.slot_x : 0;
@@ -527,9 +527,9 @@ extern "C" int kf_layer_norm_bwd(int in_dtype, const void* x, int64_t ldx, int d
   const bool wide = d % 8 == 0 && ln_aligned(x, ldx * ln_size(in_dtype)) && ln_aligned(dy, lddy * ln_size(dy_dtype)) && ln_aligned(dres, ldres * ln_size(in_dtype)) &&
                     ln_aligned(dx, 0) && ln_aligned(w, 0);
   const int rc = ln_by_type(in_dtype, dy_dtype, wide, d, a.W, [&](auto ti, auto to, auto ch, auto nc) {
-    return ln_launch<layer_norm_bwd_kernel<decltype(ti), decltype(to), decltype(ch)::value, decltype(nc)::value>>("kf_layer_norm_bwd launch", rows, smem, st, a, ws_bytes, &grid);
+    return ln_launch<layer_norm_bwd_kernel<decltype(ti), decltype(to), decltype(ch)::value, decltype(nc)::value>>("kf_layer_norm_bwd launch", rows, smem, st, a, dw ? ws_bytes : -1, &grid);
   });
-  if (rc != KF_OK) return rc;
+  if (rc != KF_OK || !dw) return rc;
   return cuda_status(launch_maybe_pdl(1, layer_norm_cols_kernel, dim3((2 * d + 31) / 32), dim3(1024), 0, st, static_cast<const float*>(ws), grid, d, dw, db),
                      "kf_layer_norm_bwd column sums launch");
 }

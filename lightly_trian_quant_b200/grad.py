@@ -38,7 +38,7 @@ class _LayerNorm(torch.autograd.Function):
     def backward(ctx, dy):
         x, w, mean, rstd = ctx.saved_tensors
         _eager_backward()
-        dx, dw, db = ops.layer_norm_bwd(_rows(dy), x, w, mean, rstd, bias=ctx.bias)
+        dx, dw, db = ops.layer_norm_bwd(_rows(dy), x, w, mean, rstd, bias=ctx.bias, affine=any(ctx.needs_input_grad[1:3]))
         return dx, dw, db, None, None
 
 
@@ -70,7 +70,7 @@ class _AttnPacked(torch.autograd.Function):
         q, k, v, out, lse, slopes = ctx.saved_tensors
         plan, scale, cap = ctx.how
         _eager_backward()
-        return (*ops.attn_packed_bwd(_rows(dout), q, k, v, out, lse, plan, scale=scale, cap=cap, slopes=slopes), None, None, None, None)
+        return (*ops.attn_packed_bwd(_rows(dout), q, k, v, out, lse, plan, scale=scale, cap=cap, slopes=slopes, keys=any(ctx.needs_input_grad[1:3])), None, None, None, None)
 
 
 def _eager_backward() -> None:

@@ -370,10 +370,10 @@ def layer_norm_fwd(x: torch.Tensor, w: torch.Tensor, b: Optional[torch.Tensor], 
 
 
 def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, *, dres: Optional[torch.Tensor] = None,
-                   bias: bool = True):
-    """Gradients of layer_norm_fwd -> (dx in x's type, dw fp32 [d], db fp32 [d] or None with bias=False).  dres (shape and type of x) is added to
+                   bias: bool = True, affine: bool = True):
+    """Gradients of layer_norm_fwd -> (dx in x's type, dw fp32 [d], db fp32 [d] or None with bias=False); affine=False: dx alone, the others None.  dres (shape and type of x) is added to
     dx: the gradient that goes past the norm in a residual block.  No atomics: the same bits from run to run."""
-    return _counted("layer_norm_bwd", _h.layer_norm_bwd, (dy, x, w, mean, rstd, dres, bias))
+    return _counted("layer_norm_bwd", _h.layer_norm_bwd, (dy, x, w, mean, rstd, dres, bias, affine))
 
 
 class RopeTable:
@@ -452,12 +452,12 @@ def attn_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: AttnPla
 
 
 def attn_packed_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, lse: torch.Tensor, plan: AttnPlan, *,
-                    scale: Optional[float] = None, cap: float = 0.0, slopes: Optional[torch.Tensor] = None, grads=(None, None, None)):
-    """Gradients of attn_packed -> (dq, dk, dv) in the operands' type; the other arguments as the forward took and gave them (slopes have no
+                    scale: Optional[float] = None, cap: float = 0.0, slopes: Optional[torch.Tensor] = None, grads=(None, None, None), keys: bool = True):
+    """Gradients of attn_packed -> (dq, dk, dv) in the operands' type, with keys=False (dq, None, None) at half the work; the other arguments as the forward took and gave them (slopes have no
     gradient).  q and dout inside a sequence have to be finite as k and v.  grads: tensors to write instead of new ones, e.g. the parts of one
     projection's gradient; they may not overlap one another or what the call reads.  f16 gradients have the range of f16: scale the loss as for any
     f16 product.  No atomics: the same bits from run to run."""
-    return _counted("attn_packed_bwd", _h.attn_packed_bwd, (*_pack_args(q, k, v, plan, scale, cap, slopes), dout, out, lse, *grads))
+    return _counted("attn_packed_bwd", _h.attn_packed_bwd, (*_pack_args(q, k, v, plan, scale, cap, slopes), dout, out, lse, *grads, keys))
 
 
 # ------------------------------------------------------------------------------------------------ patch embed / head / pre / post

@@ -57,3 +57,57 @@ def test_launches_of_the_row_operators():
     assert _kernels(lambda: ops.layer_norm_bwd(y[:0], x[:0], w, mean[:0], rstd[:0])) == (0, 0)       # two memory sets
     table, pos = ops.RopeTable([[1.0]], 96), torch.zeros(40, 1, dtype=torch.int32, device="cuda")
     assert _kernels(lambda: ops.rope_axes(x.view(40, 1, 96), pos, table)) == (1, 1)
+
+
+@gpu
+@pytest.mark.parametrize("heads", [(4, 4), (4, 1)])
+def test_gradients_of_queries_alone(heads):
+    """frozen keys and values: the launches for their gradients are left out, dq has the bits that it has with them"""
+    from lightly_trian_quant_b200 import grad, ops
+
+    g = torch.Generator(device="cuda").manual_seed(1)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda").to(BF)  # noqa: E731
+    q, k, v, do = r(300, heads[0], 64), r(300, heads[1], 64), r(300, heads[1], 64), r(300, heads[0], 64)
+    plan = ops.AttnPlan([170, 130], causal=True)
+    out, lse = ops.attn_packed(q, k, v, plan, cap=20.0)
+    want = ops.attn_packed_bwd(do, q, k, v, out, lse, plan, cap=20.0)
+    with torch.enable_grad():
+        for need in ((True, False, False), (True, True, False), (False, False, True)):
+            leaves = [t.clone().requires_grad_(n) for t, n in zip((q, k, v), need)]
+            y = grad.attn_packed(*leaves, plan, cap=20.0)
+            before = ops.LAUNCHES
+            y.backward(do)
+            torch.cuda.synchronize()
+            assert ops.LAUNCHES - before == (1 if not any(need[1:]) else 2 if heads[0] == heads[1] else 3)
+            for t, n, w in zip(leaves, need, want):
+                assert torch.equal(t.grad, w) if n else t.grad is None
+    dq, none, nothing = ops.attn_packed_bwd(do, q, k, v, out, lse, plan, cap=20.0, keys=False)
+    assert torch.equal(dq, want[0]) and none is None and nothing is None
+    given = torch.full_like(q, 7)
+    assert ops.attn_packed_bwd(do, q, k, v, out, lse, plan, cap=20.0, grads=(given, None, None), keys=False)[0] is given and torch.equal(given, want[0])
+    with pytest.raises(ops.KfError, match="keys"):
+        ops.attn_packed_bwd(do, q, k, v, out, lse, plan, cap=20.0, grads=(None, torch.empty_like(k), None), keys=False)
+    ops.check_device_error()
+
+
+@gpu
+@pytest.mark.parametrize("R,d", [(300, 96), (9000, 333), (7, 4096), (0, 64)])
+def test_gradients_of_rows_alone(R, d):
+    """a frozen norm: no column sums, dx has the bits that it has with them"""
+    from lightly_trian_quant_b200 import grad, ops
+
+    x, dy, w = torch.randn(R, d, device="cuda"), torch.randn(R, d, device="cuda"), 1 + 0.1 * torch.randn(d, device="cuda")
+    y, mean, rstd = ops.layer_norm_fwd(x, w, w, 1e-5)
+    want = ops.layer_norm_bwd(dy, x, w, mean, rstd, dres=dy)
+    dx, none, nothing = ops.layer_norm_bwd(dy, x, w, mean, rstd, dres=dy, affine=False)
+    assert torch.equal(dx, want[0]) and none is None and nothing is None
+    with torch.enable_grad():
+        for need in ((True, False, False), (True, True, True), (False, False, True)):
+            leaves = [t.clone().requires_grad_(n) for t, n in zip((x, w, w), need)]
+            out = grad.layer_norm(*leaves, 1e-5)
+            before = ops.LAUNCHES
+            out.backward(dy)
+            torch.cuda.synchronize()
+            assert ops.LAUNCHES - before == (0 if R == 0 else 2 if any(need[1:]) else 1)
+            assert [t.grad is not None for t in leaves] == list(need)
+    ops.check_device_error()
