@@ -15,9 +15,22 @@ from . import ops
 from ._lib import KfError
 
 
-def _eager(*tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors) and torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+def _capturing(t: torch.Tensor) -> bool:
+    """does the stream capture that an operator on t launches on: the current one of its device"""
+    if t.device.index == torch.cuda.current_device():
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(t.device):
+        return torch.cuda.is_current_stream_capturing()
+
+
+def _eager_backward(t: torch.Tensor) -> None:
+    if _capturing(t):
         raise KfError("grad: no autograd inside a CUDA graph capture; capture the operators of ops (forward and gradient) instead")
+
+
+def _eager(*tensors) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors) and tensors[0].device.type == "cuda":
+        _eager_backward(tensors[0])
 
 
 def _rows(g: torch.Tensor) -> torch.Tensor:
@@ -37,7 +50,7 @@ class _LayerNorm(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         x, w, mean, rstd = ctx.saved_tensors
-        _eager_backward()
+        _eager_backward(x)
         dx, dw, db = ops.layer_norm_bwd(_rows(dy), x, w, mean, rstd, bias=ctx.bias, affine=any(ctx.needs_input_grad[1:3]))
         return dx, dw, db, None, None
 
@@ -52,7 +65,7 @@ class _RopeAxes(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        _eager_backward()
+        _eager_backward(dy)
         return ops.rope_axes(_rows(dy), *ctx.saved_tensors, ctx.table, inverse=True), None, None
 
 
@@ -69,13 +82,8 @@ class _AttnPacked(torch.autograd.Function):
     def backward(ctx, dout):
         q, k, v, out, lse, slopes = ctx.saved_tensors
         plan, scale, cap = ctx.how
-        _eager_backward()
+        _eager_backward(q)
         return (*ops.attn_packed_bwd(_rows(dout), q, k, v, out, lse, plan, scale=scale, cap=cap, slopes=slopes, keys=any(ctx.needs_input_grad[1:3])), None, None, None, None)
-
-
-def _eager_backward() -> None:
-    if torch.cuda.is_current_stream_capturing():
-        raise KfError("grad: no autograd inside a CUDA graph capture; capture the operators of ops (forward and gradient) instead")
 
 
 def layer_norm(x: torch.Tensor, w: torch.Tensor, b: Optional[torch.Tensor], eps: float, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
