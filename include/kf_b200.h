@@ -343,13 +343,16 @@ typedef struct kf_attn_pack_params {
   float* lse;              /* fp32 [Hq, Tq]: written by the forward, read by the gradient              */
   kf_heads q, k, v, o;     /* o: written by the forward, read by the gradient                          */
   kf_heads dout, dq, dk, dv; /* gradient only                                                          */
-  void* ws;                /* gradient only: kf_attn_pack_ws_bytes bytes, 32-byte aligned              */
+  void* ws;                /* gradient only: kf_attn_pack_bwd_ws_bytes bytes, 32-byte aligned          */
   int64_t ws_bytes;
+  int64_t k_work;          /* gradient only: queries that see a record of k_tiles (from the lowest one of the record's first key on), summed over the records ... */
+  int k_longest;           /* ... and the most of one; 0 if not known: then shared key heads are only split where every query head finds an SM */
 } kf_attn_pack_params;
 KF_API int kf_attn_pack_fwd(const kf_attn_pack_params* p, void* stream);
 /* dq, dk, dv from dout and what the forward read and wrote (the same tables, scale, cap and slopes; slopes have no gradient).  dk.ptr and dv.ptr both NULL:
  * dq alone, in one launch, with the workspace of n_k_tiles = 0.  No atomics. */
-KF_API int64_t kf_attn_pack_ws_bytes(int Hq, int Hk, int n_q_tiles, int n_k_tiles); /* for the current device */
+KF_API int64_t kf_attn_pack_bwd_ws_bytes(const kf_attn_pack_params* p);              /* of this call (its ws and ws_bytes are not looked at), for the current device */
+KF_API int64_t kf_attn_pack_ws_bytes(int Hq, int Hk, int n_q_tiles, int n_k_tiles); /* of a call without k_work and k_longest */
 KF_API int kf_attn_pack_bwd(const kf_attn_pack_params* p, void* stream);
 
 #ifdef __cplusplus

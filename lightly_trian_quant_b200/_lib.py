@@ -50,7 +50,7 @@ class AttnPackParams(C.Structure):
     _fields_ = [("dtype", C.c_int), ("Hq", C.c_int), ("Hk", C.c_int), ("n_q_tiles", C.c_int), ("n_k_tiles", C.c_int), ("longest", C.c_int), ("scale", C.c_float), ("cap", C.c_float),
                 ("Tq", C.c_int64), ("Tk", C.c_int64), ("q_tiles", C.c_void_p), ("k_tiles", C.c_void_p), ("slopes", C.c_void_p), ("lse", C.c_void_p),
                 ("q", Heads), ("k", Heads), ("v", Heads), ("o", Heads), ("dout", Heads), ("dq", Heads), ("dk", Heads), ("dv", Heads), ("ws", C.c_void_p),
-                ("ws_bytes", C.c_int64)]
+                ("ws_bytes", C.c_int64), ("k_work", C.c_int64), ("k_longest", C.c_int)]
 
 
 _lib = None
@@ -77,6 +77,8 @@ def lib() -> C.CDLL:
         L.kf_sf_bytes.restype = C.c_int64
         L.kf_sf_bytes.argtypes = [C.c_int64, C.c_int64, C.c_int]
         vp, i32, i64, f32 = C.c_void_p, C.c_int, C.c_int64, C.c_float
+        L.kf_attn_pack_bwd_ws_bytes.restype = i64
+        L.kf_attn_pack_bwd_ws_bytes.argtypes = [C.POINTER(AttnPackParams)]
         L.kf_attn_pack_ws_bytes.restype = i64
         L.kf_attn_pack_ws_bytes.argtypes = [i32, i32, i32, i32]
         L.kf_launch_count.restype = i64

@@ -987,7 +987,8 @@ std::vector<int64_t> lengths(PyObject* o, const char* what) {
   return v;
 }
 
-// q lengths, k lengths | None, causal, prefixes | None -> (table int32 [query tiles + key tiles, 8] on the CPU, query tiles, query rows, key rows, the most keys a query tile sees):
+// q lengths, k lengths | None, causal, prefixes | None -> (table int32 [query tiles + key tiles, 8] on the CPU, query tiles, query rows, key rows, the most keys a query tile sees, the queries that see
+// a key tile: of all, the most of one):
 // the records of kf_attn_pack_params, of queries and then of keys, each with the longest work first
 PyObject* attn_plan(PyObject* const* v) {
   constexpr int64_t T = 128, MOST = INT32_MAX - 256;
@@ -1033,12 +1034,16 @@ PyObject* attn_plan(PyObject* const* v) {
   int32_t* to = table.data_ptr<int32_t>();
   for (const std::vector<Tile>* tiles : {&q, &k})
     for (const Tile& t : *tiles) to = std::copy(t.w, t.w + 8, to);
-  PyObject* r = PyTuple_New(5);
+  int64_t k_work = 0;
+  for (const Tile& t : k) k_work += std::max(t.work, (int64_t)0);
+  PyObject* r = PyTuple_New(7);
   PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(std::move(table)));
   PyTuple_SET_ITEM(r, 1, PyLong_FromLongLong(nq));
   PyTuple_SET_ITEM(r, 2, PyLong_FromLongLong(rows_q));
   PyTuple_SET_ITEM(r, 3, PyLong_FromLongLong(rows_k));
   PyTuple_SET_ITEM(r, 4, PyLong_FromLongLong(q.empty() ? 0 : q[0].work));
+  PyTuple_SET_ITEM(r, 5, PyLong_FromLongLong(k_work));
+  PyTuple_SET_ITEM(r, 6, PyLong_FromLongLong(k.empty() ? 0 : std::max(k[0].work, (int64_t)0)));
   return r;
 }
 
@@ -1074,7 +1079,7 @@ PyObject* attn_packed(PyObject* const* v) {
   return t;
 }
 
-// ..., dout, out, lse, dq | None, dk | None, dv | None, want dk and dv
+// ..., dout, out, lse, dq | None, dk | None, dv | None, want dk and dv, the plan's queries that see a key tile: of all, the most of one
 PyObject* attn_packed_bwd(PyObject* const* v) {
   const char* const op = "attn_packed_bwd";
   Pack c = pack_operands(v, op);
@@ -1113,8 +1118,10 @@ PyObject* attn_packed_bwd(PyObject* const* v) {
     c.p.dk = pack_heads(g[1]);
     c.p.dv = pack_heads(g[2]);
   }
-  c.p.ws_bytes = kf_attn_pack_ws_bytes(c.p.Hq, c.p.Hk, c.p.n_q_tiles, keys ? c.p.n_k_tiles : 0);
-  if (c.p.ws_bytes < 0) check((int)c.p.ws_bytes, "kf_attn_pack_ws_bytes");
+  c.p.k_work = to_int(v[18]);
+  c.p.k_longest = (int)to_int(v[19]);
+  c.p.ws_bytes = kf_attn_pack_bwd_ws_bytes(&c.p);
+  if (c.p.ws_bytes < 0) check((int)c.p.ws_bytes, "kf_attn_pack_bwd_ws_bytes");
   at::Tensor ws = empty({c.p.ws_bytes / 4}, at::kFloat, c.q.device());
   c.p.ws = ws.data_ptr();
   launch(op, kf_attn_pack_bwd, (const kf_attn_pack_params*)&c.p, stream());
@@ -1162,7 +1169,7 @@ PyMethodDef g_methods[] = {KF_ENTRY(quant_rows, 4),     KF_ENTRY(ln_quant, 7),  
                            KF_ENTRY(ln_tail, 8),        KF_ENTRY(attn_fwd, 3),   KF_ENTRY(attn_fwd_quant, 4), KF_ENTRY(im2col_patch16, 1), KF_ENTRY(dw_ln, 10),
                            KF_ENTRY(semantic, 3),       KF_ENTRY(amax_scale, 5), KF_ENTRY(ln_amax_scale, 7),
                            KF_ENTRY(layer_norm_fwd, 5), KF_ENTRY(layer_norm_bwd, 8), KF_ENTRY(rope_axes, 9),
-                           KF_ENTRY(attn_plan, 4),      KF_ENTRY(attn_packed, 12),   KF_ENTRY(attn_packed_bwd, 18),
+                           KF_ENTRY(attn_plan, 4),      KF_ENTRY(attn_packed, 12),   KF_ENTRY(attn_packed_bwd, 20),
                            KF_ENTRY(reads_weight_early, 1), KF_ENTRY(launch_count, 0), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_kf_host", "native operator layer over libkf_b200.so", -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -680,10 +680,22 @@ __global__ void __launch_bounds__(JOIN_THREADS) bwd_join_kernel(const __grid_con
   *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Items per key head in the second launch.  A key head that several query heads share makes an item of that many times the steps; where there are few
-// items, an item per query head fills the device evenly, at the price of fp32 sums through memory (10 sequences of 1 to 2053 tokens, 12 heads
-// on 4: 240 items, the longest with 66 steps where 37 are the mean).
-static int bwd_split(int Hq, int Hk, int n_k_tiles, int sms) { return (int64_t)n_k_tiles * Hk < 4ll * sms ? Hq / Hk : 1; }
+// Items per key head in the second launch: one, or one for every query head that shares it, whose sums go through memory in fp32 (64 KB each).  Whole items of many
+// query heads are long chains, split ones fill the device evenly; which is shorter is worked out in steps (0.7 us) from the batch's lengths, the longest chain or the
+// mean of an SM: an item costs 6 steps beside its own, the join 6.  Measured, both directions in us, whole / split:
+//   16 heads on 1   1 x 1605 tokens 242 / 77, 8 x 1605 371 / 367, 16 x 1605 710 / 758; 20 x 130 54 / 70, 60 x 130 84 / 155, 150 x 130 215 / 352
+//   12 heads on 4   1 x 1605 causal 63 / 43, 4 x 1605 causal 92 / 102, 4 x 1605 154 / 158, 60 x 130 81 / 121; ten causal clips of 1 to 2053 with a cap, f16 209 / 189
+// (a choice by the number of items alone, fewer than four rounds, took up to 1.84 times the shorter time over 218 such cases, this one up to 1.15)
+static int bwd_split(const kf_attn_pack_params* p, int n_k_tiles, int sms) {
+  const int share = p->Hq / p->Hk;
+  if (share == 1 || n_k_tiles == 0) return 1;
+  if (p->k_work <= 0) return (int64_t)n_k_tiles * p->Hq <= sms ? share : 1;
+  constexpr double ITEM = 6, JOIN = 6;
+  const double n = n_k_tiles, longest = (p->k_longest + PB_W - 1) / PB_W, all = (double)p->k_work / PB_W + 0.5 * n, per_sm = (double)p->Hk / sms;
+  const auto larger = [](double x, double y) { return x > y ? x : y; };
+  const double whole = larger(longest * share + ITEM, (all * share + n * ITEM) * per_sm), split = larger(longest + ITEM, (all + n * ITEM) * share * per_sm) + JOIN;
+  return split < whole ? share : 1;
+}
 static int64_t bwd_stat_bytes(int Hq, int n_q_tiles) { return 2 * ((int64_t)Hq * n_q_tiles + 1) * PB_T * 4; }      // the last passing tile may reach behind the last row
 
 using BwdFn = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, PackBwdArgs);
@@ -702,6 +714,16 @@ static int bwd_ready(BwdFn kern, int which, size_t smem) {
   return split_ready(reinterpret_cast<const void*>(kern), ready[which], PB_REGS, smem, "kf_attn_pack_bwd");
 }
 
+static bool wants_keys(const kf_attn_pack_params* p) { return p->dk.ptr || p->dv.ptr; }      // else dq alone: the first launch
+
+static int64_t bwd_ws_bytes(const kf_attn_pack_params* p, int n_k_tiles) {
+  int sms = 0;
+  const int rc = device_sm_count(&sms);
+  if (rc != KF_OK) return rc > 0 ? KF_ERR_UNSUPPORTED : rc;
+  const int64_t split = bwd_split(p, n_k_tiles, sms);
+  return bwd_stat_bytes(p->Hq, p->n_q_tiles) + (split > 1 ? split * n_k_tiles * p->Hk * 2 * PB_T * PB_D * 4 : 0);
+}
+
 }  // namespace kf
 
 using namespace kf;
@@ -711,21 +733,23 @@ extern "C" int64_t kf_attn_pack_ws_bytes(int Hq, int Hk, int n_q_tiles, int n_k_
     set_error("kf_attn_pack_ws_bytes: bad argument Hq=%d Hk=%d n_q_tiles=%d n_k_tiles=%d", Hq, Hk, n_q_tiles, n_k_tiles);
     return KF_ERR_BAD_ARGUMENT;
   }
-  int sms = 0;
-  const int rc = device_sm_count(&sms);
-  if (rc != KF_OK) return rc > 0 ? KF_ERR_UNSUPPORTED : rc;
-  const int64_t split = bwd_split(Hq, Hk, n_k_tiles, sms);
-  return bwd_stat_bytes(Hq, n_q_tiles) + (split > 1 ? split * n_k_tiles * Hk * 2 * PB_T * PB_D * 4 : 0);
+  kf_attn_pack_params p{};
+  p.Hq = Hq; p.Hk = Hk; p.n_q_tiles = n_q_tiles;
+  return bwd_ws_bytes(&p, n_k_tiles);
+}
+
+extern "C" int64_t kf_attn_pack_bwd_ws_bytes(const kf_attn_pack_params* p) {
+  const int rc = check_pack(p);
+  return rc != KF_OK ? rc : bwd_ws_bytes(p, wants_keys(p) ? p->n_k_tiles : 0);
 }
 
 extern "C" int kf_attn_pack_bwd(const kf_attn_pack_params* p, void* stream) {
   int rc = check_pack(p);
   if (rc != KF_OK) return rc;
   if (p->n_q_tiles == 0 && p->n_k_tiles == 0) return KF_OK;
-  // (dq alone: the first launch)
   constexpr float LOG2E = 1.4426950408889634f;
   kf_heads q{}, k{}, v{}, o{}, go{}, gq{}, gk{}, gv{};
-  const bool any_q = p->n_q_tiles > 0, any_k = p->n_k_tiles > 0 && (p->dk.ptr || p->dv.ptr);
+  const bool any_q = p->n_q_tiles > 0, any_k = p->n_k_tiles > 0 && wants_keys(p);
   KF_REQUIRE((!any_q || (p->Tq > 0 && p->q_tiles && p->lse)) && (!any_k || (p->Tk > 0 && p->k_tiles)), "kf_attn_pack_bwd: null pointer");
   if (p->Tq > 0) {
     if ((rc = check_heads("q", p->q, p->Tq, p->Hq, &q)) != KF_OK) return rc;
@@ -739,7 +763,7 @@ extern "C" int kf_attn_pack_bwd(const kf_attn_pack_params* p, void* stream) {
     if (any_k && (rc = check_heads("dk", p->dk, p->Tk, p->Hk, &gk)) != KF_OK) return rc;
     if (any_k && (rc = check_heads("dv", p->dv, p->Tk, p->Hk, &gv)) != KF_OK) return rc;
   }
-  const int64_t need = kf_attn_pack_ws_bytes(p->Hq, p->Hk, p->n_q_tiles, any_k ? p->n_k_tiles : 0);
+  const int64_t need = bwd_ws_bytes(p, any_k ? p->n_k_tiles : 0);
   if (need < 0) return (int)need;
   KF_REQUIRE(p->ws && (reinterpret_cast<uintptr_t>(p->ws) & 31) == 0 && p->ws_bytes >= need, "kf_attn_pack_bwd: workspace of %lld bytes, needs %lld, 32-byte aligned",
              (long long)p->ws_bytes, (long long)need);
@@ -787,7 +811,7 @@ extern "C" int kf_attn_pack_bwd(const kf_attn_pack_params* p, void* stream) {
   }
   if (any_k) {
     a.tiles = reinterpret_cast<const int4*>(p->k_tiles);
-    a.split = bwd_split(p->Hq, p->Hk, p->n_k_tiles, sms);
+    a.split = bwd_split(p, p->n_k_tiles, sms);
     a.heads = p->Hk * a.split;
     a.n_items = p->n_k_tiles * a.heads;
     a.parts = static_cast<float*>(p->ws) + bwd_stat_bytes(p->Hq, p->n_q_tiles) / 4;

@@ -424,10 +424,10 @@ class AttnPlan:
 
     A record per 128 rows of queries and of keys, the longest work first: the kernels' CTAs take them in turn."""
 
-    __slots__ = ("q_rows", "k_rows", "longest", "causal", "q_tiles", "k_tiles")
+    __slots__ = ("q_rows", "k_rows", "longest", "k_work", "k_longest", "causal", "q_tiles", "k_tiles")
 
     def __init__(self, q_lens, k_lens=None, *, causal: bool = False, prefix=None, device="cuda"):
-        table, n, self.q_rows, self.k_rows, self.longest = _h.attn_plan(q_lens, k_lens, causal, prefix)
+        table, n, self.q_rows, self.k_rows, self.longest, self.k_work, self.k_longest = _h.attn_plan(q_lens, k_lens, causal, prefix)
         self.causal = bool(causal)
         table = table.to(device)
         self.q_tiles, self.k_tiles = table[:n], table[n:]
@@ -457,7 +457,7 @@ def attn_packed_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
     gradient).  q and dout inside a sequence have to be finite as k and v.  grads: tensors to write instead of new ones, e.g. the parts of one
     projection's gradient; they may not overlap one another or what the call reads.  f16 gradients have the range of f16: scale the loss as for any
     f16 product.  No atomics: the same bits from run to run."""
-    return _counted("attn_packed_bwd", _h.attn_packed_bwd, (*_pack_args(q, k, v, plan, scale, cap, slopes), dout, out, lse, *grads, keys))
+    return _counted("attn_packed_bwd", _h.attn_packed_bwd, (*_pack_args(q, k, v, plan, scale, cap, slopes), dout, out, lse, *grads, keys, plan.k_work, plan.k_longest))
 
 
 # ------------------------------------------------------------------------------------------------ patch embed / head / pre / post

@@ -67,8 +67,8 @@ def test_gradients_of_queries_alone(heads):
 
     g = torch.Generator(device="cuda").manual_seed(1)
     r = lambda *s: torch.randn(*s, generator=g, device="cuda").to(BF)  # noqa: E731
-    q, k, v, do = r(300, heads[0], 64), r(300, heads[1], 64), r(300, heads[1], 64), r(300, heads[0], 64)
-    plan = ops.AttnPlan([170, 130], causal=True)
+    q, k, v, do = r(500, heads[0], 64), r(500, heads[1], 64), r(500, heads[1], 64), r(500, heads[0], 64)
+    plan = ops.AttnPlan([370, 130], causal=True)
     out, lse = ops.attn_packed(q, k, v, plan, cap=20.0)
     want = ops.attn_packed_bwd(do, q, k, v, out, lse, plan, cap=20.0)
     with torch.enable_grad():
@@ -111,3 +111,44 @@ def test_gradients_of_rows_alone(R, d):
             assert ops.LAUNCHES - before == (0 if R == 0 else 2 if any(need[1:]) else 1)
             assert [t.grad is not None for t in leaves] == list(need)
     ops.check_device_error()
+
+
+CHOICES = [([1605], 16, 1, False, 3), ([1605] * 8, 16, 1, True, 3), ([130] * 20, 16, 1, False, 2), ([130] * 60, 16, 1, False, 2), ([130] * 60, 16, 1, True, 2), ([130] * 150, 8, 1, False, 2),
+           ([1605], 12, 4, True, 3), ([1605] * 4, 12, 4, True, 2), ([130] * 60, 12, 4, True, 2), ([1029, 261, 517, 2053, 133, 1, 1605, 711, 64, 129], 12, 4, True, 3), ([200], 16, 8, False, 2)]
+
+
+@gpu
+@pytest.mark.parametrize("lens,Hq,Hk,causal,kernels", CHOICES, ids=lambda v: f"{len(v)}x{max(v)}" if isinstance(v, list) else str(v))
+def test_shared_key_heads_are_split_where_that_is_shorter(lens, Hq, Hk, causal, kernels):
+    """the choices of the second launch on 148 SMs, and the workspace that goes with them: 64 KB per key tile and query head of a split, which only batches of few items are"""
+    from lightly_trian_quant_b200 import ops
+
+    if torch.cuda.get_device_properties(0).multi_processor_count != 148:
+        pytest.skip("the choice depends on the number of SMs")
+    q, k = torch.zeros(sum(lens), Hq, 64, dtype=BF, device="cuda"), torch.zeros(sum(lens), Hk, 64, dtype=BF, device="cuda")
+    plan = ops.AttnPlan(lens, causal=causal)
+    out, lse = ops.attn_packed(q, k, k, plan)
+    before = ops.LAUNCHES
+    ops.attn_packed_bwd(q, q, k, k, out, lse, plan)
+    ops.check_device_error()
+    assert ops.LAUNCHES - before == kernels
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, torch.float16])
+def test_split_and_whole_key_heads_against_the_same_reference(dtype):
+    """a plan that does not know its lengths splits wherever every query head finds an SM"""
+    from lightly_trian_quant_b200 import ops
+    from tests.test_attn_pack_gpu import NAMES, case, close, reference, run
+
+    lens, Hq, Hk = [130] * 9, 4, 1
+    q, k, v, do = case(lens, lens, Hq, Hk, dtype, 41)
+    ref = reference(q, k, v, do, lens, lens, True, None, 0.125, 0.0, None, dtype)
+    plan = ops.AttnPlan(lens, causal=True)
+    assert plan.k_longest == 130 and plan.k_work == 9 * 132
+    for known, kernels in ((True, 2), (False, 3)):
+        if not known:
+            plan.k_work = plan.k_longest = 0
+        before = ops.LAUNCHES
+        close(run(q, k, v, do, plan), ref, NAMES)
+        assert ops.LAUNCHES - before == 1 + kernels
