@@ -14,7 +14,8 @@ gpu = pytest.mark.gpu
 # rows so many that on 148 SMs with at most 4 CTAs each every group of warps takes 5 rows or more (slots and phases come round twice), in every
 # number of warps per row (forward 1 up to 1024 wide, 2 up to 2048, 4 up to 4096, 8; backward 1 up to 512, 2 up to 1024, 4 up to 2048, 8), both widths of access
 CASES = [(40009, 333, BF, BF), (24001, 512, F16, F32), (23700, 77, F32, F32), (24003, 1024, F32, BF), (24005, 1000, F16, F16), (12001, 2048, F32, BF), (12003, 1999, BF, F32), (6007, 4096, BF, BF),
-         (6007, 3001, F32, F16), (3001, 8192, BF, F32), (3003, 8191, BF, BF)]
+         (6007, 3001, F32, F16), (3001, 8192, BF, F32), (3003, 8191, BF, BF),
+         (24007, 397, BF, BF), (24001, 603, F32, BF), (24007, 801, F16, F32), (12007, 1001, BF, BF), (12001, 1201, F32, F32), (12005, 1601, BF, F16), (6001, 3501, F16, F16), (3007, 5001, F32, BF)]
 
 
 def _check_norm(x, w, b, ty, dy, dres, y, dx, dw, db):

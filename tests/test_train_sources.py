@@ -50,3 +50,19 @@ def test_rotary_positions_have_no_kernel_that_nothing_reaches():
     assert {v for t, v, _ in kernels if t.startswith("f")} == {"1", "2", "4"}
     assert {v for t, v, _ in kernels if not t.startswith("f")} == {"1", "2", "4", "8"}
     assert ("ff", "1", "1") not in kernels                       # pairs side by side need two values at once
+
+
+def test_layer_norm_has_a_step_near_every_width():
+    """values per lane are compiled in steps, and empty places of a step cost as much as full ones: no width pays for more than twice its own and two"""
+    code = _code("kf_norm.cu")
+    body = code[code.index("static int ln_by_width"):]
+    body = body[:body.index("\n}\n")]
+    body = body[body.index("const int n = (d + lanes - 1)"):]
+    steps = [int(n) for n in re.findall(r"std::integral_constant<int, 1>\{\}, std::integral_constant<int, (\d+)>", body)]
+    assert steps == sorted(steps) and [int(n) for n in re.findall(r"if \(n <= (\d+)\)", body)] == steps[:-1]
+    for backward, warps in ((False, ((1024, 1), (2048, 2), (4096, 4), (8192, 8))), (True, ((512, 1), (1024, 2), (2048, 4), (8192, 8)))):
+        for d in range(1, 8193):
+            lanes = 32 * next(w for most, w in warps if d <= most)
+            n = -(-d // lanes)
+            step = next(s for s in steps if n <= s)
+            assert step <= 2 * n + 2, (backward, d, n, step)
