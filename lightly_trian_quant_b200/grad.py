@@ -33,9 +33,10 @@ def _eager(*tensors) -> None:
         _eager_backward(tensors[0])
 
 
-def _rows(g: torch.Tensor) -> torch.Tensor:
-    """a gradient as the kernels take it: contiguous (autograd may hand on expanded or permuted ones)"""
-    return g if g.is_contiguous() else g.contiguous()
+def _rows(g: torch.Tensor, align: int = 1) -> torch.Tensor:
+    """a gradient as the kernels take it: contiguous, at a multiple of `align` bytes (autograd hands on expanded and permuted ones, and views of others at any offset)"""
+    g = g if g.is_contiguous() else g.contiguous()
+    return g if g.data_ptr() % align == 0 else g.clone()
 
 
 class _LayerNorm(torch.autograd.Function):
@@ -66,7 +67,7 @@ class _RopeAxes(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         _eager_backward(dy)
-        return ops.rope_axes(_rows(dy), *ctx.saved_tensors, ctx.table, inverse=True), None, None
+        return ops.rope_axes(_rows(dy, 2 * dy.element_size() if ctx.table.interleaved else 1), *ctx.saved_tensors, ctx.table, inverse=True), None, None
 
 
 class _AttnPacked(torch.autograd.Function):
@@ -83,7 +84,7 @@ class _AttnPacked(torch.autograd.Function):
         q, k, v, out, lse, slopes = ctx.saved_tensors
         plan, scale, cap = ctx.how
         _eager_backward(q)
-        return (*ops.attn_packed_bwd(_rows(dout), q, k, v, out, lse, plan, scale=scale, cap=cap, slopes=slopes, keys=any(ctx.needs_input_grad[1:3])), None, None, None, None)
+        return (*ops.attn_packed_bwd(_rows(dout, 16), q, k, v, out, lse, plan, scale=scale, cap=cap, slopes=slopes, keys=any(ctx.needs_input_grad[1:3])), None, None, None, None)
 
 
 def layer_norm(x: torch.Tensor, w: torch.Tensor, b: Optional[torch.Tensor], eps: float, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
