@@ -36,7 +36,11 @@ constexpr int PK_KV = 3;
 constexpr int PK_QTILE = PK_BM * PK_D * 2, PK_KTILE = PK_BN * PK_D * 2;
 constexpr int PK_OFF_K = 2 * PK_QTILE, PK_OFF_V = PK_OFF_K + PK_KV * PK_KTILE, PK_OFF_BAR = PK_OFF_V + PK_KV * PK_KTILE;
 constexpr size_t PK_SMEM = (size_t)PK_OFF_BAR + 256;
-constexpr float PK_SUM_LIMIT = 32768.f;
+// P is 2^shift times the weight relative to the running maximum, which stays as it is while a tile's sum keeps to the limit (and with it each P to f16's range).  In f16
+// weights far below the maximum would lose their digits (one key and 400 002 others that weigh as much together: 2.2 % off), and with 2^8 rows that start with few keys, as causal
+// ones do, leave the limit too often (capped f16 clips 49.4 -> 53.4 us).
+__host__ __device__ constexpr float pk_shift(int f16) { return f16 ? 6.f : 0.f; }
+__host__ __device__ constexpr float pk_sum_limit(int f16) { return f16 ? 65504.f : 32768.f; }
 constexpr int PK_POLY_K = 3;                           // element pairs PK_POLY_K .. 3 of every four take the polynomial exponential
 constexpr int PK_SBUF = 2;
 constexpr int PK_TMEM_COLS = 256, PK_COL_O = PK_SBUF * PK_BN;
@@ -322,6 +326,7 @@ attn_pack_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     constexpr bool RAW = !CAP && !BIAS;                          // the registers hold raw products: the scale is applied with the maximum
     const float sc = RAW ? a.scale_log2 : 1.f;
     const float2 sc2 = splat2(sc);
+    constexpr float SHIFT = pk_shift(F16);
     bool ok = true;
     uint32_t buf = 0, sph = 0;
     auto exp_half = [&](const uint32_t (&r)[32], uint32_t* w, float2 mn2, float2& s0, float2& s1) {
@@ -436,7 +441,7 @@ attn_pack_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         if (!BIAS && m_run == -INFINITY) m_run = 0.f;            // a row that sees nothing
       }
       const bool unseen = BIAS && m_run == -INFINITY;            // none of its keys so far
-      const float2 mn2 = splat2(unseen ? 0.f : -m_run * sc);
+      const float2 mn2 = splat2(unseen ? 0.f : fmaf(-m_run, sc, SHIFT));
       float2 s0 = make_float2(0.f, 0.f), s1 = s0;
       uint32_t w[48];
       exp_half(ra, w, mn2, s0, s1);
@@ -451,7 +456,7 @@ attn_pack_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       exp_half(rc, w + 32, mn2, s0, s1);
       if (prefetch) tmem_ld32(t_lane + buf * PK_BN + 64, rc);
       float sum = (s0.x + s0.y) + (s1.x + s1.y), alpha = 1.f;
-      const bool need = lim >= 0 && (!(sum <= PK_SUM_LIMIT) || (unseen && lim > 0));   // rows that are not stored go on with whatever they have
+      const bool need = lim >= 0 && (!(sum <= pk_sum_limit(F16)) || (unseen && lim > 0));   // rows that are not stored go on with whatever they have
       if (__any_sync(0xffffffffu, need)) {
         uint32_t r[32];
         float mx = m_run;
@@ -467,7 +472,7 @@ attn_pack_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
           alpha = ex2((m_run - mx) * sc);
           m_run = mx;
         }
-        const float2 mn = splat2(BIAS && m_run == -INFINITY ? 0.f : -m_run * sc);
+        const float2 mn = splat2(BIAS && m_run == -INFINITY ? 0.f : fmaf(-m_run, sc, SHIFT));
         s0 = s1 = make_float2(0.f, 0.f);
 #pragma unroll 1
         for (int c = 0; c < PK_BN / 32; ++c) {
@@ -556,7 +561,7 @@ attn_pack_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         uint8_t* dst = static_cast<uint8_t*>(a.O) + 2 * ((int64_t)(tile.row + row) * a.o_st + (int64_t)h * a.o_sh);
 #pragma unroll
         for (int i = 0; i < 4; ++i) store32(dst + 32 * i, w + 8 * i);
-        a.lse[(int64_t)h * a.lse_ld + tile.row + row] = none ? -INFINITY : (m_run * sc + log2f(l_run)) * 0.6931471805599453f;
+        a.lse[(int64_t)h * a.lse_ld + tile.row + row] = none ? -INFINITY : (fmaf(m_run, sc, -SHIFT) + log2f(l_run)) * 0.6931471805599453f;
       }
     }
     }   // items
@@ -599,7 +604,7 @@ attn_pack_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                              : make_uint4(pack16(o[0] * inv, o[1] * inv, F16), pack16(o[2] * inv, o[3] * inv, F16), pack16(o[4] * inv, o[5] * inv, F16), pack16(o[6] * inv, o[7] * inv, F16));
         uint8_t* dst = static_cast<uint8_t*>(a.O) + 2 * ((int64_t)(tile.row + r) * a.o_st + (int64_t)h * a.o_sh);
         reinterpret_cast<uint4*>(dst)[c] = w;
-        if (c == 0) a.lse[(int64_t)h * a.lse_ld + tile.row + r] = none ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+        if (c == 0) a.lse[(int64_t)h * a.lse_ld + tile.row + r] = none ? -INFINITY : (m - pk_shift(F16) + log2f(l)) * 0.6931471805599453f;
       }
     }
     }

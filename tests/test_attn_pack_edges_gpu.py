@@ -236,3 +236,34 @@ def test_a_chain_of_the_operators_in_every_launch_mode(mode):
     for _ in range(20):
         assert all(torch.equal(a, b) for a, b in zip(step(), want))
     ops.check_device_error()
+
+
+# ------------------------------------------------------------------------------------------------ many small weights beside a large one in f16
+@gpu
+@pytest.mark.parametrize("cap,bias", [(0.0, False), (60.0, False), (0.0, True)])
+@pytest.mark.parametrize("split", [True, False])
+def test_f16_weights_far_below_the_largest(split, cap, bias):
+    """the first key weighs about as much as 400 002 others together, each at 20.5 steps of 2^-24 of it: f16 weights relative to the largest would lose a fortieth of each, the same
+    way.  Tolerance: weights and output rounded once by u = 2^-11, the exponents to 2e-5 (scores of 13.6, the cap's 60 * 2^-22).  The products are summed 16 keys at a time in fp32 without rounding to nearest: each of the n = 25 000 additions may cut
+2^-23 of a sum that grows evenly, n / 2 * 2^-23 = 1.5e-3 in all (an eighth of it where eight CTAs share the keys).  The weights' own sum takes 96 keys at a time, rounded to nearest, with equal terms the same way over long
+stretches: 4167 / 2 * 2^-24 = 1.2e-4 of the sum, and so of the log-sum-exp."""
+    ops = _ops()
+    Lq, Lk, u = 3, 400003, 2.0 ** -11
+    q, k = torch.zeros(Lq, 1, 64, dtype=F16, device="cuda"), torch.zeros(Lk, 1, 64, dtype=F16, device="cuda")
+    v = torch.ones(Lk, 1, 64, dtype=F16, device="cuda")
+    q[..., 0], k[0, 0, 0], v[0] = 8, 13.615, 0
+    if cap:
+        k[0, 0, 0] = cap * math.atanh(13.615 / cap)
+    slopes = torch.zeros(1, device="cuda") if bias else None
+    plan = ops.AttnPlan([Lq], [Lk])
+    if not split:
+        plan.longest = 0
+    out, lse = ops.attn_packed(q, k, v, plan, cap=cap, slopes=slopes)
+    ops.check_device_error()
+    s = k[0, 0, 0].double().item()
+    s = cap * math.tanh(s / cap) if cap else s
+    total = math.exp(s) + Lk - 1
+    want = (Lk - 1) / total
+    sums = Lk / 16 / 2 * 2.0 ** -23 / (8 if split else 1)
+    assert (out.double() - want).abs().max() <= (2 * u + 2e-5 + sums) * want, (out.double() / want - 1).abs().max()
+    assert (lse.double() - math.log(total)).abs().max() <= 2e-5 + Lk / 96 / 2 * 2.0 ** -24 / (8 if split else 1)
