@@ -274,6 +274,7 @@ KF_API int64_t kf_launch_count(void);
 
 /* LayerNorm that keeps each row's statistics: x [rows, d] (row stride ldx elements; f32 | bf16 | f16) -> y [rows, d] contiguous
  * (f32 | bf16 | f16), mean and rstd fp32 [rows].  w fp32 [d], b fp32 [d] or NULL.  d from 1 to 8192.
+ * Rows are read in whole 16-byte units: up to 15 bytes in front of and behind a tensor that starts or ends inside one are read too (never past its allocation).
  * Statistics and products in fp32; no counterpart kernel in the reference, whose training runs nn.LayerNorm
  * (src/lightly_train/_models/dinov3/dinov3_src/models/vision_transformer.py:44). */
 KF_API int kf_layer_norm_fwd(int in_dtype, const void* x, int64_t ldx, const float* w, const float* b, float eps, int rows, int d, int out_dtype,
@@ -296,7 +297,7 @@ KF_API int kf_layer_norm_bwd(int in_dtype, const void* x, int64_t ldx, int dy_dt
 
 /* Rotary positions with several axes: x [G, T, H, D] -> y, the first 2P channels of every head turned by
  * angle(t, p) = pos[t, axis[p]] * freq[p] * pi, the others copied.  Pair p: channels (p, p + P), or (2p, 2p + 1) with interleaved != 0.
- * inverse != 0 turns by the negative angle, which is the gradient.  y may be x.  P <= 128, D <= 256.
+ * inverse != 0 turns by the negative angle, which is the gradient.  y may be x.  P <= 128, D <= 256.  Angles are products in fp64: off by 2^-52 of their size.
  * Counterpart of the turn itself: apply_rope (src/lightly_train/_models/dinov3/dinov3_src/layers/attention.py:23-34). */
 typedef struct kf_rope_params {
   const void* x;         /* f32 | bf16 | f16, channels contiguous                                  */

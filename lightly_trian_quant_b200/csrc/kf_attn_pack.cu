@@ -18,8 +18,9 @@
 //   - the polynomial exponential is a degree finer, for the log-sum-exp, and 0 for masked keys
 //   - few items over long keys (SPLIT): a cluster of up to eight CTAs takes an item, each a share of the key tiles, and joins its parts through the
 //     shared memory of its CTAs: accumulators, maxima and sums in fp32, in the order of the parts
-// Measured (16 heads, bf16 unless noted): 8 x 1605 tokens 127 us (0.66 PFLOP/s), sizes of 1 to 4101 tokens 147, a causal clip of 8197 tokens in f16 191; bound by
-// the softmax' instructions, two warps per scheduler
+// Measured (16 heads, bf16 unless noted): 8 x 1605 tokens 124.6 us (0.68 PFLOP/s), sizes of 1 to 4101 tokens 143, a causal clip of 8197 tokens in f16 187.  No unit is full
+// (8 x 1605, cold: issue slots 50 %, exponential unit 53 %, FMA pipes 39 %, tensor cores 33 %): the two softmax warps of a scheduler wait for tensor memory and for
+// their own instructions, one after the other in each step
 #include <cfloat>
 #include <type_traits>
 

@@ -6,8 +6,8 @@
 // Two launches of one kernel, which share the mathematics and differ in what stays and what passes by:
 //   ROWS = queries  a CTA keeps 128 queries (Q, dO) and goes through key tiles (K, V):        dQ
 //   ROWS = keys     a CTA keeps 128 keys (K, V) and goes through query tiles (Q, dO) of every head that shares them:   dK, dV
-// S and dP are computed in both (7 products where one pass over the pairs takes 5): each gradient is then summed in one place, in tensor
-// memory, in a fixed order.  One pass would add dQ from every key tile to memory by atomics, 32 KB per pair of tiles, in an order that changes
+// S and dP are computed in both (8 products, the one for delta below among them, where one pass over the pairs takes 5): each gradient is then summed in one place, in
+// tensor memory, in a fixed order.  One pass would add dQ from every key tile to memory by atomics, 32 KB per pair of tiles, in an order that changes
 // from run to run.
 //
 //   CTA      one per SM, persistent over (tile, head) items, the longest first; steps of 96 passing rows
@@ -25,7 +25,8 @@
 //   numerics P and dS are rounded to the 16-bit type of the operands (the products' A operand); everything else fp32.  With f16 P is 2^14 times what it is, by the
 //            exponent's offset: probabilities of long rows lie below f16's normal range (at 818 401 keys dV was 2.4 % off, the same way in every row).  Delta and dP take
 //            the power of two back in front of dS, by the multiplication that was an addition; dV and the product P K at the end.
-//   measured 8 x 1605 tokens, 16 heads, bf16: first launch 165 us, second 178; issue slots 57 and 53 % busy, tensor cores 43 %, special-function unit 50 and 38 %
+//   measured 8 x 1605 tokens, 16 heads, bf16: first launch 162 us, second 177 (0.83 and 0.76 PFLOP/s of the four products of each); cold, issue slots 53 and 47 % busy,
+//            tensor cores 52 and 47 %, special-function unit 50 and 53 %: warps wait for tensor memory, with ROWS = keys for shared memory too
 #include "kf_attn.cuh"
 
 namespace kf {

@@ -407,7 +407,8 @@ class RopeTable:
 def rope_axes(x: torch.Tensor, pos: torch.Tensor, table: RopeTable, *, inverse: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x [T, H, D] or [G, T, H, D] (f32 | bf16 | f16, channels contiguous, any other strides; interleaved pairs at even ones) with every head turned by
     its token's positions pos [T, axes] (int32 | int64 | fp32).  inverse=True turns back, which is also the gradient.  out may be x, but not overlap it
-    otherwise.  Tokens that are not to be turned (cls, registers, queries) have position 0.  Angles are exact to fp32 however far the position."""
+    otherwise.  Tokens that are not to be turned (cls, registers, queries) have position 0.  Angles are products in fp64, off by 2^-52 of their size: up to 10^8 radians
+    less than a rounding of their sine to fp32."""
     global LAUNCHES
     LAUNCHES += 1
     args = (x, pos, table.freq, table.axis, table.axes, table.head_dim, table.interleaved, inverse, out)
@@ -440,9 +441,9 @@ def _pack_args(q, k, v, plan: AttnPlan, scale, cap, slopes) -> tuple:
 def attn_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: AttnPlan, *, scale: Optional[float] = None, cap: float = 0.0,
                 slopes: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None):
     """Attention over packed sequences: q [Tq, Hq, 64], k, v [Tk, Hk, 64] (bf16 | f16, Hq a multiple of Hk; channels contiguous, 16-byte aligned rows
-    and heads with any strides, e.g. parts of one projection) -> (out [Tq, Hq, 64], lse fp32 [Hq, Tq]).
+    and heads at strides of 64 elements or more, in any order, e.g. parts of one projection) -> (out [Tq, Hq, 64], lse fp32 [Hq, Tq]).
 
-    score = scale * q . k (scale 1/8 by default), then cap * tanh(score / cap) with cap > 0, then minus slopes[head] * |distance| (fp32 [Hq]);
+    score = scale * q . k (scale 1/8 by default), then cap * tanh(score / cap) with cap > 0 (one that fp32 cannot hold is refused), then minus slopes[head] * |distance| (fp32 [Hq]);
     plan says which keys a query sees.  A query that sees nothing gets 0 and -inf.  Rows behind the last sequence: zero in new tensors, left as they
     were in a given out, which may not overlap q, k or v.  Keys and values inside a sequence have to be finite; rows outside the sequences may hold anything."""
     global LAUNCHES
