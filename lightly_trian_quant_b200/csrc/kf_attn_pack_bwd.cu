@@ -25,7 +25,7 @@
 //   numerics P and dS are rounded to the 16-bit type of the operands (the products' A operand); everything else fp32.  With f16 P is 2^14 times what it is, by the
 //            exponent's offset: probabilities of long rows lie below f16's normal range (at 818 401 keys dV was 2.4 % off, the same way in every row).  Delta and dP take
 //            the power of two back in front of dS, by the multiplication that was an addition; dV and the product P K at the end.
-//   measured 8 x 1605 tokens, 16 heads, bf16: first launch 162 us, second 177 (0.83 and 0.76 PFLOP/s of the four products of each); cold, issue slots 53 and 47 % busy,
+//   measured 8 x 1605 tokens, 16 heads, bf16: first launch 162 us, second 177 (four products in each: 1.04 and 0.95 PFLOP/s); cold, issue slots 53 and 47 % busy,
 //            tensor cores 52 and 47 %, special-function unit 50 and 53 %: warps wait for tensor memory, with ROWS = keys for shared memory too
 #include "kf_attn.cuh"
 
