@@ -445,7 +445,10 @@ def attn_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: AttnPla
 
     score = scale * q . k (scale 1/8 by default), then cap * tanh(score / cap) with cap > 0 (one that fp32 cannot hold is refused), then minus slopes[head] * |distance| (fp32 [Hq]);
     plan says which keys a query sees.  A query that sees nothing gets 0 and -inf.  Rows behind the last sequence: zero in new tensors, left as they
-    were in a given out, which may not overlap q, k or v.  Keys and values inside a sequence have to be finite; rows outside the sequences may hold anything."""
+    were in a given out, which may not overlap q, k or v.  Keys and values inside a sequence have to be finite; rows outside the sequences may hold anything.
+
+    The same batch gives the same bits every time.  A sequence in another batch may differ by roundings: few items are split along their keys, and with a cap which
+    of two formulas (both to 1e-7 of the cap) a piece of scores takes is decided for 32 rows at once, those behind the sequence's end among them."""
     global LAUNCHES
     LAUNCHES += 1
     args = (*_pack_args(q, k, v, plan, scale, cap, slopes), out)
